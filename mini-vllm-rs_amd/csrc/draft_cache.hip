@@ -1,0 +1,281 @@
+// The cache side of drafted trees for gfx950 (MI355X, CDNA4): norm, rotation and
+// append of new rows, compaction of an accepted path, copies of pages.
+//
+// All three move rows once: they are bound by HBM where a call has many rows,
+// and by the chain of dependent table loads (request, lengths, page, row) where
+// it has few.
+#include "draft_cache.hpp"
+
+#include <math.h>
+
+namespace mvr {
+namespace {
+
+typedef _Float16 half_t;
+typedef half_t half4 __attribute__((ext_vector_type(4)));
+typedef float float4v __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(4))) int32_t const_i32;
+
+constexpr int kThreads = 256;
+constexpr int kWave = 64;
+constexpr int kItem = 8; // elements (4 rotation pairs) per thread
+
+__device__ __forceinline__ float4v load4(const float* p) { return *reinterpret_cast<const float4v*>(p); }
+__device__ __forceinline__ float4v load4(const half_t* p) {
+  return __builtin_convertvector(*reinterpret_cast<const half4*>(p), float4v);
+}
+__device__ __forceinline__ void store4(float* p, float4v v) { *reinterpret_cast<float4v*>(p) = v; }
+__device__ __forceinline__ void store4(half_t* p, float4v v) {
+  *reinterpret_cast<half4*>(p) = __builtin_convertvector(v, half4);
+}
+
+// Entries of the ascending table cu[0 .. count) that are <= n, by a search with
+// one entry per lane and round (one round up to 64 entries).
+__device__ __forceinline__ int entries_up_to(const int32_t* cu, int count, int n) {
+  const int l = __lane_id();
+  int lo = 0, len = count; // the answer is in [lo, lo + len]
+  while (len > kWave) {
+    const int step = (len + kWave - 1) / kWave;
+    const int at = lo + l * step;
+    const int below = __popcll(__ballot(at < lo + len && cu[min(at, lo + len - 1)] <= n)); // probes that are <= n
+    if (below == 0) return lo;
+    const int end = lo + len;
+    lo += (below - 1) * step;
+    len = min(step, end - lo);
+  }
+  return lo + __popcll(__ballot(l < len && cu[lo + min(l, len - 1)] <= n));
+}
+
+// Norm, rotation and append.  One block row (blockIdx.x) per packed token, a
+// group of 2^k >= D/8 lanes per row, 8 elements (the 4 pairs they rotate as) per
+// lane: the row's mean square is a butterfly over its lanes, and nothing is
+// read twice.  Row = query heads, then KV heads for K, then for V.
+template <typename T, int ROPE>
+__global__ __launch_bounds__(kThreads) void norm_rope_append_kernel(NormRopeAppendParams p, int lanes_log2) {
+  const int n = blockIdx.x;
+  const int D = p.head_dim, lanes = 1 << lanes_log2;
+  const int row = (blockIdx.y * kThreads + threadIdx.x) >> lanes_log2;
+  const int j = threadIdx.x & (lanes - 1);
+  const int rows = p.num_q_heads + 2 * p.num_kv_heads;
+  const bool active = row < rows && j < D / kItem;
+  const int kind = row < p.num_q_heads ? 0 : row < p.num_q_heads + p.num_kv_heads ? 1 : 2; // Q, K, V
+  const int h = kind == 0 ? row : kind == 1 ? row - p.num_q_heads : row - p.num_q_heads - p.num_kv_heads;
+  // The lane's pairs are (lo[e], hi[e]) (Neox), or the neighbours in lo, hi.
+  const int lo_off = kind == 2 || ROPE == 1 ? kItem * j : 4 * j;
+  const int hi_off = kind == 2 || ROPE == 1 ? kItem * j + 4 : D / 2 + 4 * j;
+  // The row first: its latency overlaps the chain of table loads below.
+  float4v lo = {0.f, 0.f, 0.f, 0.f}, hi = lo, wlo = {1.f, 1.f, 1.f, 1.f}, whi = wlo;
+  const T* weight = static_cast<const T*>(kind == 0 ? p.q_weight : kind == 1 ? p.k_weight : nullptr);
+
+  int b = 0, q_start = 0, q_len = p.total_q;
+  if (p.cu_q_lens) {
+    // The request that holds token n: empty requests before it share its start.
+    b = __builtin_amdgcn_readfirstlane(entries_up_to(p.cu_q_lens, p.num_seqs + 1, n)) - 1;
+    if (b < 0 || b >= p.num_seqs) return; // behind the last request (a padded batch)
+    const const_i32* cu = (const const_i32*)p.cu_q_lens;
+    q_start = cu[b];
+    q_len = cu[b + 1] - q_start;
+  }
+  if (active) {
+    const T* src = kind == 0 ? static_cast<const T*>(p.q) + h * p.q_stride_head + n * p.q_stride_token
+                 : kind == 1 ? static_cast<const T*>(p.k) + h * p.k_stride_head + n * p.k_stride_token
+                             : static_cast<const T*>(p.v) + h * p.v_stride_head + n * p.v_stride_token;
+    lo = load4(src + lo_off);
+    hi = load4(src + hi_off);
+    if (weight) {
+      wlo = load4(weight + lo_off);
+      whi = load4(weight + hi_off);
+    }
+  }
+  const int seq_len = p.seq_lens ? ((const const_i32*)p.seq_lens)[b] : p.max_seq_len;
+  const int slot = seq_len - q_len + (n - q_start);
+  const int pos = p.positions ? ((const const_i32*)p.positions)[n] : slot;
+  // Only tables that break the contract hold such values: nothing is written.
+  if (slot < 0 || slot >= p.max_seq_len || pos < 0 || pos >= p.rope_len) return;
+  const int64_t page = ((const const_i32*)p.block_tables)[(int64_t)b * p.block_table_stride + slot / p.page_size];
+  if (page < 0 || page >= p.num_pages) return;
+
+  if (weight) {
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; e++) ss = fmaf(lo[e], lo[e], fmaf(hi[e], hi[e], ss));
+    for (int off = lanes >> 1; off >= 1; off >>= 1) ss += __shfl_xor(ss, off);
+    const float inv = 1.f / sqrtf(ss / (float)D + p.eps);
+    lo = lo * inv * wlo;
+    hi = hi * inv * whi;
+  }
+  if (!active) return;
+  const int64_t at = ((page * p.num_kv_heads + h) * p.page_size + slot % p.page_size) * D;
+  T* dst = kind == 0 ? static_cast<T*>(p.q_out) + h * p.q_out_stride_head + n * p.q_out_stride_token
+         : kind == 1 ? static_cast<T*>(p.key_pool) + at
+                     : static_cast<T*>(p.value_pool) + at;
+  if (kind != 2) {
+    const float4v c = load4(static_cast<const T*>(p.cos_table) + (int64_t)pos * (D / 2) + 4 * j);
+    const float4v s = load4(static_cast<const T*>(p.sin_table) + (int64_t)pos * (D / 2) + 4 * j);
+    float4v ylo, yhi;
+    if (ROPE == 0) {
+      ylo = lo * c - hi * s;
+      yhi = lo * s + hi * c;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        ylo[2 * e] = lo[2 * e] * c[e] - lo[2 * e + 1] * s[e];
+        ylo[2 * e + 1] = lo[2 * e] * s[e] + lo[2 * e + 1] * c[e];
+        yhi[2 * e] = hi[2 * e] * c[e + 2] - hi[2 * e + 1] * s[e + 2];
+        yhi[2 * e + 1] = hi[2 * e] * s[e + 2] + hi[2 * e + 1] * c[e + 2];
+      }
+    }
+    lo = ylo;
+    hi = yhi;
+  }
+  store4(dst + lo_off, lo);
+  store4(dst + hi_off, hi);
+}
+
+template <typename T>
+hipError_t launch_append(const NormRopeAppendParams& p, int rope_type, hipStream_t stream) {
+  int lanes_log2 = 0;
+  while ((1 << lanes_log2) < p.head_dim / kItem) lanes_log2++;
+  const int rows = p.num_q_heads + 2 * p.num_kv_heads, per_block = kThreads >> lanes_log2;
+  const dim3 grid((unsigned)p.total_q, (unsigned)((rows + per_block - 1) / per_block));
+  if (rope_type == 0)
+    hipLaunchKernelGGL((norm_rope_append_kernel<T, 0>), grid, dim3(kThreads), 0, stream, p, lanes_log2);
+  else
+    hipLaunchKernelGGL((norm_rope_append_kernel<T, 1>), grid, dim3(kThreads), 0, stream, p, lanes_log2);
+  return hipGetLastError();
+}
+
+// Compaction.  A wavefront per (layer, request, KV head, pool): the rows of one
+// head's path, in batches that fit its registers, all of a batch read before any
+// of it is written.  Indices ascend, so a row's source lies at or behind its
+// destination, and behind every destination of the batches before: whatever is
+// written, its old content has been read.
+constexpr int kBatch = 8; // vectors per lane and batch
+
+template <typename V>
+__global__ __launch_bounds__(kThreads) void compact_drafts_kernel(CompactDraftsParams p, int row_vecs, int64_t units) {
+  const int64_t unit = (int64_t)blockIdx.x * (kThreads / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  if (unit >= units) return;
+  const int l = threadIdx.x % kWave;
+  const int pool_index = (int)(unit % 2);
+  int64_t rest = unit / 2;
+  const int h = (int)(rest % p.num_kv_heads);
+  rest /= p.num_kv_heads; // layer * num_seqs + request
+  const int b = (int)(rest % p.num_seqs);
+  const int seq_len = p.seq_lens[b];
+  const int q_len = p.cu_q_lens[b + 1] - p.cu_q_lens[b];
+  const int first = seq_len - q_len;
+  const int count = max(0, min(p.accepted_lens[b], min(q_len, p.max_accepted)));
+  if (unit < 2 * (int64_t)p.num_kv_heads * p.num_seqs && unit % (2 * p.num_kv_heads) == 0 && l == 0 && p.new_seq_lens)
+    p.new_seq_lens[b] = first + count;
+  if (first < 0 || q_len <= 0 || seq_len > p.max_seq_len) return; // (a broken table)
+  V* pool = static_cast<V*>(pool_index ? p.value_pool : p.key_pool);
+  const int32_t* accepted = p.accepted + (int64_t)b * p.max_accepted;
+  const int32_t* bt = p.block_tables + rest * p.block_table_stride;
+  // First vector of the row at cache slot t, or -1.
+  auto row_at = [&](int t) -> int64_t {
+    const int64_t page = bt[t / p.page_size];
+    if (page < 0 || page >= p.num_pages) return -1;
+    return ((page * p.num_kv_heads + h) * p.page_size + t % p.page_size) * (int64_t)row_vecs;
+  };
+  const int batch_rows = max(1, kWave * kBatch / row_vecs);
+  for (int j0 = 0; j0 < count; j0 += batch_rows) {
+    const int64_t vecs = (int64_t)min(batch_rows, count - j0) * row_vecs;
+    // (One pass, but for rows of more vectors than a batch holds: two different
+    // rows, copied piece by piece.)
+    for (int64_t v0 = 0; v0 < vecs; v0 += kWave * kBatch) {
+      V held[kBatch];
+      int64_t to[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; u++) {
+        const int64_t v = v0 + l + kWave * u;
+        to[u] = -1;
+        if (v < vecs) {
+          const int j = j0 + (int)(v / row_vecs), c = (int)(v % row_vecs);
+          const int s = accepted[j];
+          if (s > j && s < q_len && (j == 0 || s > accepted[j - 1])) { // (s == j is in place)
+            const int64_t src = row_at(first + s), dst = row_at(first + j);
+            if (src >= 0 && dst >= 0) {
+              held[u] = pool[src + c];
+              to[u] = dst + c;
+            }
+          }
+        }
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the batch is in registers
+#pragma unroll
+      for (int u = 0; u < kBatch; u++)
+        if (to[u] >= 0) pool[to[u]] = held[u];
+    }
+  }
+}
+
+// Copies of pages.  A block per piece of kCopyVecs * 256 vectors of one page's
+// leading tokens, K and V in turn; all of a thread's loads before its stores.
+constexpr int kCopyVecs = 4;
+
+template <typename V>
+__global__ __launch_bounds__(kThreads) void copy_pages_kernel(CopyPagesParams p, int row_vecs, int pieces) {
+  const int64_t block = blockIdx.x;
+  const int piece = (int)(block % pieces);
+  const int64_t i = block / pieces / 2;
+  V* pool = static_cast<V*>(block / pieces % 2 ? p.value_pool : p.key_pool);
+  const int64_t src = ((const const_i32*)p.src_pages)[i], dst = ((const const_i32*)p.dst_pages)[i];
+  const int tokens = p.tokens ? min(max(((const const_i32*)p.tokens)[i], 0), p.page_size) : p.page_size;
+  if (src < 0 || src >= p.num_pages || dst < 0 || dst >= p.num_pages) return;
+  const unsigned per_head = (unsigned)tokens * row_vecs, head_stride = (unsigned)p.page_size * row_vecs;
+  const unsigned vecs = per_head * p.num_kv_heads;
+  const unsigned v0 = (unsigned)piece * kCopyVecs * kThreads + threadIdx.x;
+  const V* from = pool + src * ((int64_t)head_stride * p.num_kv_heads);
+  V* to = pool + dst * ((int64_t)head_stride * p.num_kv_heads);
+  V held[kCopyVecs];
+  unsigned at[kCopyVecs];
+#pragma unroll
+  for (int u = 0; u < kCopyVecs; u++) {
+    const unsigned v = v0 + u * kThreads;
+    if (v < vecs) {
+      at[u] = v / per_head * head_stride + v % per_head;
+      held[u] = from[at[u]];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kCopyVecs; u++)
+    if (v0 + u * kThreads < vecs) to[at[u]] = held[u];
+}
+
+// Widest vector that rows and pools allow.
+template <typename F>
+hipError_t with_vector(int64_t row_bytes, const void* a, const void* b, F launch) {
+  const uintptr_t align = (uintptr_t)a | (uintptr_t)b | (uintptr_t)row_bytes;
+  if (align % 16 == 0) return launch(u32x4{}, (int)(row_bytes / 16));
+  if (align % 4 == 0) return launch(uint32_t{}, (int)(row_bytes / 4));
+  return launch(uint16_t{}, (int)(row_bytes / 2));
+}
+
+} // namespace
+
+hipError_t launch_norm_rope_append(const NormRopeAppendParams& params, int dtype, int rope_type, hipStream_t stream) {
+  return dtype == 1 ? launch_append<half_t>(params, rope_type, stream) : launch_append<float>(params, rope_type, stream);
+}
+
+hipError_t launch_compact_drafts(const CompactDraftsParams& params, int64_t row_bytes, hipStream_t stream) {
+  const int64_t units = 2 * (int64_t)params.num_layers * params.num_seqs * params.num_kv_heads;
+  const unsigned blocks = (unsigned)((units + kThreads / kWave - 1) / (kThreads / kWave));
+  return with_vector(row_bytes, params.key_pool, params.value_pool, [&](auto v, int row_vecs) {
+    hipLaunchKernelGGL(compact_drafts_kernel<decltype(v)>, dim3(blocks), dim3(kThreads), 0, stream, params, row_vecs, units);
+    return hipGetLastError();
+  });
+}
+
+hipError_t launch_copy_pages(const CopyPagesParams& params, int64_t row_bytes, hipStream_t stream) {
+  return with_vector(row_bytes, params.key_pool, params.value_pool, [&](auto v, int row_vecs) {
+    const int64_t vecs = (int64_t)params.num_kv_heads * params.page_size * row_vecs;
+    const int64_t pieces = (vecs + kCopyVecs * kThreads - 1) / (kCopyVecs * kThreads);
+    hipLaunchKernelGGL(copy_pages_kernel<decltype(v)>, dim3((unsigned)(2 * pieces * params.num_copies)), dim3(kThreads),
+                       0, stream, params, row_vecs, (int)pieces);
+    return hipGetLastError();
+  });
+}
+
+} // namespace mvr

@@ -17,6 +17,7 @@
 #include <mutex>
 #include <vector>
 
+#include "api_common.hpp"
 #include "kv_append.hpp"
 #include "kv_gather.hpp"
 #include "paged_attention_kernels.hpp"
@@ -1233,6 +1234,41 @@ CascadePlan make_cascade_plan(const mvr_paged_attention_args* a, const mvr_casca
 }
 
 } // namespace
+
+// For the entry points of other files (api_common.hpp).
+namespace mvr {
+namespace api {
+
+int fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+void clear_error() { g_last_error[0] = 0; }
+
+bool checked() { return checked_mode(); }
+
+bool copy_to_host(const int32_t* dev, size_t count, void* stream, std::vector<int32_t>& host) {
+  return copy_table(dev, count, static_cast<hipStream_t>(stream), host);
+}
+
+int check_attention_scalars(const mvr_paged_attention_args* a) { return check_scalars(a); }
+
+int compute_units() { return device_cus(); }
+
+Range::Range(const char* name) : on_(roctx_enabled()) {
+  if (on_) roctxRangePushA(name);
+}
+
+Range::~Range() {
+  if (on_) roctxRangePop();
+}
+
+} // namespace api
+} // namespace mvr
 
 extern "C" {
 
