@@ -15,6 +15,7 @@
 #include "api_common.hpp"
 #include "draft_attention.hpp"
 #include "draft_cache.hpp"
+#include "paged_attention_kernels.hpp" // kChunkTokens
 #include "paged_prefill.hpp" // page_divider
 
 namespace {
@@ -65,6 +66,9 @@ int check_tree(const mvr_paged_attention_args* a, const mvr_draft_trees* t) {
   if (t->mask_words < (a->max_q_len - 1) / 32 + 1)
     return fail(MVR_E_INVALID_ARGUMENT, "mask rows of %d words cannot hold max_q_len %d drafts", t->mask_words,
                 a->max_q_len);
+  if (a->page_size % mvr::kChunkTokens != 0 && (int64_t)a->page_size * a->head_dim * es_of(a->dtype) > INT32_MAX)
+    return fail(MVR_E_UNSUPPORTED, "pages of 2 GiB per KV head whose size is not a multiple of %d tokens",
+                mvr::kChunkTokens);
   // The kernels count a page's rows, a head's rows and work items in 32 bits.
   if (a->num_pages > INT32_MAX || (int64_t)a->num_kv_heads * a->page_size > INT32_MAX)
     return fail(MVR_E_UNSUPPORTED, "pools of over 2^31 pages, or pages of over 2^31 rows");
@@ -93,14 +97,14 @@ void each_request(const mvr_paged_attention_args* a, F f) {
   for (int s = 0; s < a->num_seqs; s++) f(fits ? Request{cu[s + 1] - cu[s], sl[s]} : Request{a->max_q_len, a->max_seq_len});
 }
 
-// Row tiles of 16 rows, or 32 where a request has more rows than 16 (each tile
-// reads the keys once, so fewer, larger tiles read less).  The keys of a tile
-// are split into parts until the blocks fill the CUs.
+// Row tiles of 16, 32, 64 or 128 rows, the least that holds the longest
+// request's rows (each tile reads the keys once, so fewer, larger tiles read
+// less).  The keys of a tile are split into parts until the blocks fill the CUs.
 mvr::DraftAttentionPlan plan_tree(const mvr_paged_attention_args* a, size_t limit) {
   mvr::DraftAttentionPlan plan{};
   const int group = a->num_q_heads / a->num_kv_heads;
   const int64_t rows = (int64_t)group * a->max_q_len;
-  plan.tile_rows = rows <= 16 || a->head_dim > 128 ? 16 : 32;
+  plan.tile_rows = rows <= 16 ? 16 : a->head_dim > 128 ? 128 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
   plan.row_tiles = (int)((rows + plan.tile_rows - 1) / plan.tile_rows);
   plan.blocks = a->num_seqs * a->num_kv_heads * plan.row_tiles;
   // Tiles, and the keys that they read, in units.
@@ -115,10 +119,11 @@ mvr::DraftAttentionPlan plan_tree(const mvr_paged_attention_args* a, size_t limi
   });
   const int64_t capacity = 2 * (int64_t)mvr::api::compute_units();
   if (tiles == 0 || tiles >= capacity) return plan;
+  if (limit == 0) return plan;
+  // The planner's choice of parts.
   const int64_t floor_units = 4;
   int64_t part = std::max(floor_units, (work + capacity - 1) / capacity);
   if (part >= longest) return plan;
-  const size_t slot = (size_t)plan.tile_rows * (a->head_dim + 2) * sizeof(float);
   for (;; part++) {
     if (part >= longest) return plan;
     int64_t items = 0;
@@ -131,7 +136,6 @@ mvr::DraftAttentionPlan plan_tree(const mvr_paged_attention_args* a, size_t limi
     const size_t bytes = align_up((size_t)items * plan.tile_rows * a->head_dim * sizeof(float), 256) +
                          align_up((size_t)items * plan.tile_rows * 2 * sizeof(float), 256);
     if (bytes > limit) continue;
-    (void)slot;
     plan.part_units = (int)part;
     plan.blocks = plan.max_items = (int)items;
     plan.partial_bytes = bytes;

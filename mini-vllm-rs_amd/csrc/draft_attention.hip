@@ -10,259 +10,10 @@
 //
 // The masks matter to the key chunks that hold drafts only: all the others are
 // seen by every row, and take no mask, no test and no table read.
-#include "draft_attention.hpp"
-
-#include "chunk_traits.hpp"
-#include "wave_scan.hpp"
-
-#include <math.h>
+#include "draft_common.hpp"
 
 namespace mvr {
 namespace {
-
-constexpr int kDraftWaves = 4; // wavefronts per block
-constexpr int kXcds = 8;
-
-struct DraftSeq {
-  int seq_len, q_start, q_len;
-};
-
-// The tables' loads, an absent table's from one that is there, go out together.
-__device__ __forceinline__ DraftSeq load_draft_seq(const DraftAttentionParams& p, int b) {
-  const int32_t* any = p.cu_q_lens ? p.cu_q_lens : p.seq_lens ? p.seq_lens : p.block_tables;
-  const int seq_len = *(p.seq_lens ? p.seq_lens + b : any);
-  const int q_start = *(p.cu_q_lens ? p.cu_q_lens + b : any);
-  const int q_end = *(p.cu_q_lens ? p.cu_q_lens + b + 1 : any);
-  DraftSeq s;
-  // Clamped to the bounds that the host has checked tables and masks for.
-  s.seq_len = p.seq_lens ? min(seq_len, p.max_seq_len) : p.max_seq_len;
-  s.q_start = p.cu_q_lens ? q_start : 0;
-  s.q_len = p.cu_q_lens ? min(q_end - q_start, p.max_q_len) : p.max_q_len;
-  if (s.seq_len <= 0 || s.q_len <= 0) s.seq_len = s.q_len = 0;
-  return s;
-}
-
-__device__ __forceinline__ DraftSeq uniform_seq(const DraftSeq& s, int src) {
-  auto lane = [&](int v) { return __builtin_amdgcn_readlane(v, src); };
-  return DraftSeq{lane(s.seq_len), lane(s.q_start), lane(s.q_len)};
-}
-
-template <int kTileRows>
-__device__ __forceinline__ int row_tiles_of(const DraftAttentionParams& p, const DraftSeq& s) {
-  return (p.group_size * s.q_len + kTileRows - 1) / kTileRows;
-}
-
-__device__ __forceinline__ int key_units_of(const DraftSeq& s) {
-  return (s.seq_len + kDraftUnitTokens - 1) / kDraftUnitTokens;
-}
-
-// Parts of each of a request's row tiles (at least 1; only meaningful where it
-// has rows).
-__device__ __forceinline__ int parts_of(const DraftAttentionParams& p, const DraftSeq& s, bool split) {
-  if (!split) return 1;
-  return min((key_units_of(s) + p.part_units - 1) / p.part_units, kDraftMaxParts);
-}
-
-// Work of one block: part `part` of `parts` of row tile (b, h, rt).
-struct DraftItem {
-  int b, h, rt, part, parts;
-  DraftSeq s;
-};
-
-// Items are numbered request by request, within a request part by part, KV head
-// by KV head, and the row tiles of one (KV head, part), which read the same keys,
-// next to each other.  One request per lane, 64 at a time.
-struct DraftScan {
-  int total;   // items of the whole call
-  bool split;  // false: more items than slots, every row tile is one item
-};
-
-template <int kTileRows>
-__device__ __forceinline__ int items_of_lane(const DraftAttentionParams& p, int b0, bool split, DraftSeq& s) {
-  const int b = b0 + lane_id();
-  s = load_draft_seq(p, min(b, p.num_seqs - 1));
-  return b < p.num_seqs ? row_tiles_of<kTileRows>(p, s) * parts_of(p, s, split) * p.num_kv_heads : 0;
-}
-
-template <int kTileRows>
-__device__ __forceinline__ int count_items(const DraftAttentionParams& p, bool split) {
-  int total = 0;
-  for (int b0 = 0; b0 < p.num_seqs; b0 += kWaveSize) {
-    DraftSeq s;
-    total += __builtin_amdgcn_readlane(wave_inclusive_sum(items_of_lane<kTileRows>(p, b0, split, s)), kWaveSize - 1);
-  }
-  return total;
-}
-
-// The request of item w and the item's number within it (false: no such item).
-template <int kTileRows>
-__device__ __forceinline__ bool find_request(const DraftAttentionParams& p, int w, bool split, int& b_out, int& local,
-                                             DraftSeq& s_out) {
-  for (int b0 = 0; b0 < p.num_seqs; b0 += kWaveSize) {
-    DraftSeq s;
-    const int n = items_of_lane<kTileRows>(p, b0, split, s);
-    const int incl = wave_inclusive_sum(n);
-    const int sum = __builtin_amdgcn_readlane(incl, kWaveSize - 1);
-    if (w < sum) {
-      const int src = __builtin_ctzll(__ballot(w < incl));
-      b_out = b0 + src;
-      local = w - __builtin_amdgcn_readlane(incl - n, src);
-      s_out = uniform_seq(s, src);
-      return true;
-    }
-    w -= sum;
-  }
-  return false;
-}
-
-// Block index -> item number: the blocks of one XCD (workgroups are dealt to
-// the 8 XCDs round-robin) take a contiguous range of items, so that the row
-// tiles of one (KV head, part) find each other's keys in that XCD's L2.
-__device__ __forceinline__ int xcd_item(int block, int blocks) {
-  const int xcd = block % kXcds, per = blocks / kXcds, more = blocks % kXcds;
-  return xcd * per + min(xcd, more) + block / kXcds;
-}
-
-// Visibility of the 32 keys from slot `off` of the drafts on (negative: keys
-// before the drafts, which every row sees), from the row's mask.
-struct RowMask {
-  const uint32_t* words; // the row's mask words
-  uint32_t w0, w1;       // the first two
-  int q_len;
-};
-
-__device__ __forceinline__ uint32_t mask_word(const RowMask& m, int k) {
-  const int bits = m.q_len - 32 * k; // that belong to drafts
-  if (bits <= 0) return 0;
-  const uint32_t w = k == 0 ? m.w0 : k == 1 ? m.w1 : m.words[k];
-  return bits >= 32 ? w : w & ((1u << bits) - 1);
-}
-
-__device__ __forceinline__ RowMask load_row_mask(const DraftAttentionParams& p, const DraftSeq& s, bool valid, int i) {
-  RowMask m;
-  m.words = p.masks + (int64_t)(s.q_start + i) * p.mask_words;
-  m.q_len = valid ? s.q_len : 0; // a row that is none sees no draft
-  m.w0 = valid ? m.words[0] : 0;
-  m.w1 = valid && s.q_len > 32 ? m.words[1] : 0;
-  return m;
-}
-
-__device__ __forceinline__ uint32_t visible_bits(const RowMask& m, int off) {
-  if (off <= -32) return ~0u;
-  if (off < 0) return (mask_word(m, 0) << -off) | ((1u << -off) - 1);
-  const int k = off >> 5, sh = off & 31;
-  const uint32_t lo = mask_word(m, k) >> sh;
-  return sh ? lo | mask_word(m, k + 1) << (32 - sh) : lo;
-}
-
-// 0 for a row without a key (its sum is 0: no exponential was added), else 1 / sum.
-__device__ __forceinline__ float inverse_sum(float sum) { return __float_as_uint(sum) == 0 ? 0.f : 1.f / sum; }
-
-__device__ __forceinline__ bool any_non_finite(const half8& v) {
-  typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-  const u32x4 x = __builtin_bit_cast(u32x4, v);
-  bool bad = false;
-#pragma unroll
-  for (int e = 0; e < 4; e++) bad |= (x[e] & 0x7c00u) == 0x7c00u || (x[e] & 0x7c000000u) == 0x7c000000u;
-  return bad;
-}
-
-__device__ __forceinline__ bool any_non_finite(const float4v& v) {
-  bool bad = false;
-#pragma unroll
-  for (int e = 0; e < 4; e++) bad |= (__float_as_uint(v[e]) & 0x7f800000u) == 0x7f800000u;
-  return bad;
-}
-
-// One value of V split into its finite part and whether it is +infinity (or
-// NaN) or -infinity (or NaN): what a row that sees it gets, and only such a row.
-template <typename T>
-struct SplitValue {
-  T finite, plus, minus;
-};
-__device__ __forceinline__ SplitValue<half_t> split_value(half_t v) {
-  const uint16_t x = __builtin_bit_cast(uint16_t, v);
-  const bool bad = (x & 0x7c00u) == 0x7c00u, nan = bad && (x & 0x3ffu);
-  return {bad ? (half_t)0 : v, bad && (nan || !(x & 0x8000u)) ? (half_t)1 : (half_t)0,
-          bad && (nan || (x & 0x8000u)) ? (half_t)1 : (half_t)0};
-}
-__device__ __forceinline__ SplitValue<float> split_value(float v) {
-  const uint32_t x = __float_as_uint(v);
-  const bool bad = (x & 0x7f800000u) == 0x7f800000u, nan = bad && (x & 0x7fffffu);
-  return {bad ? 0.f : v, bad && (nan || !(x >> 31)) ? 1.f : 0.f, bad && (nan || (x >> 31)) ? 1.f : 0.f};
-}
-
-__device__ __forceinline__ void add_infinities(float4v& o, const float4v& plus, const float4v& minus) {
-#pragma unroll
-  for (int e = 0; e < 4; e++) {
-    if (plus[e] > 0.f) o[e] += INFINITY;
-    if (minus[e] > 0.f) o[e] -= INFINITY;
-  }
-}
-
-// O^T += V^T P^T of a chunk whose V holds an infinity or a NaN: a masked key's
-// 0 * infinity would reach every row of the product, so the finite values are
-// multiplied by P and the others by the rows' visibility (1 or 0).
-template <int D>
-struct GuardedPv {
-  template <int NB>
-  __device__ static void run(F16Traits<D>, half_t* lds, int l, const float (&p)[NB][4], const uint32_t (&vis)[NB],
-                             float4v (&o)[NB][D / 16]) {
-    const int g = l >> 4, qd = l & 15;
-    const int row = 4 * g + (qd >> 2);
-    const int sw = F16Traits<D>::swz(row);
-#pragma unroll
-    for (int n = 0; n < D / 16; n++) {
-      half_t* addr = lds + row * D + ((n ^ sw) * 16) + 4 * (qd & 3);
-      const half4 vt = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(addr)));
-      half4 fin, plus, minus;
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const SplitValue<half_t> sv = split_value(vt[e]);
-        fin[e] = sv.finite, plus[e] = sv.plus, minus[e] = sv.minus;
-      }
-#pragma unroll
-      for (int nb = 0; nb < NB; nb++) {
-        half4 pb, seen;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          pb[e] = (half_t)p[nb][e];
-          seen[e] = (vis[nb] >> e) & 1 ? (half_t)1 : (half_t)0;
-        }
-        const float4v zero = {0.f, 0.f, 0.f, 0.f};
-        o[nb][n] = __builtin_amdgcn_mfma_f32_16x16x16f16(fin, pb, o[nb][n], 0, 0, 0);
-        add_infinities(o[nb][n], __builtin_amdgcn_mfma_f32_16x16x16f16(plus, seen, zero, 0, 0, 0),
-                       __builtin_amdgcn_mfma_f32_16x16x16f16(minus, seen, zero, 0, 0, 0));
-      }
-    }
-  }
-
-  template <int NB>
-  __device__ static void run(F32Traits<D>, float* lds, int l, const float (&p)[NB][4], const uint32_t (&vis)[NB],
-                             float4v (&o)[NB][D / 16]) {
-    const int g = l >> 4, qd = l & 15;
-#pragma unroll
-    for (int n = 0; n < D / 16; n++) {
-      float4v plus[NB], minus[NB];
-#pragma unroll
-      for (int nb = 0; nb < NB; nb++) plus[nb] = minus[nb] = float4v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int row = 4 * g + j;
-        const SplitValue<float> sv = split_value(lds[row * D + ((n ^ F32Traits<D>::swz(row)) * 16) + qd]);
-#pragma unroll
-        for (int nb = 0; nb < NB; nb++) {
-          const float seen = (vis[nb] >> j) & 1 ? 1.f : 0.f;
-          o[nb][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(sv.finite, p[nb][j], o[nb][n], 0, 0, 0);
-          plus[nb] = __builtin_amdgcn_mfma_f32_16x16x4f32(sv.plus, seen, plus[nb], 0, 0, 0);
-          minus[nb] = __builtin_amdgcn_mfma_f32_16x16x4f32(sv.minus, seen, minus[nb], 0, 0, 0);
-        }
-      }
-#pragma unroll
-      for (int nb = 0; nb < NB; nb++) add_infinities(o[nb][n], plus[nb], minus[nb]);
-    }
-  }
-};
 
 // ---------------------------------------------------------------------------
 // Key streaming: a block of 4 wavefronts per item, 16 * NB rows, each wavefront
@@ -412,31 +163,53 @@ __device__ __forceinline__ void stream_item(const DraftAttentionParams& p, const
     Tr::template pv<NB>(lds, l, pr, o);
   };
 
-  // Any chunk, under the rows' masks.
+  // Any chunk, under the rows' masks.  A draft's V may hold infinities and NaN:
+  // in a product, 0 times one of those would reach the rows that do not see the
+  // draft.  Such a chunk's are added to the rows that see them one by one, and
+  // the finite rest goes through the product.
   auto process_drafts = [&](int k, const RowMask (&mask)[NB], const typename Tr::kreg_t (&kr)[Tr::kLoads],
-                            const typename Tr::vreg_t (&vr)[Tr::kLoads]) {
-    const int tok0 = k * kChunkTokens;
+                            typename Tr::vreg_t (&vr)[Tr::kLoads]) {
+    const int tok0 = k * kChunkTokens, tokens = min(s.seq_len - tok0, kChunkTokens);
     asm volatile("" ::: "memory");
-    Tr::stage_v(lds, l, s.seq_len - tok0, vr);
+    Tr::stage_v(lds, l, tokens, vr);
     bool bad = false;
 #pragma unroll
-    for (int u = 0; u < Tr::kLoads; u++) bad |= Tr::v_row(l, u) < s.seq_len - tok0 && any_non_finite(vr[u]);
-    uint32_t vis[NB]; // of the lane's 4 tokens
+    for (int u = 0; u < Tr::kLoads; u++) bad |= Tr::v_row(l, u) < tokens && any_non_finite(vr[u]);
+    uint32_t vis[NB]; // of the chunk's tokens
     float pr[NB][4];
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
       const float4v sc = Tr::qk(kr, q[nb]);
-      vis[nb] = visible_bits(mask[nb], tok0 - prefix) >> (4 * g);
+      vis[nb] = visible_bits(mask[nb], tok0 - prefix);
       float sv[4];
 #pragma unroll
-      for (int i = 0; i < 4; i++) sv[i] = (vis[nb] >> i) & 1 ? sc[i] * p.scale_log2 : -INFINITY;
+      for (int i = 0; i < 4; i++) sv[i] = (vis[nb] >> (4 * g + i)) & 1 ? sc[i] * p.scale_log2 : -INFINITY;
       softmax(nb, sv, pr[nb]);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (__any(bad))
-      GuardedPv<D>::template run<NB>(Tr{}, lds, l, pr, vis, o);
-    else
-      Tr::template pv<NB>(lds, l, pr, o);
+    if (__any(bad)) {
+      for (int t = 0; t < tokens; t++) {
+#pragma unroll
+        for (int n = 0; n < D / 16; n++) {
+          // The lane's dims 16 n + 4 g + e of token t, where stage_v put them.
+          const T* src = lds + t * D + (n ^ Tr::swz(t)) * 16 + 4 * g;
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float x = non_finite_part(src[e]);
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) o[nb][n][e] += (vis[nb] >> t) & 1 ? x : 0.f;
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < Tr::kLoads; u++)
+#pragma unroll
+        for (int e = 0; e < (int)(sizeof(vr[u]) / sizeof(T)); e++) vr[u][e] = finite_or_zero(vr[u][e]);
+      asm volatile("" ::: "memory"); // (a wavefront's LDS accesses complete in order)
+      Tr::stage_v(lds, l, tokens, vr);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    Tr::template pv<NB>(lds, l, pr, o);
   };
 
   // kDepth chunks in flight; a tail past k1 reloads chunk k1 - 1 (an L2 hit)
@@ -605,32 +378,43 @@ __global__ __launch_bounds__(256) void draft_merge_kernel(DraftAttentionParams p
 }
 
 template <typename Tr, int D, int NB>
-hipError_t launch_rows(const DraftAttentionPlan& plan, const DraftAttentionParams& p, hipStream_t stream) {
+hipError_t launch_stream(const DraftAttentionPlan& plan, const DraftAttentionParams& p, hipStream_t stream) {
   const dim3 grid((unsigned)plan.blocks), block(kWaveSize * kDraftWaves);
   if (p.page_size % kChunkTokens == 0)
     hipLaunchKernelGGL((draft_stream_kernel<Tr, D, NB, false>), grid, block, 0, stream, p);
   else
     hipLaunchKernelGGL((draft_stream_kernel<Tr, D, NB, true>), grid, block, 0, stream, p);
-  hipError_t err = hipGetLastError();
-  if (err != hipSuccess || plan.max_items == 0) return err;
-  constexpr int kCells = 16 * NB * (D / 4);
-  const dim3 merge((kCells + 255) / 256, (unsigned)(p.num_seqs * p.num_kv_heads * p.row_tiles));
-  hipLaunchKernelGGL((draft_merge_kernel<Tr, D, 16 * NB>), merge, dim3(256), 0, stream, p);
+  return hipGetLastError();
+}
+
+template <typename Tr, int D, int kTileRows>
+hipError_t launch_merge(const DraftAttentionParams& p, hipStream_t stream) {
+  constexpr int kCells = kTileRows * (D / 4);
+  const dim3 grid((kCells + 255) / 256, (unsigned)(p.num_seqs * p.num_kv_heads * p.row_tiles));
+  hipLaunchKernelGGL((draft_merge_kernel<Tr, D, kTileRows>), grid, dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 
 template <typename Tr, int D>
-hipError_t launch_dim(const DraftAttentionPlan& plan, const DraftAttentionParams& p, hipStream_t stream) {
-  if (plan.tile_rows == 16) return launch_rows<Tr, D, 1>(plan, p, stream);
+hipError_t launch_dim(const DraftAttentionPlan& plan, const DraftAttentionParams& p, int dtype, hipStream_t stream) {
+  hipError_t err = hipErrorInvalidValue;
+  if (plan.tile_rows == 16) err = launch_stream<Tr, D, 1>(plan, p, stream);
   if constexpr (D <= 128) {
-    if (plan.tile_rows == 32) return launch_rows<Tr, D, 2>(plan, p, stream);
+    if (plan.tile_rows == 32) err = launch_stream<Tr, D, 2>(plan, p, stream);
   }
-  return hipErrorInvalidValue;
+  if (plan.tile_rows >= 64) err = launch_draft_tiles(plan, p, dtype, D, stream);
+  if (err != hipSuccess || plan.max_items == 0) return err;
+  switch (plan.tile_rows) {
+  case 16: return launch_merge<Tr, D, 16>(p, stream);
+  case 32: return launch_merge<Tr, D, 32>(p, stream);
+  case 64: return launch_merge<Tr, D, 64>(p, stream);
+  default: return launch_merge<Tr, D, 128>(p, stream);
+  }
 }
 
 template <int D>
 hipError_t launch_type(const DraftAttentionPlan& plan, const DraftAttentionParams& p, int dtype, hipStream_t stream) {
-  return dtype == 1 ? launch_dim<F16Traits<D>, D>(plan, p, stream) : launch_dim<F32Traits<D>, D>(plan, p, stream);
+  return dtype == 1 ? launch_dim<F16Traits<D>, D>(plan, p, dtype, stream) : launch_dim<F32Traits<D>, D>(plan, p, dtype, stream);
 }
 
 } // namespace

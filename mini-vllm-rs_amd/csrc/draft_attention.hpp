@@ -48,7 +48,7 @@ struct DraftAttentionParams {
 };
 
 struct DraftAttentionPlan {
-  int tile_rows; // 16 or 32
+  int tile_rows; // 16 or 32 (key streaming), 64 or 128 (key tiles in LDS)
   int row_tiles;
   int part_units; // 0: not split
   int blocks;
@@ -56,6 +56,12 @@ struct DraftAttentionPlan {
   size_t partial_bytes;
 };
 
+// draft_tiles.hip: the attention itself, of row tiles of 64 (head_dim up to 128)
+// and 128 rows.
+hipError_t launch_draft_tiles(const DraftAttentionPlan& plan, const DraftAttentionParams& params, int dtype,
+                              int head_dim, hipStream_t stream);
+
+// The attention, then the merge of what was split.
 hipError_t launch_draft_attention(const DraftAttentionPlan& plan, const DraftAttentionParams& params, int dtype,
                                   int head_dim, hipStream_t stream);
 

@@ -1,0 +1,198 @@
+// What the drafted-tree attention kernels share: the requests' lengths, which
+// part of which row tile a block works on, the rows' masks.
+#pragma once
+
+#include "chunk_traits.hpp"
+#include "draft_attention.hpp"
+#include "wave_scan.hpp"
+
+#include <math.h>
+
+namespace mvr {
+namespace {
+
+constexpr int kDraftWaves = 4; // wavefronts per block
+constexpr int kXcds = 8;
+
+struct DraftSeq {
+  int seq_len, q_start, q_len;
+};
+
+// The tables' loads, an absent table's from one that is there, go out together.
+__device__ __forceinline__ DraftSeq load_draft_seq(const DraftAttentionParams& p, int b) {
+  const int32_t* any = p.cu_q_lens ? p.cu_q_lens : p.seq_lens ? p.seq_lens : p.block_tables;
+  const int seq_len = *(p.seq_lens ? p.seq_lens + b : any);
+  const int q_start = *(p.cu_q_lens ? p.cu_q_lens + b : any);
+  const int q_end = *(p.cu_q_lens ? p.cu_q_lens + b + 1 : any);
+  DraftSeq s;
+  // Clamped to the bounds that the host has checked tables and masks for.
+  s.seq_len = p.seq_lens ? min(seq_len, p.max_seq_len) : p.max_seq_len;
+  s.q_start = p.cu_q_lens ? q_start : 0;
+  s.q_len = p.cu_q_lens ? min(q_end - q_start, p.max_q_len) : p.max_q_len;
+  if (s.seq_len <= 0 || s.q_len <= 0) s.seq_len = s.q_len = 0;
+  return s;
+}
+
+__device__ __forceinline__ DraftSeq uniform_seq(const DraftSeq& s, int src) {
+  auto lane = [&](int v) { return __builtin_amdgcn_readlane(v, src); };
+  return DraftSeq{lane(s.seq_len), lane(s.q_start), lane(s.q_len)};
+}
+
+template <int kTileRows>
+__device__ __forceinline__ int row_tiles_of(const DraftAttentionParams& p, const DraftSeq& s) {
+  return (p.group_size * s.q_len + kTileRows - 1) / kTileRows;
+}
+
+__device__ __forceinline__ int key_units_of(const DraftSeq& s) {
+  return (s.seq_len + kDraftUnitTokens - 1) / kDraftUnitTokens;
+}
+
+// Parts of each of a request's row tiles (at least 1; only meaningful where it
+// has rows).
+__device__ __forceinline__ int parts_of(const DraftAttentionParams& p, const DraftSeq& s, bool split) {
+  if (!split) return 1;
+  return min((key_units_of(s) + p.part_units - 1) / p.part_units, kDraftMaxParts);
+}
+
+// Work of one block: part `part` of `parts` of row tile (b, h, rt).
+struct DraftItem {
+  int b, h, rt, part, parts;
+  DraftSeq s;
+};
+
+// Items are numbered request by request, within a request part by part, KV head
+// by KV head, and the row tiles of one (KV head, part), which read the same keys,
+// next to each other.  One request per lane, 64 at a time.
+struct DraftScan {
+  int total;   // items of the whole call
+  bool split;  // false: more items than slots, every row tile is one item
+};
+
+template <int kTileRows>
+__device__ __forceinline__ int items_of_lane(const DraftAttentionParams& p, int b0, bool split, DraftSeq& s) {
+  const int b = b0 + lane_id();
+  s = load_draft_seq(p, min(b, p.num_seqs - 1));
+  return b < p.num_seqs ? row_tiles_of<kTileRows>(p, s) * parts_of(p, s, split) * p.num_kv_heads : 0;
+}
+
+template <int kTileRows>
+__device__ __forceinline__ int count_items(const DraftAttentionParams& p, bool split) {
+  int total = 0;
+  for (int b0 = 0; b0 < p.num_seqs; b0 += kWaveSize) {
+    DraftSeq s;
+    total += __builtin_amdgcn_readlane(wave_inclusive_sum(items_of_lane<kTileRows>(p, b0, split, s)), kWaveSize - 1);
+  }
+  return total;
+}
+
+// The request of item w and the item's number within it (false: no such item).
+template <int kTileRows>
+__device__ __forceinline__ bool find_request(const DraftAttentionParams& p, int w, bool split, int& b_out, int& local,
+                                             DraftSeq& s_out) {
+  for (int b0 = 0; b0 < p.num_seqs; b0 += kWaveSize) {
+    DraftSeq s;
+    const int n = items_of_lane<kTileRows>(p, b0, split, s);
+    const int incl = wave_inclusive_sum(n);
+    const int sum = __builtin_amdgcn_readlane(incl, kWaveSize - 1);
+    if (w < sum) {
+      const int src = __builtin_ctzll(__ballot(w < incl));
+      b_out = b0 + src;
+      local = w - __builtin_amdgcn_readlane(incl - n, src);
+      s_out = uniform_seq(s, src);
+      return true;
+    }
+    w -= sum;
+  }
+  return false;
+}
+
+// Block index -> item number: the blocks of one XCD (workgroups are dealt to
+// the 8 XCDs round-robin) take a contiguous range of items, so that the row
+// tiles of one (KV head, part) find each other's keys in that XCD's L2.
+__device__ __forceinline__ int xcd_item(int block, int blocks) {
+  const int xcd = block % kXcds, per = blocks / kXcds, more = blocks % kXcds;
+  return xcd * per + min(xcd, more) + block / kXcds;
+}
+
+// Visibility of the 32 keys from slot `off` of the drafts on (negative: keys
+// before the drafts, which every row sees), from the row's mask.
+struct RowMask {
+  const uint32_t* words; // the row's mask words
+  uint32_t w0, w1;       // the first two
+  int q_len;
+};
+
+__device__ __forceinline__ uint32_t mask_word(const RowMask& m, int k) {
+  const int bits = m.q_len - 32 * k; // that belong to drafts
+  if (bits <= 0) return 0;
+  const uint32_t w = k == 0 ? m.w0 : k == 1 ? m.w1 : m.words[k];
+  return bits >= 32 ? w : w & ((1u << bits) - 1);
+}
+
+__device__ __forceinline__ RowMask load_row_mask(const DraftAttentionParams& p, const DraftSeq& s, bool valid, int i) {
+  RowMask m;
+  m.words = p.masks + (int64_t)(s.q_start + i) * p.mask_words;
+  m.q_len = valid ? s.q_len : 0; // a row that is none sees no draft
+  m.w0 = valid ? m.words[0] : 0;
+  m.w1 = valid && s.q_len > 32 ? m.words[1] : 0;
+  return m;
+}
+
+__device__ __forceinline__ uint32_t visible_bits(const RowMask& m, int off) {
+  if (off <= -32) return ~0u;
+  if (off < 0) return (mask_word(m, 0) << -off) | ((1u << -off) - 1);
+  const int k = off >> 5, sh = off & 31;
+  const uint32_t lo = mask_word(m, k) >> sh;
+  return sh ? lo | mask_word(m, k + 1) << (32 - sh) : lo;
+}
+
+// 0 for a row without a key (its sum is 0: no exponential was added), else 1 / sum.
+__device__ __forceinline__ float inverse_sum(float sum) { return __float_as_uint(sum) == 0 ? 0.f : 1.f / sum; }
+
+// Infinities and NaN are told by their bits, which are opaque to the optimiser
+// here: where a file is compiled without regard for NaN, it would take such a
+// test for one that only infinities pass.
+__device__ __forceinline__ uint32_t opaque_bits(uint32_t x) {
+  asm("" : "+v"(x));
+  return x;
+}
+__device__ __forceinline__ bool non_finite_bits(half_t, uint32_t x) { return (x & 0x7c00u) == 0x7c00u; }
+__device__ __forceinline__ bool non_finite_bits(float, uint32_t x) { return (x & 0x7f800000u) == 0x7f800000u; }
+__device__ __forceinline__ uint32_t bits_of(half_t v) { return opaque_bits(__builtin_bit_cast(uint16_t, v)); }
+__device__ __forceinline__ uint32_t bits_of(float v) { return opaque_bits(__float_as_uint(v)); }
+__device__ __forceinline__ half_t from_bits(half_t, uint32_t x) { return __builtin_bit_cast(half_t, (uint16_t)x); }
+__device__ __forceinline__ float from_bits(float, uint32_t x) { return __uint_as_float(x); }
+
+__device__ __forceinline__ bool any_non_finite(const half8& v) {
+  typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+  const u32x4 x = __builtin_bit_cast(u32x4, v);
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const uint32_t pair = opaque_bits(x[e]);
+    bad |= (pair & 0x7c00u) == 0x7c00u || (pair & 0x7c000000u) == 0x7c000000u;
+  }
+  return bad;
+}
+__device__ __forceinline__ bool any_non_finite(const float4v& v) {
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 4; e++) bad |= non_finite_bits(v[e], bits_of(v[e]));
+  return bad;
+}
+
+template <typename T>
+__device__ __forceinline__ T finite_or_zero(T v) {
+  const uint32_t x = bits_of(v);
+  return from_bits(v, non_finite_bits(v, x) ? 0 : x);
+}
+
+// An infinity or a NaN itself, 0 for a finite value.
+template <typename T>
+__device__ __forceinline__ float non_finite_part(T v) {
+  const uint32_t x = bits_of(v);
+  return (float)from_bits(v, non_finite_bits(v, x) ? x : 0);
+}
+
+} // namespace
+} // namespace mvr
