@@ -82,65 +82,133 @@ int check_tree(const mvr_paged_attention_args* a, const mvr_draft_trees* t) {
 // The requests as the planner sees them: the host tables where they are given
 // and within the call's bounds, else every request at those bounds.
 struct Request {
-  int q, n;
+  int64_t count, rows, units; // requests alike: grouped rows per KV head, key units
+  int64_t more;               // units and parts that one may have beyond these
 };
 
-template <typename F>
-void each_request(const mvr_paged_attention_args* a, F f) {
+bool host_tables_fit(const mvr_paged_attention_args* a) {
   const int32_t* cu = a->cu_q_lens_host;
   const int32_t* sl = a->seq_lens_host;
-  bool fits = cu && sl;
-  for (int s = 0; fits && s < a->num_seqs; s++) {
+  if (!cu || !sl) return false;
+  for (int s = 0; s < a->num_seqs; s++) {
     const int64_t q = (int64_t)cu[s + 1] - cu[s];
-    fits = q >= 0 && q <= a->max_q_len && sl[s] >= q && sl[s] <= a->max_seq_len;
+    if (q < 0 || q > a->max_q_len || sl[s] < q || sl[s] > a->max_seq_len) return false;
   }
-  for (int s = 0; s < a->num_seqs; s++) f(fits ? Request{cu[s + 1] - cu[s], sl[s]} : Request{a->max_q_len, a->max_seq_len});
+  return true;
 }
 
-// Row tiles of 16, 32, 64 or 128 rows, the least that holds the longest
-// request's rows (each tile reads the keys once, so fewer, larger tiles read
-// less).  The keys of a tile are split into parts until the blocks fill the CUs.
-mvr::DraftAttentionPlan plan_tree(const mvr_paged_attention_args* a, size_t limit) {
-  mvr::DraftAttentionPlan plan{};
-  const int group = a->num_q_heads / a->num_kv_heads;
-  const int64_t rows = (int64_t)group * a->max_q_len;
-  plan.tile_rows = rows <= 16 ? 16 : a->head_dim > 128 ? 128 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-  plan.row_tiles = (int)((rows + plan.tile_rows - 1) / plan.tile_rows);
-  plan.blocks = a->num_seqs * a->num_kv_heads * plan.row_tiles;
-  // Tiles, and the keys that they read, in units.
-  int64_t tiles = 0, work = 0, longest = 0;
-  each_request(a, [&](Request r) {
-    if (r.q == 0 || r.n == 0) return;
-    const int64_t t = (int64_t)a->num_kv_heads * ((group * (int64_t)r.q + plan.tile_rows - 1) / plan.tile_rows);
-    const int64_t units = (r.n + mvr::kDraftUnitTokens - 1) / mvr::kDraftUnitTokens;
-    tiles += t;
-    work += t * units;
-    longest = std::max(longest, units);
-  });
-  const int64_t capacity = 2 * (int64_t)mvr::api::compute_units();
-  if (tiles == 0 || tiles >= capacity) return plan;
-  if (limit == 0) return plan;
-  // The planner's choice of parts.
-  const int64_t floor_units = 4;
-  int64_t part = std::max(floor_units, (work + capacity - 1) / capacity);
-  if (part >= longest) return plan;
-  for (;; part++) {
-    if (part >= longest) return plan;
-    int64_t items = 0;
-    each_request(a, [&](Request r) {
-      if (r.q == 0 || r.n == 0) return;
-      const int64_t t = (int64_t)a->num_kv_heads * ((group * (int64_t)r.q + plan.tile_rows - 1) / plan.tile_rows);
-      const int64_t units = (r.n + mvr::kDraftUnitTokens - 1) / mvr::kDraftUnitTokens;
-      items += t * std::min<int64_t>((units + part - 1) / part, mvr::kDraftMaxParts);
-    });
-    const size_t bytes = align_up((size_t)items * plan.tile_rows * a->head_dim * sizeof(float), 256) +
-                         align_up((size_t)items * plan.tile_rows * 2 * sizeof(float), 256);
-    if (bytes > limit) continue;
-    plan.part_units = (int)part;
-    plan.blocks = plan.max_items = (int)items;
-    plan.partial_bytes = bytes;
-    return plan;
+int64_t units_of(int64_t tokens) { return (tokens + mvr::kDraftUnitTokens - 1) / mvr::kDraftUnitTokens; }
+
+template <typename F>
+void each_request(const mvr_paged_attention_args* a, bool tables, F f) {
+  const int64_t group = a->num_q_heads / a->num_kv_heads;
+  if (!tables) {
+    // sum_seq_lens alone tells the average context: requests of other lengths round
+    // up to a unit and a part more each.
+    const int64_t tokens = a->sum_seq_lens > 0 ? (a->sum_seq_lens + a->num_seqs - 1) / a->num_seqs : a->max_seq_len;
+    f(Request{a->num_seqs, group * a->max_q_len, units_of(tokens), tokens < a->max_seq_len});
+    return;
   }
+  for (int s = 0; s < a->num_seqs; s++) {
+    const int64_t q = a->cu_q_lens_host[s + 1] - a->cu_q_lens_host[s];
+    if (q > 0) f(Request{1, group * q, units_of(a->seq_lens_host[s]), 0});
+  }
+}
+
+// What a block of one tile size costs, in us, for head_dim 128: `fixed` beside
+// its keys, `unit` per 64 keys with one, two or three blocks on its CU.
+struct TileCost {
+  int rows;
+  double fixed, unit[3];
+};
+
+// Measured (one box, HIP events around calls of 1 to 64 requests on 100 to 16,000
+// tokens with 4 to 840 rows per KV head): F16, one block per CU, 4 / 63 key units:
+// 16 rows 8.6 / 49.8 us, 32 rows 9.4 / 61.0, 64 rows 11.4 (3 units) / 63.5, 128
+// rows 12.4 (3) / 96.4; more blocks per CU: 16 rows 1.79 us per unit with three, 32
+// rows 1.42 with two, 64 rows 1.1, 128 rows 2.1 (16 x 400 rows on 1,000 tokens,
+// 512 blocks of 18 units: 49.6 us).  F32, whose products take 7 times as long: 16
+// rows 2.1 us per unit, 32 rows 3.35, 64 rows 4.4, 128 rows 7.9.  A unit grows with
+// head_dim, in F16 a little slower than it (the softmax does not).
+constexpr TileCost kF16Costs[] = {{16, 5.8, {0.70, 1.25, 1.79}}, {32, 5.9, {0.875, 1.42, 1.42}},
+                                  {64, 8.3, {0.88, 1.1, 1.1}}, {128, 9.3, {1.38, 2.1, 2.1}}};
+constexpr TileCost kF32Costs[] = {{16, 5.0, {2.1, 3.8, 3.8}}, {32, 5.0, {3.35, 6.0, 6.0}},
+                                  {64, 8.5, {4.4, 7.9, 7.9}}, {128, 11.0, {7.9, 15.0, 15.0}}};
+
+// The tile size and the split of its keys that these costs make fastest: every
+// tile whole, or in as many parts as fill the CUs with one block each, or with as
+// many as they hold.  A call takes its blocks' time (all of them in one round; in
+// more rounds the average load and most of a last block), joined with the time
+// that its keys take from HBM (as a 3-norm: 128 blocks of 126 units and a bound of
+// 89 us ran in 119, 256 of 63 in 98).  A split call scans the lengths and merges:
+// 4.5 us, and its partial results at 10 TB/s (they stay in the caches).
+mvr::DraftAttentionPlan plan_tree(const mvr_paged_attention_args* a, size_t limit) {
+  const bool f16 = a->dtype == MVR_DTYPE_F16, tables = host_tables_fit(a);
+  const double dims = a->head_dim / 128.0, unit_scale = f16 ? 0.15 + 0.85 * dims : dims;
+  const int64_t cus = mvr::api::compute_units(), hkv = a->num_kv_heads;
+  const int64_t longest_rows = (int64_t)(a->num_q_heads / a->num_kv_heads) * a->max_q_len;
+  const double key_us = 2.0 * mvr::kDraftUnitTokens * hkv * a->head_dim * es_of(a->dtype) / 5.9e6; // of a request's unit
+  mvr::DraftAttentionPlan best{};
+  double best_cost = INFINITY;
+  for (const TileCost& tile : f16 ? kF16Costs : kF32Costs) {
+    if (!mvr::draft_tile_supported(tile.rows, a->head_dim)) continue;
+    // (A tile that no request fills half costs what the smaller one does, or more.)
+    if (tile.rows > 16 && longest_rows <= tile.rows / 2 && best_cost < INFINITY) break;
+    const int held = mvr::draft_blocks_per_cu(tile.rows, f16, a->head_dim);
+    auto tiles_of = [&](const Request& r) { return r.count * hkv * ((r.rows + tile.rows - 1) / tile.rows); };
+    int64_t tiles = 0, work = 0, longest = 0;
+    double hbm = 0;
+    each_request(a, tables, [&](const Request& r) {
+      if (r.units == 0) return;
+      tiles += tiles_of(r);
+      work += tiles_of(r) * r.units;
+      longest = std::max(longest, r.units);
+      hbm += r.count * r.units * key_us;
+    });
+    auto cost_of = [&](int64_t blocks, int64_t part) {
+      double body;
+      if (blocks <= held * cus)
+        body = part * tile.unit[std::max<int64_t>(0, (blocks + cus - 1) / cus - 1)];
+      else
+        body = work * tile.unit[held - 1] / (held * cus) + 0.8 * part * tile.unit[0] + 6;
+      body *= unit_scale;
+      return tile.fixed + cbrt(body * body * body + hbm * hbm * hbm);
+    };
+    auto take = [&](double cost, int64_t part, int64_t items, size_t bytes) {
+      if (!(cost < best_cost)) return;
+      best_cost = cost;
+      best.tile_rows = tile.rows;
+      best.row_tiles = (int)((longest_rows + tile.rows - 1) / tile.rows);
+      best.part_units = (int)part;
+      best.max_items = (int)items;
+      best.blocks = part ? (int)items : (int)(a->num_seqs * hkv * best.row_tiles);
+      best.partial_bytes = bytes;
+    };
+    take(cost_of(tiles, longest), 0, 0, 0);
+    if (limit == 0) continue;
+    for (int64_t target : {cus, held * cus}) {
+      if (tiles >= target || longest < 2) continue;
+      // The shortest parts whose blocks are no more than `target`: from an estimate
+      // (a request's last part is half full on average) upwards.
+      int64_t part = std::max<int64_t>(1, work / (target - tiles / 2)), items = 0, part_longest = 0;
+      size_t bytes = 0;
+      for (; part < longest; part += 1 + part / 16) {
+        items = part_longest = 0;
+        each_request(a, tables, [&](const Request& r) {
+          const int64_t parts = std::min<int64_t>((r.units + r.more + part - 1) / part + r.more, mvr::kDraftMaxParts);
+          if (parts == 0) return;
+          items += tiles_of(r) * parts;
+          part_longest = std::max(part_longest, (r.units + parts - 1) / parts);
+        });
+        bytes = align_up((size_t)items * tile.rows * a->head_dim * sizeof(float), 256) +
+                align_up((size_t)items * tile.rows * 2 * sizeof(float), 256);
+        if (items <= target && bytes <= limit) break;
+      }
+      if (part >= longest) continue;
+      take(cost_of(items, part_longest) + 4.5 + 2 * bytes / 10e6, part, items, bytes);
+    }
+  }
+  return best;
 }
 
 } // namespace

@@ -27,12 +27,14 @@ constexpr int stream_depth() {
   return sizeof(typename Tr::elem) == 4 && D > 128 ? 1 : 2;
 }
 
-// Blocks per CU (wavefronts per SIMD) that the registers allow without scratch.
-// Rows with a page of their own (TP) hold an address each.
+// Blocks per CU (wavefronts per SIMD): what the planner counts on, where the
+// registers allow it without scratch.  Rows with a page of their own (TP) hold an
+// address each.
 template <typename Tr, int D, int NB, bool TP>
 constexpr int stream_blocks() {
-  if (sizeof(typename Tr::elem) == 2) return D <= 64 ? 4 - NB : D <= 96 ? (TP ? 3 - NB : 2) : D <= 128 ? 3 - NB : D <= 160 ? 2 : 1;
-  return D <= 64 || (D <= 96 && NB == 1) ? 2 : 1;
+  constexpr bool f16 = sizeof(typename Tr::elem) == 2;
+  constexpr int planned = draft_blocks_per_cu(16 * NB, f16, D);
+  return TP && f16 && D == 96 && NB == 2 ? 1 : planned;
 }
 
 // TP: page sizes that are not a multiple of 16, where every token row has a page
@@ -102,11 +104,11 @@ __device__ __forceinline__ void stream_item(const DraftAttentionParams& p, const
   auto load_entry = [&](int k) { return (uint32_t)bt[page_div(min(k * kChunkTokens + (l & 15), s.seq_len - 1))]; };
   uint32_t next_entry = 0;
   auto load_chunk = [&](int k, typename Tr::kreg_t (&kr)[Tr::kLoads], typename Tr::vreg_t (&vr)[Tr::kLoads]) {
+    // (The lane index is opaque here, so that the rows' offsets are worked out where
+    // they are used and not held, and spilled, over the key loop.)
+    int le = l;
+    asm volatile("" : "+v"(le));
     if constexpr (TP) {
-      // (The lane index is opaque here, so that the rows' numbers are worked out
-      // where they are used and not held, and spilled, over the key loop.)
-      int le = l;
-      asm volatile("" : "+v"(le));
       const uint32_t entry = min(next_entry, p.last_page);
       next_entry = load_entry(min(k + 1, k1 - 1));
       auto at = [&](int token_row, uint32_t page) {
@@ -123,8 +125,8 @@ __device__ __forceinline__ void stream_item(const DraftAttentionParams& p, const
       const int t = k * kChunkTokens, pi = page_div(t);
       const uint32_t page = min((uint32_t)((const const_i32*)bt)[__builtin_amdgcn_readfirstlane(pi)], p.last_page);
       const uint64_t off = ((uint64_t)page * page_rows + head_rows + (uint32_t)(t - pi * p.page_size)) * D;
-      Tr::load_k(kpool + off, l, kr);
-      Tr::load_v(vpool + off, l, vr);
+      Tr::load_k(kpool + off, le, kr);
+      Tr::load_v(vpool + off, le, vr);
     }
   };
 
@@ -250,8 +252,8 @@ __device__ __forceinline__ void stream_item(const DraftAttentionParams& p, const
     }
   }
 
-  // Every wavefront's rows into LDS over the V tiles, then rows wave, wave + 4,
-  // ... are merged, a lane per 4 elements (the lanes past D / 4 re-read the last).
+  // Every wavefront's rows into LDS over the V tiles, then they are merged, a
+  // thread per 4 elements.
   __syncthreads();
 #pragma unroll
   for (int nb = 0; nb < NB; nb++) {
@@ -306,38 +308,23 @@ __global__ __launch_bounds__(kWaveSize* kDraftWaves, (stream_blocks<Tr, D, NB, T
   constexpr size_t kTileBytes = (size_t)kDraftWaves * kChunkTokens * D * sizeof(typename Tr::elem);
   constexpr size_t kMergeBytes = (size_t)kDraftWaves * kTileRows * (D + 4 + 2) * sizeof(float);
   __shared__ __attribute__((aligned(16))) char lds_raw[kTileBytes > kMergeBytes ? kTileBytes : kMergeBytes];
-  const int first = xcd_item(blockIdx.x, gridDim.x);
-  if (p.part_units == 0) {
-    DraftItem it;
-    it.rt = first % p.row_tiles;
-    it.h = (first / p.row_tiles) % p.num_kv_heads;
-    it.b = first / (p.row_tiles * p.num_kv_heads);
-    it.part = 0, it.parts = 1;
-    it.s = uniform_seq(load_draft_seq(p, it.b), 0);
-    if (it.rt < row_tiles_of<kTileRows>(p, it.s)) stream_item<Tr, D, NB, TP>(p, it, 0, lds_raw);
-    return;
-  }
-  const bool split = count_items<kTileRows>(p, true) <= p.max_items;
+  const bool split = p.part_units > 0 && count_items<kTileRows>(p, true) <= p.max_items;
   // (One round, unless the device tables hold more than the host planned for.)
-  for (int w = first;; w += gridDim.x) {
-    DraftItem it;
-    int local;
-    if (!find_request<kTileRows>(p, w, split, it.b, local, it.s)) break;
-    const int tiles = row_tiles_of<kTileRows>(p, it.s);
-    it.rt = local % tiles;
-    it.h = (local / tiles) % p.num_kv_heads;
-    it.part = local / (tiles * p.num_kv_heads);
-    it.parts = parts_of(p, it.s, split);
-    stream_item<Tr, D, NB, TP>(p, it, w, lds_raw);
+  for (int w = xcd_item(blockIdx.x, gridDim.x);; w += gridDim.x) {
+    const DraftItem it = find_item<kTileRows>(p, w, split);
+    if (it.b >= p.num_seqs) break;
+    if (it.rt < row_tiles_of<kTileRows>(p, it.s)) stream_item<Tr, D, NB, TP>(p, it, w, lds_raw);
     __syncthreads(); // the LDS is used again
   }
 }
 
 // out = sum_j 2^(m_j - M) o_j / sum_j 2^(m_j - M) l_j over the parts of each row
-// tile that was split; one thread per 4 elements.
+// tile that was split; one thread per 4 elements, 4 parts' loads in flight, one
+// pass with a running maximum.
 template <typename Tr, int D, int kTileRows>
 __global__ __launch_bounds__(256) void draft_merge_kernel(DraftAttentionParams p) {
   typedef typename Tr::elem T;
+  constexpr int kAhead = 4;
   const int c = blockIdx.x * 256 + threadIdx.x;
   const int rr = c / (D / 4), d = 4 * (c % (D / 4));
   int tile = blockIdx.y;
@@ -346,30 +333,48 @@ __global__ __launch_bounds__(256) void draft_merge_kernel(DraftAttentionParams p
   const int h = tile % p.num_kv_heads, b = tile / p.num_kv_heads;
   // Items before the request's, and of the whole call.
   int base = 0, total = 0;
+  DraftSeq s = {0, 0, 0};
   for (int b0 = 0; b0 < p.num_seqs; b0 += kWaveSize) {
     DraftSeq sl;
     const int n = items_of_lane<kTileRows>(p, b0, true, sl);
     const int incl = wave_inclusive_sum(n);
-    if (b >= b0 && b < b0 + kWaveSize) base = total + __builtin_amdgcn_readlane(incl - n, b - b0);
+    if (b >= b0 && b < b0 + kWaveSize) {
+      base = total + __builtin_amdgcn_readlane(incl - n, b - b0);
+      s = uniform_seq(sl, b - b0);
+    }
     total += __builtin_amdgcn_readlane(incl, kWaveSize - 1);
   }
   if (total > p.max_items) return; // nothing was split
-  const DraftSeq s = load_draft_seq(p, b);
   const int tiles = row_tiles_of<kTileRows>(p, s), parts = parts_of(p, s, true);
   const int rho = rt * kTileRows + rr;
   if (parts <= 1 || rr >= kTileRows || rho >= p.group_size * s.q_len) return;
   const int64_t stride = (int64_t)p.num_kv_heads * tiles * kTileRows; // rows from one part to the next
   const int64_t row0 = ((int64_t)base + h * tiles + rt) * kTileRows + rr;
-  float mmax = -INFINITY;
-  for (int j = 0; j < parts; j++) mmax = fmaxf(mmax, p.partial_ml[(row0 + j * stride) * 2]);
-  const float m_use = mmax == -INFINITY ? 0.f : mmax;
   float4v acc = {0.f, 0.f, 0.f, 0.f};
-  float sum = 0.f;
-  for (int j = 0; j < parts; j++) {
-    const float2v ml = *reinterpret_cast<const float2v*>(p.partial_ml + (row0 + j * stride) * 2);
-    const float w = __builtin_amdgcn_exp2f(ml[0] - m_use);
-    sum += w * ml[1];
-    acc += w * *reinterpret_cast<const float4v*>(p.partial_o + (row0 + j * stride) * D + d);
+  float sum = 0.f, m = -INFINITY;
+  for (int j0 = 0; j0 < parts; j0 += kAhead) {
+    float2v ml[kAhead];
+    float4v o[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; u++) { // (past the last part: the last again, with no weight)
+      const int64_t row = row0 + min(j0 + u, parts - 1) * stride;
+      ml[u] = *reinterpret_cast<const float2v*>(p.partial_ml + row * 2);
+      o[u] = *reinterpret_cast<const float4v*>(p.partial_o + row * D + d);
+    }
+    float m_new = m;
+#pragma unroll
+    for (int u = 0; u < kAhead; u++) m_new = fmaxf(m_new, ml[u][0]);
+    const float m_use = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(m - m_use);
+    acc *= alpha;
+    sum *= alpha;
+#pragma unroll
+    for (int u = 0; u < kAhead; u++) {
+      const float w = j0 + u < parts ? __builtin_amdgcn_exp2f(ml[u][0] - m_use) : 0.f;
+      sum += w * ml[u][1];
+      acc += w * o[u];
+    }
+    m = m_new;
   }
   const int r = rho / s.q_len, i = rho - r * s.q_len;
   T* dst = static_cast<T*>(p.out) + (int64_t)(h * p.group_size + r) * p.out_stride_head +

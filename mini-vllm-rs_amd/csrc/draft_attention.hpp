@@ -14,6 +14,20 @@ constexpr int kDraftUnitTokens = 64;
 // Parts of one row tile, at most.
 constexpr int kDraftMaxParts = 64;
 
+// Row tiles: 16 rows for every head dimension, 128 too, 32 and 64 up to 128.
+constexpr bool draft_tile_supported(int tile_rows, int head_dim) {
+  return tile_rows == 16 || tile_rows == 128 || ((tile_rows == 32 || tile_rows == 64) && head_dim <= 128);
+}
+
+// Blocks that a CU holds at once, by registers (16- and 32-row tiles, whose
+// wavefronts keep K and V chunks in them) and LDS (64 and 128 rows).
+constexpr int draft_blocks_per_cu(int tile_rows, bool f16, int head_dim) {
+  if (tile_rows == 16) return f16 ? (head_dim <= 128 ? 3 : head_dim <= 160 ? 2 : 1) : head_dim <= 96 ? 2 : 1;
+  if (tile_rows == 32) return f16 ? 2 : head_dim <= 64 ? 2 : 1;
+  if (tile_rows == 64) return f16 || head_dim <= 64 ? 2 : 1;
+  return head_dim <= 128 ? 2 : 1;
+}
+
 // One launch.  A row tile holds tile_rows grouped query rows rho = r * q_len +
 // i of one (request, KV head): r the query head within its group, i the draft.
 // An item is one part of one row tile's keys.

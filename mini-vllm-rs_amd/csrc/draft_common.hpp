@@ -63,11 +63,6 @@ struct DraftItem {
 // Items are numbered request by request, within a request part by part, KV head
 // by KV head, and the row tiles of one (KV head, part), which read the same keys,
 // next to each other.  One request per lane, 64 at a time.
-struct DraftScan {
-  int total;   // items of the whole call
-  bool split;  // false: more items than slots, every row tile is one item
-};
-
 template <int kTileRows>
 __device__ __forceinline__ int items_of_lane(const DraftAttentionParams& p, int b0, bool split, DraftSeq& s) {
   const int b = b0 + lane_id();
@@ -85,10 +80,15 @@ __device__ __forceinline__ int count_items(const DraftAttentionParams& p, bool s
   return total;
 }
 
-// The request of item w and the item's number within it (false: no such item).
+// The request of item w and the item's number within it (b = num_seqs: no such
+// item).
+struct FoundRequest {
+  int b, local;
+  DraftSeq s;
+};
+
 template <int kTileRows>
-__device__ __forceinline__ bool find_request(const DraftAttentionParams& p, int w, bool split, int& b_out, int& local,
-                                             DraftSeq& s_out) {
+__device__ __forceinline__ FoundRequest find_request(const DraftAttentionParams& p, int w, bool split) {
   for (int b0 = 0; b0 < p.num_seqs; b0 += kWaveSize) {
     DraftSeq s;
     const int n = items_of_lane<kTileRows>(p, b0, split, s);
@@ -96,14 +96,33 @@ __device__ __forceinline__ bool find_request(const DraftAttentionParams& p, int 
     const int sum = __builtin_amdgcn_readlane(incl, kWaveSize - 1);
     if (w < sum) {
       const int src = __builtin_ctzll(__ballot(w < incl));
-      b_out = b0 + src;
-      local = w - __builtin_amdgcn_readlane(incl - n, src);
-      s_out = uniform_seq(s, src);
-      return true;
+      return FoundRequest{b0 + src, w - __builtin_amdgcn_readlane(incl - n, src), uniform_seq(s, src)};
     }
     w -= sum;
   }
-  return false;
+  return FoundRequest{p.num_seqs, 0, DraftSeq{0, 0, 0}};
+}
+
+// Item w of the call (b = num_seqs: past the last one).  Calls that are not split
+// at all number a row tile for every request, KV head and row tile of the longest
+// request: nothing to scan (rt past the request's own row tiles: no work).
+template <int kTileRows>
+__device__ __forceinline__ DraftItem find_item(const DraftAttentionParams& p, int w, bool split) {
+  FoundRequest f;
+  int tiles, parts;
+  if (p.part_units == 0) {
+    tiles = p.row_tiles;
+    parts = 1;
+    f.b = min(w / (tiles * p.num_kv_heads), p.num_seqs);
+    f.local = w % (tiles * p.num_kv_heads);
+    f.s = uniform_seq(load_draft_seq(p, min(f.b, p.num_seqs - 1)), 0);
+  } else {
+    f = find_request<kTileRows>(p, w, split);
+    tiles = max(row_tiles_of<kTileRows>(p, f.s), 1);
+    parts = parts_of(p, f.s, split);
+  }
+  const int rest = f.local / tiles;
+  return DraftItem{f.b, rest % p.num_kv_heads, f.local % tiles, rest / p.num_kv_heads, parts, f.s};
 }
 
 // Block index -> item number: the blocks of one XCD (workgroups are dealt to

@@ -22,11 +22,11 @@ namespace mvr {
 namespace {
 
 typedef float float16v __attribute__((ext_vector_type(16)));
+typedef int int4v __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr float kRescaleThreshold = 8.0f; // log2 units
-constexpr int kStages = 2;                // LDS stages: one is read while the next one lands
 
 // 16 bytes per lane at `base` + the lane's byte offset straight into LDS at lds
 // + 16 * lane; lanes past `bytes` read zeros.  `base` and `lds` are wave-uniform.
@@ -37,18 +37,18 @@ __device__ __forceinline__ void load_to_lds16(const void* base, uint32_t bytes, 
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)lds, 16, offset, 0, 0, 0);
 }
 
-// Waits for this wavefront's tile loads and LDS reads, then meets the others.
-// (The compiler's own s_waitcnt, so that its count of the loads stays exact; the
-// empty asm keeps memory accesses on their side.)
-__device__ __forceinline__ void tile_barrier() {
-  __builtin_amdgcn_s_waitcnt(0x0070); // vmcnt(0) expcnt(7) lgkmcnt(0)
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
+// Waits until at most kNewer of this wavefront's tile loads are in flight.  (The
+// compiler's own s_waitcnt, so that its count of the loads stays exact; the empty
+// asm keeps memory accesses on their side.)
+template <int kNewer>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(kNewer < 64, "vmcnt has 6 bits");
+  __builtin_amdgcn_s_waitcnt((kNewer & 0xF) | ((kNewer >> 4) << 14) | (0x7 << 4) | (0xF << 8)); // vmcnt alone
   asm volatile("" ::: "memory");
 }
 
-// Waits for this wavefront's LDS accesses (its tile loads stay in flight), then
-// meets the others.
+// Waits for this wavefront's LDS accesses (tile loads stay in flight), then meets
+// the others.
 __device__ __forceinline__ void stage_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
@@ -79,7 +79,13 @@ struct Tile {
   }
 };
 
-template <int D, typename T, int RW, bool TP>
+// How a wavefront's loads find their pages: its run of 8 or 16 tokens lies in one
+// page (page sizes that are multiples of 16), or every load's whole token rows do
+// (multiples of the rows that 64 lanes of 16 bytes cover), or neither.
+enum PageRuns { kRuns, kWholeLoads, kAnyPages };
+
+// S: LDS stages; S - 1 steps' loads are in flight while a step is computed.
+template <int D, typename T, int RW, int PAGES, int S>
 __device__ __forceinline__ void tile_item(const DraftAttentionParams& p, const DraftItem& it, int64_t slot) {
   typedef Tile<D, T, RW> TL;
   constexpr bool kF32 = TL::kF32;
@@ -89,11 +95,15 @@ __device__ __forceinline__ void tile_item(const DraftAttentionParams& p, const D
   constexpr int kQFrags = kF32 ? D / 8 : D / 16;
   // One object per stage and operand: the compiler follows the loads into LDS by
   // object, so a read of one stage does not wait for another's.
-  __shared__ __attribute__((aligned(16))) T k_lds0[TL::kElems], k_lds1[TL::kElems];
-  __shared__ __attribute__((aligned(16))) T v_lds0[TL::kElems], v_lds1[TL::kElems];
+  __shared__ __attribute__((aligned(16))) T k_lds0[TL::kElems], k_lds1[TL::kElems], k_lds2[TL::kElems],
+      k_lds3[TL::kElems];
+  __shared__ __attribute__((aligned(16))) T v_lds0[TL::kElems], v_lds1[TL::kElems], v_lds2[TL::kElems],
+      v_lds3[TL::kElems];
   __shared__ float ml_xfer[RW][2][64]; // hand-off between groups (O goes through the stages)
-  T* const k_st[2] = {k_lds0, k_lds1};
-  T* const v_st[2] = {v_lds0, v_lds1};
+  __shared__ __attribute__((aligned(16))) int non_finite[S][kDraftWaves]; // by stage: what each wavefront loaded holds any
+  static_assert(S >= 2 && S <= 4, "2, 3 or 4 stages");
+  T* const k_st[4] = {k_lds0, k_lds1, k_lds2, k_lds3};
+  T* const v_st[4] = {v_lds0, v_lds1, v_lds2, v_lds3};
 
   const int l = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -130,6 +140,13 @@ __device__ __forceinline__ void tile_item(const DraftAttentionParams& p, const D
     for (int st = 0; st < kQFrags; st++)
       q[st] = valid ? *reinterpret_cast<const qfrag_t*>(qrow + kFragDims * st + (kFragDims / 2) * hh) : qfrag_t{};
   }
+  RowMask row_mask; // (its first words now: they are there when the drafts are)
+  {
+    bool valid;
+    int r, i;
+    row_of(valid, r, i);
+    row_mask = load_row_mask(p, s, valid, i);
+  }
 
   float16v o[D / 32];
 #pragma unroll
@@ -148,31 +165,45 @@ __device__ __forceinline__ void tile_item(const DraftAttentionParams& p, const D
   auto rows_at = [&](uint32_t page, uint32_t row) {
     return ((uint64_t)min(page, p.last_page) * page_rows + (head_rows + row)) * kRowBytes;
   };
-  uint32_t off_k[TL::kLoads], off_v[TL::kLoads]; // bytes from the wavefront's first token row (TP: within the row)
+  // Bytes from the wavefront's first token row (kWholeLoads: the load's; kAnyPages: within the row).
+  constexpr int kLoadTokens = PAGES == kWholeLoads ? 64 / TL::kChunksPerRow : 1;
+  static_assert(PAGES != kWholeLoads || 64 % TL::kChunksPerRow == 0, "loads of whole token rows");
+  uint32_t off_k[TL::kLoads], off_v[TL::kLoads];
 #pragma unroll
   for (int u = 0; u < TL::kLoads; u++) {
     const int P = (wave * TL::kLoads + u) * 64 + l;
     const int t = P / TL::kChunksPerRow, cs = P % TL::kChunksPerRow;
-    const int dt = TP ? 0 : t - wave * TL::kWaveTokens;
+    const int dt = PAGES == kRuns ? t - wave * TL::kWaveTokens : PAGES == kWholeLoads ? l / TL::kChunksPerRow : 0;
     off_k[u] = (uint32_t)(dt * D + TL::kChunkElems * (cs ^ TL::kswz(t))) * sizeof(T);
     off_v[u] = (uint32_t)(dt * D + TL::kChunkElems * (2 * ((cs >> 1) ^ TL::vswz(t)) + (cs & 1))) * sizeof(T);
   }
   const int n_steps = (j1 - j0 + G - 1) / G, last_step = n_steps - 1;
   const int last_key = s.seq_len - 1;
-  // First token that the wavefront stages in step si (the last key past the end:
-  // those tokens are masked).
-  auto first_token = [&](int si) {
-    return min((j0 + G * si) * kTileTokens + wave * TL::kWaveTokens, last_key);
+  // First token of the wavefront's load u in step si (kRuns: of all its loads), or
+  // the last key past the end (those tokens are masked).
+  auto first_token = [&](int si, int u) {
+    return min((j0 + G * si) * kTileTokens + wave * TL::kWaveTokens + u * kLoadTokens, last_key);
   };
-  // A block-table entry is read a step ahead of its loads: waiting for a scalar
+  // Block-table entries are read a step ahead of their loads: waiting for a scalar
   // load would also wait for every LDS read in flight.
-  auto fetch_page = [&](int si) { return TP ? 0u : (uint32_t)bt[page_div(first_token(si))]; };
-  auto issue_stage = [&](int si, uint32_t entry, T* kb, T* vb) {
+  struct Entries {
+    uint32_t page[PAGES == kWholeLoads ? TL::kLoads : 1];
+  };
+  auto fetch_pages = [&](int si) {
+    Entries e{};
+    if constexpr (PAGES == kRuns) e.page[0] = (uint32_t)bt[page_div(first_token(si, 0))];
+    if constexpr (PAGES == kWholeLoads) {
+#pragma unroll
+      for (int u = 0; u < TL::kLoads; u++) e.page[u] = (uint32_t)bt[page_div(first_token(si, u))];
+    }
+    return e;
+  };
+  auto issue_stage = [&](int si, const Entries& entries, T* kb, T* vb) {
     const char* kpool = static_cast<const char*>(p.key_pool);
     const char* vpool = static_cast<const char*>(p.value_pool);
-    if constexpr (TP) {
-      // Pages that do not hold whole runs of kWaveTokens: a load's tokens may lie
-      // in several pages, which take their lanes in turn.  Lanes of tokens past
+    if constexpr (PAGES == kAnyPages) {
+      // A load's tokens may lie in several pages, which take their lanes in turn.
+      // Lanes of tokens past
       // the last key go with the last page, whose bound reads them as zeros.
       const int last_page_index = page_div(last_key);
 #pragma unroll
@@ -194,11 +225,18 @@ __device__ __forceinline__ void tile_item(const DraftAttentionParams& p, const D
         }
       }
     } else {
-      const int t = first_token(si), row0 = t - page_div(t) * p.page_size;
-      const uint64_t at = rows_at(entry, (uint32_t)row0);
-      const uint32_t bytes = (uint32_t)min(min(p.page_size - row0, s.seq_len - t), TL::kWaveTokens) * kRowBytes;
+      // All wave-uniform: a run's first token, its page row, and the bytes from
+      // there to the run's end, or the end of the keys.
+      constexpr int kRunTokens = PAGES == kRuns ? TL::kWaveTokens : kLoadTokens;
+      uint64_t at = 0;
+      uint32_t bytes = 0;
 #pragma unroll
       for (int u = 0; u < TL::kLoads; u++) {
+        if (u == 0 || PAGES == kWholeLoads) {
+          const int t = first_token(si, u);
+          at = rows_at(entries.page[PAGES == kWholeLoads ? u : 0], (uint32_t)(t - page_div(t) * p.page_size));
+          bytes = (uint32_t)min(s.seq_len - t, kRunTokens) * kRowBytes;
+        }
         const int dst = (wave * TL::kLoads + u) * 64 * TL::kChunkElems;
         load_to_lds16(kpool + at, bytes, off_k[u], kb + dst);
         load_to_lds16(vpool + at, bytes, off_v[u], vb + dst);
@@ -312,15 +350,9 @@ __device__ __forceinline__ void tile_item(const DraftAttentionParams& p, const D
     }
   };
   // A draft's V may hold infinities and NaN: in a product, 0 times one of those
-  // would reach the rows that do not see the draft.  Where a stage holds any, they
-  // are added to the rows that see them one by one, and cleared before the product.
-  auto has_non_finite = [&](const T* vb) { // the whole stage: the same answer for every wavefront
-    bool bad = false;
-#pragma unroll 2
-    for (int c = 0; c < TL::kElems / TL::kChunkElems / 64; c++)
-      bad |= any_non_finite(*reinterpret_cast<const qfrag_t*>(vb + (c * 64 + l) * TL::kChunkElems));
-    return __any(bad);
-  };
+  // would reach the rows that do not see the draft.  Each wavefront looks
+  // at what it loaded as it lands; where a stage holds any, they are added to the
+  // rows that see them one by one, and cleared before the product.
   auto clear_non_finite = [&](T* vb) {
 #pragma unroll 1
     for (int c = wave; c < TL::kElems / TL::kChunkElems / 64; c += kDraftWaves) {
@@ -352,7 +384,7 @@ __device__ __forceinline__ void tile_item(const DraftAttentionParams& p, const D
   // Every stage starts zeroed: a lane past its bound reads zeros, and should it
   // leave its bytes unwritten instead, they hold zeros or keys of this call.
 #pragma unroll
-  for (int a = 0; a < kStages; a++)
+  for (int a = 0; a < S; a++)
 #pragma unroll
     for (int u = 0; u < TL::kLoads; u++) {
       const int e = ((wave * TL::kLoads + u) * 64 + l) * TL::kChunkElems;
@@ -360,16 +392,37 @@ __device__ __forceinline__ void tile_item(const DraftAttentionParams& p, const D
       *reinterpret_cast<u32x4*>(v_st[a] + e) = u32x4{0u, 0u, 0u, 0u};
     }
   __builtin_amdgcn_s_waitcnt(0xC07F); // lgkmcnt(0)
-  issue_stage(0, fetch_page(0), k_st[0], v_st[0]);
-  uint32_t next_entry = fetch_page(min(1, last_step));
-  tile_barrier(); // step 0 has landed
-
-  // Step si reads stage si % 2 while step si + 1 lands in the other one, whose
-  // readers met at the last barrier.  (Loads past the last step repeat it, into a
-  // stage that nobody reads again.)
-  auto clear_step = [&](int si, auto stage) {
+  // Tiles j < clear_tiles end before the drafts and need no masks: whole rounds of
+  // S steps of them come first.
+  const int clear_tiles = min(j1, max(prefix, 0) / kTileTokens);
+  const int clear_steps = max(0, (clear_tiles - j0) / G) / S * S;
+  // Step si's stage lands: this wavefront's loads of it (the S - 2 steps after it
+  // stay in flight; loads by page as many as there are pages, so there all), then
+  // everybody's.
+  auto land = [&](int si, auto stage) {
     constexpr int st = decltype(stage)::value;
-    issue_stage(min(si + 1, last_step), next_entry, k_st[1 - st], v_st[1 - st]);
+    wait_loads<PAGES == kAnyPages ? 0 : (S - 2) * 2 * TL::kLoads>();
+    if (si >= clear_steps) {
+      bool bad = false;
+#pragma unroll
+      for (int u = 0; u < TL::kLoads; u++)
+        bad |= any_non_finite(
+            *reinterpret_cast<const qfrag_t*>(v_st[st] + ((wave * TL::kLoads + u) * 64 + l) * TL::kChunkElems));
+      non_finite[st][wave] = __any(bad);
+    }
+    stage_barrier();
+  };
+#pragma unroll
+  for (int a = 0; a < S - 1; a++) issue_stage(min(a, last_step), fetch_pages(min(a, last_step)), k_st[a], v_st[a]);
+  Entries next_pages = fetch_pages(min(S - 1, last_step));
+  land(0, std::integral_constant<int, 0>());
+
+  // Step si reads stage si % S; meanwhile step si + S - 1 lands in the stage that
+  // step si - 1 read, whose readers met at the last barrier.  (Loads past the last
+  // step repeat it, into stages that nobody reads again.)
+  auto clear_step = [&](int si, auto stage) {
+    constexpr int st = decltype(stage)::value, into = (st + S - 1) % S;
+    issue_stage(min(si + S - 1, last_step), next_pages, k_st[into], v_st[into]);
     if (live) {
       float16v sc[kSub];
       qk(k_st[st], sc);
@@ -377,15 +430,16 @@ __device__ __forceinline__ void tile_item(const DraftAttentionParams& p, const D
       exps(sc);
       pv(v_st[st], sc);
     }
-    next_entry = fetch_page(min(si + 2, last_step));
-    tile_barrier();
+    next_pages = fetch_pages(min(si + S, last_step));
+    land(si + 1, std::integral_constant<int, (st + 1) % S>());
   };
-  auto draft_step = [&](int si, const RowMask& row_mask, auto stage) {
-    constexpr int st = decltype(stage)::value;
-    issue_stage(min(si + 1, last_step), next_entry, k_st[1 - st], v_st[1 - st]);
+  auto draft_step = [&](int si, auto stage) {
+    constexpr int st = decltype(stage)::value, into = (st + S - 1) % S;
+    issue_stage(min(si + S - 1, last_step), next_pages, k_st[into], v_st[into]);
     const int j = j0 + G * si + grp;
     const bool works = live && j < j1;
-    const bool bad = has_non_finite(v_st[st]);
+    const int4v flags = *reinterpret_cast<const int4v*>(non_finite[st]);
+    const bool bad = __builtin_amdgcn_readfirstlane(flags[0] | flags[1] | flags[2] | flags[3]);
     float16v sc[kSub];
     uint32_t bits[kSub];
     if (works) {
@@ -407,28 +461,34 @@ __device__ __forceinline__ void tile_item(const DraftAttentionParams& p, const D
       stage_barrier();
     }
     if (works) pv(v_st[st], sc);
-    next_entry = fetch_page(min(si + 2, last_step));
-    tile_barrier();
+    next_pages = fetch_pages(min(si + S, last_step));
+    land(si + 1, std::integral_constant<int, (st + 1) % S>());
   };
-  // Tiles before the drafts need no masks: whole rounds of two steps of them first.
-  const int clear_tiles = min(j1, max(prefix, 0) / kTileTokens); // tiles j < this are clear
-  const int clear_steps = max(0, (clear_tiles - j0) / G) / 2 * 2;
-  for (int si = 0; si < clear_steps; si += 2) {
-    clear_step(si, std::integral_constant<int, 0>());
-    clear_step(si + 1, std::integral_constant<int, 1>());
+#define MVR_STAGE(K) std::integral_constant<int, K>()
+  // (Each stage is named statically.)
+  for (int si = 0; si < clear_steps; si += S) {
+    clear_step(si, MVR_STAGE(0));
+    clear_step(si + 1, MVR_STAGE(1));
+    if constexpr (S >= 3) clear_step(si + 2, MVR_STAGE(2));
+    if constexpr (S == 4) clear_step(si + 3, MVR_STAGE(3));
   }
-  if (clear_steps < n_steps) {
-    bool valid;
-    int r, i;
-    row_of(valid, r, i);
-    const RowMask row_mask = load_row_mask(p, s, valid, i);
-    for (int si = clear_steps; si < n_steps; si += 2) {
-      draft_step(si, row_mask, std::integral_constant<int, 0>());
-      if (si + 1 >= n_steps) break;
-      draft_step(si + 1, row_mask, std::integral_constant<int, 1>());
+  for (int si = clear_steps; si < n_steps; si += S) {
+    draft_step(si, MVR_STAGE(0));
+    if (si + 1 >= n_steps) break;
+    draft_step(si + 1, MVR_STAGE(1));
+    if constexpr (S >= 3) {
+      if (si + 2 >= n_steps) break;
+      draft_step(si + 2, MVR_STAGE(2));
+    }
+    if constexpr (S == 4) {
+      if (si + 3 >= n_steps) break;
+      draft_step(si + 3, MVR_STAGE(3));
     }
   }
-  // (The last barrier waited for every load: the stages are free.)
+#undef MVR_STAGE
+  // Every load has landed, everybody's, before the stages are used again.
+  wait_loads<0>();
+  __syncthreads();
 
   // Group 1 hands its state to group 0: part n of O of row wavefront rw as 4 x 64
   // float4, 1024 floats from float (n * RW + rw) * 1024 of the stages.
@@ -504,50 +564,53 @@ __device__ __forceinline__ void tile_item(const DraftAttentionParams& p, const D
   }
 }
 
-// Blocks per CU that LDS and registers allow.
 template <int D, typename T, int RW>
-constexpr int tile_blocks() {
-  return D <= 128 && !(sizeof(T) == 4 && RW == 2 && D > 64) ? 2 : 1;
+constexpr int stage_bytes() { // of K and V
+  return 2 * Tile<D, T, RW>::kElems * (int)sizeof(T);
 }
 
-template <int D, typename T, int RW, bool TP>
-__global__ __launch_bounds__(kWaveSize* kDraftWaves, (tile_blocks<D, T, RW>())) void draft_tile_kernel(
+template <int D, typename T, int RW, int PAGES, int S>
+__global__ __launch_bounds__(kWaveSize* kDraftWaves, (draft_blocks_per_cu(32 * RW, sizeof(T) == 2, D))) void draft_tile_kernel(
     DraftAttentionParams p) {
   constexpr int kTileRows = 32 * RW;
-  const int first = xcd_item(blockIdx.x, gridDim.x);
-  DraftItem it;
-  if (p.part_units == 0) {
-    it.rt = first % p.row_tiles;
-    it.h = (first / p.row_tiles) % p.num_kv_heads;
-    it.b = first / (p.row_tiles * p.num_kv_heads);
-    it.part = 0, it.parts = 1;
-    it.s = uniform_seq(load_draft_seq(p, it.b), 0);
-    if (it.rt >= row_tiles_of<kTileRows>(p, it.s)) return;
-    tile_item<D, T, RW, TP>(p, it, 0);
-    return;
-  }
-  const bool split = count_items<kTileRows>(p, true) <= p.max_items;
-  for (int w = first;; w += gridDim.x) {
-    int local;
-    if (!find_request<kTileRows>(p, w, split, it.b, local, it.s)) break;
-    const int tiles = row_tiles_of<kTileRows>(p, it.s);
-    it.rt = local % tiles;
-    it.h = (local / tiles) % p.num_kv_heads;
-    it.part = local / (tiles * p.num_kv_heads);
-    it.parts = parts_of(p, it.s, split);
-    tile_item<D, T, RW, TP>(p, it, w);
+  // (One call of tile_item: its code, twice, would crowd the instruction cache.)
+  const bool split = p.part_units > 0 && count_items<kTileRows>(p, true) <= p.max_items;
+  for (int w = xcd_item(blockIdx.x, gridDim.x);; w += gridDim.x) {
+    const DraftItem it = find_item<kTileRows>(p, w, split);
+    if (it.b >= p.num_seqs) break;
+    if (it.rt < row_tiles_of<kTileRows>(p, it.s)) tile_item<D, T, RW, PAGES, S>(p, it, w);
     __syncthreads(); // the LDS is used again
   }
 }
 
+template <int D, typename T, int RW, int S>
+hipError_t launch_stages(const DraftAttentionPlan& plan, const DraftAttentionParams& p, hipStream_t stream) {
+  typedef Tile<D, T, RW> TL;
+  const dim3 grid((unsigned)plan.blocks), block(kWaveSize * kDraftWaves);
+  if (p.page_size % kChunkTokens == 0) { // a wavefront's 8 or 16 tokens lie in one page
+    hipLaunchKernelGGL((draft_tile_kernel<D, T, RW, kRuns, S>), grid, block, 0, stream, p);
+    return hipGetLastError();
+  }
+  if constexpr (D == 64 || D == 128) {
+    if (p.page_size % (64 / TL::kChunksPerRow) == 0) {
+      hipLaunchKernelGGL((draft_tile_kernel<D, T, RW, kWholeLoads, S>), grid, block, 0, stream, p);
+      return hipGetLastError();
+    }
+  }
+  // (Its loads are waited for as a whole: two stages.)
+  hipLaunchKernelGGL((draft_tile_kernel<D, T, RW, kAnyPages, 2>), grid, block, 0, stream, p);
+  return hipGetLastError();
+}
+
+// Stages: as many as two blocks per CU leave room for, 4 at most (2 at head_dim
+// 128).  4 stages and one block per CU there made no difference, 112 blocks of 33
+// steps included (39.5 us): a lone block's step waits for its own chain of product,
+// softmax and product, not for its loads.
 template <int D, typename T, int RW>
 hipError_t launch_rows(const DraftAttentionPlan& plan, const DraftAttentionParams& p, hipStream_t stream) {
-  const dim3 grid((unsigned)plan.blocks), block(kWaveSize * kDraftWaves);
-  if (p.page_size % kChunkTokens == 0) // a wavefront's 8 or 16 tokens lie in one page
-    hipLaunchKernelGGL((draft_tile_kernel<D, T, RW, false>), grid, block, 0, stream, p);
-  else
-    hipLaunchKernelGGL((draft_tile_kernel<D, T, RW, true>), grid, block, 0, stream, p);
-  return hipGetLastError();
+  constexpr int kBytes = stage_bytes<D, T, RW>();
+  constexpr int kStages = 78 * 1024 / kBytes >= 4 ? 4 : 78 * 1024 / kBytes >= 3 ? 3 : 2;
+  return launch_stages<D, T, RW, kStages>(plan, p, stream);
 }
 
 template <int D>
