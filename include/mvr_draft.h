@@ -100,7 +100,7 @@ typedef struct mvr_head_norms {
    The row of token i of request b goes to slot seq_len - q_len + i, wherever
    it is rotated to.  Arguments are mvr_rope_append's; here
      - a request may have q_len 0, and total_q may exceed cu_q_lens[num_seqs]
-       (a padded batch): rows from there on are neither read nor written;
+       (a padded batch): rows from there on do not matter and are not written;
      - rope_len need only cover the positions: rows whose position is outside
        [0, rope_len), or whose slot is outside [0, max_seq_len), or whose page
        is outside the pool, are left out. */

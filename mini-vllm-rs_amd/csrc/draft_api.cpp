@@ -357,6 +357,10 @@ static int check_norm_rope_append(const mvr_rope_append_args* a, const mvr_head_
   if (!a->q || !a->k || !a->v || !a->cos_table || !a->sin_table || !a->block_tables || !a->q_out || !a->key_pool ||
       !a->value_pool)
     return fail(MVR_E_INVALID_ARGUMENT, "null tensor, table or pool pointer");
+  // Blocks of 4 wavefronts, a row at least in each wavefront.
+  if ((int64_t)a->total_q * ((int64_t)a->num_q_heads + 2 * a->num_kv_heads) > INT32_MAX)
+    return fail(MVR_E_UNSUPPORTED, "%d tokens of %d and 2 x %d heads are more than one call takes", a->total_q,
+                a->num_q_heads, a->num_kv_heads);
   if (!(n->eps >= 0.f) || !isfinite(n->eps)) return fail(MVR_E_INVALID_ARGUMENT, "eps must be finite and >= 0");
   const size_t align = a->dtype == MVR_DTYPE_F16 ? 8 : 16; // every access moves 4 elements
   const void* ptrs[] = {a->q,        a->k,          a->v,       a->cos_table, a->sin_table, a->q_out,
