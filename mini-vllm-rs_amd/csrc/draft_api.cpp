@@ -61,6 +61,8 @@ int check_tree(const mvr_paged_attention_args* a, const mvr_draft_trees* t) {
   if (a->num_seqs == 1 && !a->cu_q_lens && a->total_q > 0 && a->total_q < a->max_q_len)
     return fail(MVR_E_INVALID_ARGUMENT, "total_q %d is smaller than max_q_len %d, the q_len of a call without cu_q_lens",
                 a->total_q, a->max_q_len);
+  if (a->max_seq_len > INT32_MAX - 1024) // (positions of whole key tiles are counted in 32 bits)
+    return fail(MVR_E_UNSUPPORTED, "max_seq_len %d is too close to 2^31", a->max_seq_len);
   if (!t->masks) return fail(MVR_E_INVALID_ARGUMENT, "masks is null");
   if ((uintptr_t)t->masks % sizeof(uint32_t)) return fail(MVR_E_INVALID_ARGUMENT, "masks must be 4-byte aligned");
   if (t->mask_words < (a->max_q_len - 1) / 32 + 1)

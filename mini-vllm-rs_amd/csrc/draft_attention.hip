@@ -172,11 +172,12 @@ __device__ __forceinline__ void stream_item(const DraftAttentionParams& p, const
   auto process_drafts = [&](int k, const RowMask (&mask)[NB], const typename Tr::kreg_t (&kr)[Tr::kLoads],
                             typename Tr::vreg_t (&vr)[Tr::kLoads]) {
     const int tok0 = k * kChunkTokens, tokens = min(s.seq_len - tok0, kChunkTokens);
-    asm volatile("" ::: "memory");
-    Tr::stage_v(lds, l, tokens, vr);
+    int le = l;
+    asm volatile("" : "+v"(le)::"memory");
+    Tr::stage_v(lds, le, tokens, vr);
     bool bad = false;
 #pragma unroll
-    for (int u = 0; u < Tr::kLoads; u++) bad |= Tr::v_row(l, u) < tokens && any_non_finite(vr[u]);
+    for (int u = 0; u < Tr::kLoads; u++) bad |= Tr::v_row(le, u) < tokens && any_non_finite(vr[u]);
     uint32_t vis[NB]; // of the chunk's tokens
     float pr[NB][4];
 #pragma unroll
@@ -208,10 +209,10 @@ __device__ __forceinline__ void stream_item(const DraftAttentionParams& p, const
 #pragma unroll
         for (int e = 0; e < (int)(sizeof(vr[u]) / sizeof(T)); e++) vr[u][e] = finite_or_zero(vr[u][e]);
       asm volatile("" ::: "memory"); // (a wavefront's LDS accesses complete in order)
-      Tr::stage_v(lds, l, tokens, vr);
+      Tr::stage_v(lds, le, tokens, vr);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
-    Tr::template pv<NB>(lds, l, pr, o);
+    Tr::template pv<NB>(lds, le, pr, o);
   };
 
   // kDepth chunks in flight; a tail past k1 reloads chunk k1 - 1 (an L2 hit)
@@ -308,10 +309,9 @@ __global__ __launch_bounds__(kWaveSize* kDraftWaves, (stream_blocks<Tr, D, NB, T
   constexpr size_t kTileBytes = (size_t)kDraftWaves * kChunkTokens * D * sizeof(typename Tr::elem);
   constexpr size_t kMergeBytes = (size_t)kDraftWaves * kTileRows * (D + 4 + 2) * sizeof(float);
   __shared__ __attribute__((aligned(16))) char lds_raw[kTileBytes > kMergeBytes ? kTileBytes : kMergeBytes];
-  const bool split = p.part_units > 0 && count_items<kTileRows>(p, true) <= p.max_items;
   // (One round, unless the device tables hold more than the host planned for.)
   for (int w = xcd_item(blockIdx.x, gridDim.x);; w += gridDim.x) {
-    const DraftItem it = find_item<kTileRows>(p, w, split);
+    const DraftItem it = find_item<kTileRows>(p, w);
     if (it.b >= p.num_seqs) break;
     if (it.rt < row_tiles_of<kTileRows>(p, it.s)) stream_item<Tr, D, NB, TP>(p, it, w, lds_raw);
     __syncthreads(); // the LDS is used again
@@ -325,9 +325,10 @@ template <typename Tr, int D, int kTileRows>
 __global__ __launch_bounds__(256) void draft_merge_kernel(DraftAttentionParams p) {
   typedef typename Tr::elem T;
   constexpr int kAhead = 4;
-  const int c = blockIdx.x * 256 + threadIdx.x;
+  constexpr int kTileBlocks = (kTileRows * (D / 4) + 255) / 256;
+  const int c = (int)(blockIdx.x % kTileBlocks) * 256 + threadIdx.x;
   const int rr = c / (D / 4), d = 4 * (c % (D / 4));
-  int tile = blockIdx.y;
+  int tile = (int)(blockIdx.x / kTileBlocks);
   const int rt = tile % p.row_tiles;
   tile /= p.row_tiles;
   const int h = tile % p.num_kv_heads, b = tile / p.num_kv_heads;
@@ -394,8 +395,8 @@ hipError_t launch_stream(const DraftAttentionPlan& plan, const DraftAttentionPar
 
 template <typename Tr, int D, int kTileRows>
 hipError_t launch_merge(const DraftAttentionParams& p, hipStream_t stream) {
-  constexpr int kCells = kTileRows * (D / 4);
-  const dim3 grid((kCells + 255) / 256, (unsigned)(p.num_seqs * p.num_kv_heads * p.row_tiles));
+  constexpr int kTileBlocks = (kTileRows * (D / 4) + 255) / 256;
+  const dim3 grid((unsigned)kTileBlocks * (unsigned)(p.num_seqs * p.num_kv_heads * p.row_tiles));
   hipLaunchKernelGGL((draft_merge_kernel<Tr, D, kTileRows>), grid, dim3(256), 0, stream, p);
   return hipGetLastError();
 }

@@ -70,44 +70,37 @@ __device__ __forceinline__ int items_of_lane(const DraftAttentionParams& p, int 
   return b < p.num_seqs ? row_tiles_of<kTileRows>(p, s) * parts_of(p, s, split) * p.num_kv_heads : 0;
 }
 
-template <int kTileRows>
-__device__ __forceinline__ int count_items(const DraftAttentionParams& p, bool split) {
-  int total = 0;
-  for (int b0 = 0; b0 < p.num_seqs; b0 += kWaveSize) {
-    DraftSeq s;
-    total += __builtin_amdgcn_readlane(wave_inclusive_sum(items_of_lane<kTileRows>(p, b0, split, s)), kWaveSize - 1);
-  }
-  return total;
-}
-
-// The request of item w and the item's number within it (b = num_seqs: no such
-// item).
+// The request of item w (b = num_seqs: no such item), the item's number within it,
+// and the items of the whole call.
 struct FoundRequest {
-  int b, local;
+  int b, local, total;
   DraftSeq s;
 };
 
 template <int kTileRows>
 __device__ __forceinline__ FoundRequest find_request(const DraftAttentionParams& p, int w, bool split) {
+  FoundRequest f = {p.num_seqs, 0, 0, DraftSeq{0, 0, 0}};
   for (int b0 = 0; b0 < p.num_seqs; b0 += kWaveSize) {
     DraftSeq s;
     const int n = items_of_lane<kTileRows>(p, b0, split, s);
     const int incl = wave_inclusive_sum(n);
-    const int sum = __builtin_amdgcn_readlane(incl, kWaveSize - 1);
-    if (w < sum) {
-      const int src = __builtin_ctzll(__ballot(w < incl));
-      return FoundRequest{b0 + src, w - __builtin_amdgcn_readlane(incl - n, src), uniform_seq(s, src)};
+    const int sum = __builtin_amdgcn_readlane(incl, kWaveSize - 1), at = w - f.total;
+    if (at >= 0 && at < sum) {
+      const int src = __builtin_ctzll(__ballot(at < incl));
+      f.b = b0 + src;
+      f.local = at - __builtin_amdgcn_readlane(incl - n, src);
+      f.s = uniform_seq(s, src);
     }
-    w -= sum;
+    f.total += sum;
   }
-  return FoundRequest{p.num_seqs, 0, DraftSeq{0, 0, 0}};
+  return f;
 }
 
 // Item w of the call (b = num_seqs: past the last one).  Calls that are not split
 // at all number a row tile for every request, KV head and row tile of the longest
 // request: nothing to scan (rt past the request's own row tiles: no work).
 template <int kTileRows>
-__device__ __forceinline__ DraftItem find_item(const DraftAttentionParams& p, int w, bool split) {
+__device__ __forceinline__ DraftItem find_item(const DraftAttentionParams& p, int w) {
   FoundRequest f;
   int tiles, parts;
   if (p.part_units == 0) {
@@ -117,7 +110,9 @@ __device__ __forceinline__ DraftItem find_item(const DraftAttentionParams& p, in
     f.local = w % (tiles * p.num_kv_heads);
     f.s = uniform_seq(load_draft_seq(p, min(f.b, p.num_seqs - 1)), 0);
   } else {
-    f = find_request<kTileRows>(p, w, split);
+    f = find_request<kTileRows>(p, w, true);
+    const bool split = f.total <= p.max_items;
+    if (!split) f = find_request<kTileRows>(p, w, false); // more items than slots: every row tile is one
     tiles = max(row_tiles_of<kTileRows>(p, f.s), 1);
     parts = parts_of(p, f.s, split);
   }

@@ -190,21 +190,36 @@ class Call:
             _refuse(f"a stream of {stream.device} for tensors of {device}")
 
     def __call__(self):
-        cuda = self._cuda
-        if cuda.current_device() != self._device.index:
+        cuda, index = self._cuda, self._device.index
+        if cuda.current_device() != index:
             with cuda.device(self._device):
                 return self()
-        stream = self._stream
-        if stream is None:
-            stream = cuda.current_stream()
-        elif stream != cuda.current_stream():
-            # Freed on their own stream before the kernels ran, their memory must not be handed out meanwhile.
-            for t in self._tensors:
-                t.record_stream(stream)
-            if self.workspace is not None:
-                self.workspace.record_stream(stream)
-        self.args.stream = stream.cuda_stream
+        current = _raw_current_stream(index)
+        if self._stream is None:
+            self.args.stream = current
+        else:
+            self.args.stream = self._stream.cuda_stream
+            if self._stream.cuda_stream != current:
+                # Freed on their own stream before the kernels ran, their memory must not be handed out meanwhile.
+                for t in self._tensors:
+                    t.record_stream(self._stream)
+                if self.workspace is not None:
+                    self.workspace.record_stream(self._stream)
         _check(self._function(*self._refs))
+
+
+def _raw_current_stream(index):
+    """Handle of the device's current stream.  (torch.cuda.current_stream() makes a Stream object: 2.7 us against 0.1,
+    where a whole small call takes 3.)"""
+    global _raw_stream
+    if _raw_stream is None:
+        torch = M._torch()
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                              lambda i: torch.cuda.current_stream(i).cuda_stream)
+    return _raw_stream(index)
+
+
+_raw_stream = None
 
 
 def _scope(device, stream):

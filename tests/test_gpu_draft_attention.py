@@ -107,6 +107,28 @@ def test_stale_hints_cost_no_rows(stale):
     check_attention(got, b)
 
 
+def test_stale_hints_that_plan_too_few_parts():
+    """Hints of one long request where all are long: more parts than the workspace was planned for, so nothing is split
+    and the blocks go on to the tiles that the grid has none for."""
+    b = Batch(50, F16, 8, 2, 128, 16, [2500, 2400, 2300, 2600], [12, 30, 1, 8], "tree")
+    lens = np.array([40, 40, 2301, 40], np.int32)
+    a = D.make_tree_call(**b.device(), out=b.device()["q"], max_q_len=b.max_q, max_seq_len=b.max_len,
+                         seq_lens_host=lens, cu_q_lens_host=b.cu, sum_seq_lens=int(lens.sum()))
+    assert a.args.workspace_bytes > 0
+    check_attention(run(b, seq_lens_host=lens, sum_seq_lens=int(lens.sum())), b)
+    check_attention(run(b, hints=False, sum_seq_lens=int(b.seq_lens.sum())), b, note="the sum alone")
+
+
+def test_thousands_of_empty_requests():
+    """A padded batch of 3,000, three of them with drafts; over 2^16 row tiles in the grid of the merge."""
+    q, cached = np.zeros(3000, np.int64), np.zeros(3000, np.int64)
+    for s, n, c in ((5, 60, 1500), (1777, 3, 2000), (2999, 1, 700)):
+        q[s], cached[s] = n, c
+    b = Batch(51, F16, 16, 2, 64, 16, cached, q, "tree")
+    check_attention(run(b), b)
+    check_attention(run(b, hints=False), b)
+
+
 def test_many_requests():
     """More requests than one scan holds, a third of them empty."""
     rng = np.random.default_rng(6)
@@ -302,6 +324,51 @@ def test_graph(cached, nodes):
         for o in outs:
             assert torch.equal(o, eager)
         check_attention(outs[0], other)
+
+
+def test_graph_replayed_for_other_lengths():
+    """A graph captured for one batch, replayed with the tables of others within its bounds: longer and shorter
+    contexts, other trees, empty requests."""
+    hkv, d, width = 2, 128, 200
+    pages = 4 * width
+    first = Batch(60, F16, 8, hkv, d, 16, [2500, 60, 1200, 9], [20, 7, 1, 33], "tree", spare=pages)
+    t = first.device()
+    t["block_tables"] = torch.zeros((4, width), dtype=torch.int32, device="cuda")
+    t["block_tables"][:, :first.table.shape[1]] = torch.from_numpy(first.table).cuda()
+    tokens, max_q, max_len = 160, 40, 3000
+    for k, shape in (("q", (8, tokens, d)), ("masks", (tokens, 2))):
+        big = torch.zeros(shape, dtype=t[k].dtype, device="cuda")
+        if k == "q":
+            big[:, :t[k].shape[1]] = t[k]
+        else:
+            big[:t[k].shape[0], :t[k].shape[1]] = t[k]
+        t[k] = big
+    out = torch.zeros_like(t["q"])
+    call = D.make_tree_call(**t, out=out, max_q_len=max_q, max_seq_len=max_len, seq_lens_host=first.seq_lens,
+                            cu_q_lens_host=first.cu, sum_seq_lens=int(first.seq_lens.sum()))
+    assert call.args.workspace_bytes > 0
+    call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call()
+    for seed, cached, q in ((61, [2900, 2900, 2900, 2900], [40, 40, 40, 40]), (62, [0, 5, 0, 1], [1, 1, 2, 3]),
+                            (63, [100, 0, 2000, 700], [0, 40, 0, 12]), (60, first.cached, first.q_lens)):
+        b = Batch(seed, F16, 8, hkv, d, 16, cached, q, "tree", words=2)
+        new = b.device()
+        t["key_pool"][:b.num_pages].copy_(new["key_pool"])
+        t["value_pool"][:b.num_pages].copy_(new["value_pool"])
+        t["q"][:, :b.queries.shape[1]].copy_(new["q"])
+        t["masks"][:b.masks.shape[0]].copy_(new["masks"])
+        t["block_tables"][:, :b.table.shape[1]].copy_(new["block_tables"])
+        t["seq_lens"].copy_(new["seq_lens"])
+        t["cu_q_lens"].copy_(new["cu_q_lens"])
+        out.fill_(9.0)
+        g.replay()
+        torch.cuda.synchronize()
+        check_attention(out[:, :b.queries.shape[1]], b, note=str(seed))
+        assert bool((out[:, int(b.cu[-1]):] == 9.0).all())
+        check_attention(run(b, dict(new)), b, note=f"eager {seed}")
 
 
 def test_streams():
