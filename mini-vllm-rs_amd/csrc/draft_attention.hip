@@ -12,6 +12,8 @@
 // seen by every row, and take no mask, no test and no table read.
 #include "draft_common.hpp"
 
+#include <type_traits>
+
 namespace mvr {
 namespace {
 
@@ -20,11 +22,10 @@ namespace {
 // its share of the part's 16-token chunks straight from the cache; their
 // results merge in LDS.
 // ---------------------------------------------------------------------------
-// Chunks in flight per wavefront: two, one where two would not fit the registers
-// (F32 rows of more than 128 elements hold a chunk of K and V in 160 to 256).
-template <typename Tr, int D>
-constexpr int stream_depth() {
-  return sizeof(typename Tr::elem) == 4 && D > 128 ? 1 : 2;
+// Chunks of one step: two of F16, whose softmax and products are then one of 32 keys.
+template <typename Tr>
+constexpr int step_chunks() {
+  return sizeof(typename Tr::elem) == 4 ? 1 : 2;
 }
 
 // Blocks per CU (wavefronts per SIMD): what the planner counts on, where the
@@ -41,18 +42,19 @@ constexpr int stream_blocks() {
 // of its own to look up.
 template <typename Tr, int D, int NB, bool TP>
 __device__ __forceinline__ void stream_item(const DraftAttentionParams& p, const DraftItem& it, int64_t slot,
-                                            char* lds_raw) {
+                                            int wave, char* lds_raw) {
   typedef typename Tr::elem T;
   constexpr int kTileRows = 16 * NB;
   constexpr int kMergeStride = D + 4;
   constexpr int kUnitChunks = kDraftUnitTokens / kChunkTokens;
-  constexpr int kDepth = stream_depth<Tr, D>();
+  constexpr int C = step_chunks<Tr>();
   float* const merge_o = reinterpret_cast<float*>(lds_raw);
   float* const merge_ml = merge_o + kDraftWaves * kTileRows * kMergeStride;
 
-  const int l = lane_id(), g = l >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
-  T* lds = reinterpret_cast<T*>(lds_raw) + (size_t)wave * kChunkTokens * D;
+  int l = lane_id();
+  asm volatile("" : "+v"(l)); // (an item's own: what is worked out from it is not held over the item loop)
+  const int g = l >> 4;
+  T* lds = reinterpret_cast<T*>(lds_raw) + (size_t)wave * C * kChunkTokens * D;
   const DraftSeq& s = it.s;
   const int rows = p.group_size * s.q_len;
   const int prefix = s.seq_len - s.q_len;
@@ -98,158 +100,207 @@ __device__ __forceinline__ void stream_item(const DraftAttentionParams& p, const
   auto page_div = [&](int t) { return (int)(((uint64_t)(uint32_t)t * p.page_magic) >> p.page_magic_shift); };
   const uint32_t page_rows = (uint32_t)(p.num_kv_heads * p.page_size), head_rows = (uint32_t)(it.h * p.page_size);
 
-  // TP: the lane's K row is token l % 16 of the chunk; its page entry is read a
-  // chunk ahead, and the V rows' pages come from the lanes that hold them.  Rows
-  // past the last key read the last key's row (masked, and zeroed in LDS).
-  auto load_entry = [&](int k) { return (uint32_t)bt[page_div(min(k * kChunkTokens + (l & 15), s.seq_len - 1))]; };
-  uint32_t next_entry = 0;
-  auto load_chunk = [&](int k, typename Tr::kreg_t (&kr)[Tr::kLoads], typename Tr::vreg_t (&vr)[Tr::kLoads]) {
-    // (The lane index is opaque here, so that the rows' offsets are worked out where
-    // they are used and not held, and spilled, over the key loop.)
+  // Loads of the C chunks from k on (past k1 the last one again, an L2 hit, rather
+  // than a branch).  TP: lane l % 32 holds the page entry of token l % 32, read a
+  // step ahead; the lanes get their rows' pages from it.  Rows past the last key
+  // read the last key's row (masked, and zeroed in LDS).
+  auto token_of = [&](int k, int c, int row) { return min(min(k + c, k1 - 1) * kChunkTokens + row, s.seq_len - 1); };
+  auto load_entry = [&](int k) { return (uint32_t)bt[page_div(token_of(k, (l >> 4) % C, l & 15))]; };
+  uint32_t entry = 0, next_entry = 0; // TP
+  uint64_t chunk_off[C];              // otherwise: element offsets of the chunks
+  auto look_up = [&](int k) {
+    if constexpr (TP) {
+      entry = min(next_entry, p.last_page);
+      next_entry = load_entry(k + C);
+    } else {
+#pragma unroll
+      for (int c = 0; c < C; c++) {
+        const int t = min(k + c, k1 - 1) * kChunkTokens, pi = page_div(t);
+        const uint32_t page = min((uint32_t)((const const_i32*)bt)[__builtin_amdgcn_readfirstlane(pi)], p.last_page);
+        chunk_off[c] = ((uint64_t)page * page_rows + head_rows + (uint32_t)(t - pi * p.page_size)) * D;
+      }
+    }
+  };
+  auto row_off = [&](int k, int c, int row) { // TP: element offset of a token row of chunk c
+    const int t = token_of(k, c, row);
+    const uint32_t page = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * (16 * c + row), (int)entry);
+    return ((uint64_t)page * page_rows + head_rows + (uint32_t)(t - page_div(t) * p.page_size)) * D;
+  };
+  // (The lane index is opaque in these, so that the rows' offsets are worked out
+  // where they are used and not held, and spilled, over the key loop.)
+  auto opaque_lane = [&]() {
     int le = l;
     asm volatile("" : "+v"(le));
-    if constexpr (TP) {
-      const uint32_t entry = min(next_entry, p.last_page);
-      next_entry = load_entry(min(k + 1, k1 - 1));
-      auto at = [&](int token_row, uint32_t page) {
-        const int t = min(k * kChunkTokens + token_row, s.seq_len - 1);
-        return ((uint64_t)page * page_rows + head_rows + (uint32_t)(t - page_div(t) * p.page_size)) * D;
-      };
-      Tr::load_k_row(kpool + at(le & 15, entry), le, kr);
+    return le;
+  };
+  auto load_k = [&](int k, typename Tr::kreg_t (&kr)[C][Tr::kLoads]) {
+    const int le = opaque_lane();
 #pragma unroll
-      for (int u = 0; u < Tr::kLoads; u++) {
-        const int row = Tr::v_row(le, u);
-        vr[u] = Tr::load_v_row(vpool + at(row, (uint32_t)__shfl((int)entry, row)), le, u);
+    for (int c = 0; c < C; c++) {
+      if constexpr (TP)
+        Tr::load_k_row(kpool + row_off(k, c, le & 15), le, kr[c]);
+      else
+        Tr::load_k(kpool + chunk_off[c], le, kr[c]);
+    }
+  };
+  auto load_v = [&](int k, typename Tr::vreg_t (&vr)[C][Tr::kLoads]) {
+    const int le = opaque_lane();
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+      if constexpr (TP) {
+#pragma unroll
+        for (int u = 0; u < Tr::kLoads; u++)
+          vr[c][u] = Tr::load_v_row(vpool + row_off(k, c, Tr::v_row(le, u)), le, u);
+      } else {
+        Tr::load_v(vpool + chunk_off[c], le, vr[c]);
+      }
+    }
+  };
+
+  // Scores of one row block to probabilities.  The running maximum moves, and what
+  // the row holds is rescaled, only where a score exceeds it by more than 2^8.
+  auto softmax = [&](int nb, float4v (&sc)[C]) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < C; c++) mx = fmaxf(mx, fmaxf(fmaxf(sc[c][0], sc[c][1]), fmaxf(sc[c][2], sc[c][3])));
+    mx = row_max(mx * p.scale_log2); // (scale > 0 keeps the order)
+    const bool grow = mx > m[nb] + kRescaleThreshold || (m[nb] == -INFINITY && mx != -INFINITY);
+    if (__any(grow)) {
+      const float m_new = grow ? mx : m[nb];
+      const float alpha = m[nb] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[nb] - m_new);
+#pragma unroll
+      for (int n = 0; n < D / 16; n++) o[nb][n] *= alpha;
+      lsum[nb] *= alpha;
+      m[nb] = m_new;
+    }
+    const float neg_m = m[nb] == -INFINITY ? 0.f : -m[nb];
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        sc[c][i] = __builtin_amdgcn_exp2f(fmaf(sc[c][i], p.scale_log2, neg_m));
+        lsum[nb] += sc[c][i];
+      }
+  };
+  // O^T += V^T P^T of the chunks.  F16: two chunks in one product of 32 keys, lane
+  // group g with tokens 4 g .. + 4 of each.
+  auto pv = [&](int le, const float4v (&pr)[NB][C]) {
+    if constexpr (sizeof(T) == 2) {
+      half8 pb[NB];
+#pragma unroll
+      for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) pb[nb][e] = (half_t)pr[nb][e >> 2][e & 3];
+      const int row = 4 * (le >> 4) + ((le & 15) >> 2), sw = Tr::swz(row);
+#pragma unroll
+      for (int n = 0; n < D / 16; n++) {
+        T* at = lds + row * D + ((n ^ sw) * 16) + 4 * (le & 3);
+        const short4v ra = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)at);
+        const short4v rb = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(at + kChunkTokens * D));
+        const half8 vt = __builtin_bit_cast(half8, __builtin_shufflevector(ra, rb, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) o[nb][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, pb[nb], o[nb][n], 0, 0, 0);
       }
     } else {
-      const int t = k * kChunkTokens, pi = page_div(t);
-      const uint32_t page = min((uint32_t)((const const_i32*)bt)[__builtin_amdgcn_readfirstlane(pi)], p.last_page);
-      const uint64_t off = ((uint64_t)page * page_rows + head_rows + (uint32_t)(t - pi * p.page_size)) * D;
-      Tr::load_k(kpool + off, le, kr);
-      Tr::load_v(vpool + off, le, vr);
+#pragma unroll
+      for (int c = 0; c < C; c++) {
+        float p4[NB][4];
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) p4[nb][i] = pr[nb][c][i];
+        Tr::template pv<NB>(lds + c * kChunkTokens * D, le, p4, o);
+      }
     }
   };
 
-  // Scores of one row block to probabilities; rescales what the row holds.
-  auto softmax = [&](int nb, const float (&sv)[4], float (&pr)[4]) {
-    const float mx = wave_max_across_groups(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])));
-    const float m_new = fmaxf(m[nb], mx);
-    const float m_use = m_new == -INFINITY ? 0.f : m_new;
-    const float alpha = __builtin_amdgcn_exp2f(m[nb] - m_use);
-    float psum = 0.f;
+  typename Tr::kreg_t kbuf[C][Tr::kLoads];
+  typename Tr::vreg_t vbuf[C][Tr::kLoads];
+  // One step: the C chunks from k on, whose K and V are in kbuf and vbuf; the next
+  // ones are requested as soon as their registers are free.
+  auto step = [&](int k, const RowMask (&mask)[NB], auto drafts) {
+    constexpr bool kDrafts = decltype(drafts)::value; // may hold drafts, or chunks past k1
+    const int le = opaque_lane();
+    float4v sc[NB][C];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      pr[i] = __builtin_amdgcn_exp2f(sv[i] - m_use);
-      psum += pr[i];
-    }
-    lsum[nb] = lsum[nb] * alpha + psum;
-    m[nb] = m_new;
+    for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-    for (int n = 0; n < D / 16; n++) o[nb][n] *= alpha;
-  };
-
-  // A chunk before the drafts: every row sees all of it.
-  auto process = [&](const typename Tr::kreg_t (&kr)[Tr::kLoads], const typename Tr::vreg_t (&vr)[Tr::kLoads]) {
-    asm volatile("" ::: "memory");
-    Tr::stage_v(lds, l, kChunkTokens, vr);
-    float pr[NB][4];
-#pragma unroll
-    for (int nb = 0; nb < NB; nb++) {
-      const float4v sc = Tr::qk(kr, q[nb]);
-      const float sv[4] = {sc[0] * p.scale_log2, sc[1] * p.scale_log2, sc[2] * p.scale_log2, sc[3] * p.scale_log2};
-      softmax(nb, sv, pr[nb]);
-    }
-    // The V tile is written by this wavefront's own lanes: wait for the LDS
-    // writes before the transposed reads of other lanes' rows.
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    Tr::template pv<NB>(lds, l, pr, o);
-  };
-
-  // Any chunk, under the rows' masks.  A draft's V may hold infinities and NaN:
-  // in a product, 0 times one of those would reach the rows that do not see the
-  // draft.  Such a chunk's are added to the rows that see them one by one, and
-  // the finite rest goes through the product.
-  auto process_drafts = [&](int k, const RowMask (&mask)[NB], const typename Tr::kreg_t (&kr)[Tr::kLoads],
-                            typename Tr::vreg_t (&vr)[Tr::kLoads]) {
-    const int tok0 = k * kChunkTokens, tokens = min(s.seq_len - tok0, kChunkTokens);
-    int le = l;
-    asm volatile("" : "+v"(le)::"memory");
-    Tr::stage_v(lds, le, tokens, vr);
+      for (int c = 0; c < C; c++) sc[nb][c] = Tr::qk(kbuf[c], q[nb]);
+    look_up(k + C);
+    load_k(k + C, kbuf);
     bool bad = false;
+    asm volatile("" ::: "memory");
 #pragma unroll
-    for (int u = 0; u < Tr::kLoads; u++) bad |= Tr::v_row(le, u) < tokens && any_non_finite(vr[u]);
-    uint32_t vis[NB]; // of the chunk's tokens
-    float pr[NB][4];
+    for (int c = 0; c < C; c++) {
+      int tokens = kChunkTokens;
+      if constexpr (kDrafts) {
+        tokens = k + c < k1 ? min(s.seq_len - (k + c) * kChunkTokens, kChunkTokens) : 0;
+#pragma unroll
+        for (int u = 0; u < Tr::kLoads; u++) bad |= Tr::v_row(le, u) < tokens && any_non_finite(vbuf[c][u]);
+      }
+      Tr::stage_v(lds + c * kChunkTokens * D, le, tokens, vbuf[c]);
+    }
+    load_v(k + C, vbuf);
+    uint32_t vis[NB]; // kDrafts: of the step's tokens
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
-      const float4v sc = Tr::qk(kr, q[nb]);
-      vis[nb] = visible_bits(mask[nb], tok0 - prefix);
-      float sv[4];
+      if constexpr (kDrafts) {
+        vis[nb] = visible_bits(mask[nb], k * kChunkTokens - prefix);
+        if (C == 1 || k + 1 >= k1) vis[nb] &= 0xffffu;
 #pragma unroll
-      for (int i = 0; i < 4; i++) sv[i] = (vis[nb] >> (4 * g + i)) & 1 ? sc[i] * p.scale_log2 : -INFINITY;
-      softmax(nb, sv, pr[nb]);
+        for (int c = 0; c < C; c++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) sc[nb][c][i] = (vis[nb] >> (16 * c + 4 * g + i)) & 1 ? sc[nb][c][i] : -INFINITY;
+      }
+      softmax(nb, sc[nb]);
     }
+    // The V tiles are written by this wavefront's own lanes: wait for the LDS
+    // writes before reads of other lanes' rows.
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (__any(bad)) {
-      for (int t = 0; t < tokens; t++) {
+    if constexpr (kDrafts) {
+      // A draft's V may hold infinities and NaN: in a product, 0 times one of those
+      // would reach the rows that do not see the draft.  They are added to the rows
+      // that see them one by one, and cleared before the product.
+      if (__any(bad)) {
+        const int tokens = min(min(k + C, k1) * kChunkTokens, s.seq_len) - k * kChunkTokens;
+        for (int t = 0; t < tokens; t++) {
 #pragma unroll
-        for (int n = 0; n < D / 16; n++) {
-          // The lane's dims 16 n + 4 g + e of token t, where stage_v put them.
-          const T* src = lds + t * D + (n ^ Tr::swz(t)) * 16 + 4 * g;
+          for (int n = 0; n < D / 16; n++) {
+            // The lane's dims 16 n + 4 g + e of token t, where stage_v put them.
+            const T* src = lds + t * D + (n ^ Tr::swz(t & 15)) * 16 + 4 * g;
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const float x = non_finite_part(src[e]);
+            for (int e = 0; e < 4; e++) {
+              const float x = non_finite_part(src[e]);
 #pragma unroll
-            for (int nb = 0; nb < NB; nb++) o[nb][n][e] += (vis[nb] >> t) & 1 ? x : 0.f;
+              for (int nb = 0; nb < NB; nb++) o[nb][n][e] += (vis[nb] >> t) & 1 ? x : 0.f;
+            }
           }
         }
+        for (int i = l; i < C * kChunkTokens * D; i += kWaveSize) lds[i] = finite_or_zero(lds[i]);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       }
-#pragma unroll
-      for (int u = 0; u < Tr::kLoads; u++)
-#pragma unroll
-        for (int e = 0; e < (int)(sizeof(vr[u]) / sizeof(T)); e++) vr[u][e] = finite_or_zero(vr[u][e]);
-      asm volatile("" ::: "memory"); // (a wavefront's LDS accesses complete in order)
-      Tr::stage_v(lds, le, tokens, vr);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
-    Tr::template pv<NB>(lds, le, pr, o);
+    pv(le, sc);
   };
 
-  // kDepth chunks in flight; a tail past k1 reloads chunk k1 - 1 (an L2 hit)
-  // rather than branching.  Whole rounds of chunks before the drafts first.
-  typename Tr::kreg_t kbuf[kDepth][Tr::kLoads];
-  typename Tr::vreg_t vbuf[kDepth][Tr::kLoads];
   if (k0 < k1) {
+    RowMask mask[NB];
     if constexpr (TP) next_entry = load_entry(k0);
-#pragma unroll
-    for (int i = 0; i < kDepth; i++) load_chunk(min(k0 + i, k1 - 1), kbuf[i], vbuf[i]);
+    look_up(k0);
+    load_k(k0, kbuf);
+    load_v(k0, vbuf);
     int k = k0;
     const int plain_end = min(k1, max(prefix, 0) / kChunkTokens); // chunks before it hold no draft
-    for (; k + kDepth <= plain_end; k += kDepth) {
-#pragma unroll
-      for (int i = 0; i < kDepth; i++) {
-        process(kbuf[i], vbuf[i]);
-        load_chunk(min(k + i + kDepth, k1 - 1), kbuf[i], vbuf[i]);
-      }
-    }
+    for (; k + C <= plain_end; k += C) step(k, mask, std::false_type());
     if (k < k1) {
-      RowMask mask[NB];
 #pragma unroll
       for (int nb = 0; nb < NB; nb++) {
         bool valid;
         int r, i;
         row_of(nb, valid, r, i);
-        mask[nb] = load_row_mask(p, s, valid, i);
+        mask[nb] = load_row_mask(p, s, i);
       }
-      for (; k < k1; k += kDepth) {
-#pragma unroll
-        for (int i = 0; i < kDepth; i++) {
-          if (k + i < k1) {
-            process_drafts(k + i, mask, kbuf[i], vbuf[i]);
-            load_chunk(min(k + i + kDepth, k1 - 1), kbuf[i], vbuf[i]);
-          }
-        }
-      }
+      for (; k < k1; k += C) step(k, mask, std::true_type());
     }
   }
 
@@ -258,7 +309,7 @@ __device__ __forceinline__ void stream_item(const DraftAttentionParams& p, const
   __syncthreads();
 #pragma unroll
   for (int nb = 0; nb < NB; nb++) {
-    const float ltot = wave_sum_across_groups(lsum[nb]);
+    const float ltot = row_sum(lsum[nb]);
     const int rr = nb * 16 + (l & 15);
     float* dst = merge_o + (wave * kTileRows + rr) * kMergeStride;
 #pragma unroll
@@ -270,7 +321,11 @@ __device__ __forceinline__ void stream_item(const DraftAttentionParams& p, const
   }
   __syncthreads();
   constexpr int kCells = kTileRows * (D / 4); // float4 of the tile
-  for (int c = threadIdx.x; c < kCells; c += kDraftWaves * kWaveSize) {
+  // (The thread's index is counted anew: no register holds it over the key loop.)
+  int none = 0;
+  asm volatile("" : "+s"(none));
+  const int first_cell = wave * kWaveSize + __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none));
+  for (int c = first_cell; c < kCells; c += kDraftWaves * kWaveSize) {
     const int rr = c / (D / 4), d = 4 * (c % (D / 4));
     const int rho = it.rt * kTileRows + rr;
     if (rho >= rows) break; // rows grow with c
@@ -302,18 +357,26 @@ __device__ __forceinline__ void stream_item(const DraftAttentionParams& p, const
   }
 }
 
+typedef __attribute__((address_space(4))) DraftAttentionParams const_params;
+
 template <typename Tr, int D, int NB, bool TP>
 __global__ __launch_bounds__(kWaveSize* kDraftWaves, (stream_blocks<Tr, D, NB, TP>())) void draft_stream_kernel(
-    DraftAttentionParams p) {
+    DraftAttentionParams) {
   constexpr int kTileRows = 16 * NB;
-  constexpr size_t kTileBytes = (size_t)kDraftWaves * kChunkTokens * D * sizeof(typename Tr::elem);
+  constexpr size_t kTileBytes = (size_t)kDraftWaves * step_chunks<Tr>() * kChunkTokens * D * sizeof(typename Tr::elem);
   constexpr size_t kMergeBytes = (size_t)kDraftWaves * kTileRows * (D + 4 + 2) * sizeof(float);
   __shared__ __attribute__((aligned(16))) char lds_raw[kTileBytes > kMergeBytes ? kTileBytes : kMergeBytes];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
   // (One round, unless the device tables hold more than the host planned for.)
+  // The parameters are read again each round: held over the loop, they and what is
+  // worked out from them do not fit the registers.
   for (int w = xcd_item(blockIdx.x, gridDim.x);; w += gridDim.x) {
+    auto args = (const const_params*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(args));
+    const DraftAttentionParams& p = *(const DraftAttentionParams*)args;
     const DraftItem it = find_item<kTileRows>(p, w);
     if (it.b >= p.num_seqs) break;
-    if (it.rt < row_tiles_of<kTileRows>(p, it.s)) stream_item<Tr, D, NB, TP>(p, it, w, lds_raw);
+    if (it.rt < row_tiles_of<kTileRows>(p, it.s)) stream_item<Tr, D, NB, TP>(p, it, w, wave, lds_raw);
     __syncthreads(); // the LDS is used again
   }
 }

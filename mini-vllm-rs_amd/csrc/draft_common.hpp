@@ -13,6 +13,7 @@ namespace {
 
 constexpr int kDraftWaves = 4; // wavefronts per block
 constexpr int kXcds = 8;
+constexpr float kRescaleThreshold = 8.0f; // log2 units: P <= 2^8 between rescales
 
 struct DraftSeq {
   int seq_len, q_start, q_len;
@@ -131,24 +132,31 @@ __device__ __forceinline__ int xcd_item(int block, int blocks) {
 // Visibility of the 32 keys from slot `off` of the drafts on (negative: keys
 // before the drafts, which every row sees), from the row's mask.
 struct RowMask {
-  const uint32_t* words; // the row's mask words
-  uint32_t w0, w1;       // the first two
+  const uint32_t* masks;
+  int mask_words, row;
+  uint32_t w0, w1; // the first two words
   int q_len;
 };
 
 __device__ __forceinline__ uint32_t mask_word(const RowMask& m, int k) {
   const int bits = m.q_len - 32 * k; // that belong to drafts
   if (bits <= 0) return 0;
-  const uint32_t w = k == 0 ? m.w0 : k == 1 ? m.w1 : m.words[k];
+  int row = m.row;
+  asm volatile("" : "+v"(row)); // (or the address is held over the key loop)
+  const uint32_t w = k == 0 ? m.w0 : k == 1 ? m.w1 : m.masks[(int64_t)row * m.mask_words + k];
   return bits >= 32 ? w : w & ((1u << bits) - 1);
 }
 
-__device__ __forceinline__ RowMask load_row_mask(const DraftAttentionParams& p, const DraftSeq& s, bool valid, int i) {
+// (A tile row past the request's last is given row 0's: what it comes to is not stored.)
+__device__ __forceinline__ RowMask load_row_mask(const DraftAttentionParams& p, const DraftSeq& s, int i) {
   RowMask m;
-  m.words = p.masks + (int64_t)(s.q_start + i) * p.mask_words;
-  m.q_len = valid ? s.q_len : 0; // a row that is none sees no draft
-  m.w0 = valid ? m.words[0] : 0;
-  m.w1 = valid && s.q_len > 32 ? m.words[1] : 0;
+  m.masks = p.masks;
+  m.mask_words = p.mask_words;
+  m.row = s.q_start + i;
+  m.q_len = s.q_len;
+  const uint32_t* words = m.masks + (int64_t)m.row * m.mask_words;
+  m.w0 = words[0];
+  m.w1 = s.q_len > 32 ? words[1] : 0;
   return m;
 }
 
@@ -162,6 +170,22 @@ __device__ __forceinline__ uint32_t visible_bits(const RowMask& m, int off) {
 
 // 0 for a row without a key (its sum is 0: no exponential was added), else 1 / sum.
 __device__ __forceinline__ float inverse_sum(float sum) { return __float_as_uint(sum) == 0 ? 0.f : 1.f / sum; }
+
+// Maximum and sum over the lanes l, l ^ 16, l ^ 32, l ^ 48, which hold one query row.
+__device__ __forceinline__ float row_max(float v) {
+  const uint32_t x = __float_as_uint(v);
+  const auto rows = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  const uint32_t y = __float_as_uint(fmaxf(__uint_as_float(rows[0]), __uint_as_float(rows[1])));
+  const auto halves = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+  return fmaxf(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
+}
+__device__ __forceinline__ float row_sum(float v) {
+  const uint32_t x = __float_as_uint(v);
+  const auto rows = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  const uint32_t y = __float_as_uint(__uint_as_float(rows[0]) + __uint_as_float(rows[1]));
+  const auto halves = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+  return __uint_as_float(halves[0]) + __uint_as_float(halves[1]);
+}
 
 // Infinities and NaN are told by their bits, which are opaque to the optimiser
 // here: where a file is compiled without regard for NaN, it would take such a

@@ -26,7 +26,6 @@ typedef int int4v __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
 
-constexpr float kRescaleThreshold = 8.0f; // log2 units
 
 // 16 bytes per lane at `base` + the lane's byte offset straight into LDS at lds
 // + 16 * lane; lanes past `bytes` read zeros.  `base` and `lds` are wave-uniform.
@@ -145,7 +144,7 @@ __device__ __forceinline__ void tile_item(const DraftAttentionParams& p, const D
     bool valid;
     int r, i;
     row_of(valid, r, i);
-    row_mask = load_row_mask(p, s, valid, i);
+    row_mask = load_row_mask(p, s, i);
   }
 
   float16v o[D / 32];
