@@ -118,35 +118,31 @@ void each_request(const mvr_paged_attention_args* a, bool tables, F f) {
 }
 
 // What a block of one tile size costs, in us, for head_dim 128: `fixed` beside
-// its keys, `unit` per 64 keys with one, two or three blocks on its CU.
+// its keys, `unit` per 64 keys with one to four blocks on its CU.  Fitted to 639
+// timed plans (tile sizes and splits of 40 calls: 1 to 64 requests on 100 to 16,000
+// tokens, 1 to 840 rows per KV head, head_dim 64 and 128, both types): the plan
+// that these costs make fastest takes 1.0% longer than the fastest of its call on
+// average, 11% at most.  F32 products take 7 times as long as F16 ones.
 struct TileCost {
   int rows;
-  double fixed, unit[3];
+  double fixed, unit[4];
 };
 
-// Measured (one box, HIP events around calls of 1 to 64 requests on 100 to 16,000
-// tokens with 4 to 840 rows per KV head): F16, one block per CU, 4 / 63 key units:
-// 16 rows 8.6 / 49.8 us, 32 rows 9.4 / 61.0, 64 rows 11.4 (3 units) / 63.5, 128
-// rows 12.4 (3) / 96.4; more blocks per CU: 16 rows 1.79 us per unit with three, 32
-// rows 1.42 with two, 64 rows 1.1, 128 rows 2.1 (16 x 400 rows on 1,000 tokens,
-// 512 blocks of 18 units: 49.6 us).  F32, whose products take 7 times as long: 16
-// rows 2.1 us per unit, 32 rows 3.35, 64 rows 4.4, 128 rows 7.9.  A unit grows with
-// head_dim, in F16 a little slower than it (the softmax does not).
-constexpr TileCost kF16Costs[] = {{16, 5.8, {0.70, 1.25, 1.79}}, {32, 5.9, {0.875, 1.42, 1.42}},
-                                  {64, 8.3, {0.88, 1.1, 1.1}}, {128, 9.3, {1.38, 2.1, 2.1}}};
-constexpr TileCost kF32Costs[] = {{16, 5.0, {2.1, 3.8, 3.8}}, {32, 5.0, {3.35, 6.0, 6.0}},
-                                  {64, 8.5, {4.4, 7.9, 7.9}}, {128, 11.0, {7.9, 15.0, 15.0}}};
+constexpr TileCost kF16Costs[] = {{16, 6.3, {0.60, 1.19, 1.79, 2.38}}, {32, 6.4, {0.77, 1.55, 2.19, 2.19}},
+                                  {64, 6.5, {1.07, 1.24, 1.24, 1.24}}, {128, 7.4, {1.43, 1.88, 1.88, 1.88}}};
+constexpr TileCost kF32Costs[] = {{16, 3.4, {1.93, 3.85, 5.46, 7.27}}, {32, 5.5, {3.13, 5.70, 7.58, 7.58}},
+                                  {64, 4.7, {5.39, 10.5, 10.5, 10.5}}, {128, 6.3, {7.62, 13.5, 13.5, 13.5}}};
 
 // The tile size and the split of its keys that these costs make fastest: every
-// tile whole, or in as many parts as fill the CUs with one block each, or with as
-// many as they hold.  A call takes its blocks' time (all of them in one round; in
-// more rounds the average load and most of a last block), joined with the time
-// that its keys take from HBM (as a 3-norm: 128 blocks of 126 units and a bound of
-// 89 us ran in 119, 256 of 63 in 98).  A split call scans the lengths and merges:
-// 4.5 us, and its partial results at 10 TB/s (they stay in the caches).
+// tile whole, or in parts that give each CU one block, two, up to as many as it
+// holds.  A call takes its blocks' time (all of them in one round; in more rounds
+// the average load and most of a last block), joined with the time that its keys
+// take from HBM (as a 3-norm: 128 blocks of 126 units and a bound of 89 us ran in
+// 119, 256 of 63 in 98).  A split call scans the lengths and merges: 4.5 us, and
+// its partial results written and read at 4 TB/s.
 mvr::DraftAttentionPlan plan_tree(const mvr_paged_attention_args* a, size_t limit) {
   const bool f16 = a->dtype == MVR_DTYPE_F16, tables = host_tables_fit(a);
-  const double dims = a->head_dim / 128.0, unit_scale = f16 ? 0.15 + 0.85 * dims : dims;
+  const double unit_scale = a->head_dim / 128.0;
   const int64_t cus = mvr::api::compute_units(), hkv = a->num_kv_heads;
   const int64_t longest_rows = (int64_t)(a->num_q_heads / a->num_kv_heads) * a->max_q_len;
   const double key_us = 2.0 * mvr::kDraftUnitTokens * hkv * a->head_dim * es_of(a->dtype) / 5.9e6; // of a request's unit
@@ -172,7 +168,7 @@ mvr::DraftAttentionPlan plan_tree(const mvr_paged_attention_args* a, size_t limi
       if (blocks <= held * cus)
         body = part * tile.unit[std::max<int64_t>(0, (blocks + cus - 1) / cus - 1)];
       else
-        body = work * tile.unit[held - 1] / (held * cus) + 0.8 * part * tile.unit[0] + 6;
+        body = work * tile.unit[held - 1] / (held * cus) + 0.73 * part * tile.unit[0] + 5.2;
       body *= unit_scale;
       return tile.fixed + cbrt(body * body * body + hbm * hbm * hbm);
     };
@@ -188,7 +184,7 @@ mvr::DraftAttentionPlan plan_tree(const mvr_paged_attention_args* a, size_t limi
     };
     take(cost_of(tiles, longest), 0, 0, 0);
     if (limit == 0) continue;
-    for (int64_t target : {cus, held * cus}) {
+    for (int64_t target = cus; target <= held * cus; target += cus) {
       if (tiles >= target || longest < 2) continue;
       // The shortest parts whose blocks are no more than `target`: from an estimate
       // (a request's last part is half full on average) upwards.
@@ -207,7 +203,7 @@ mvr::DraftAttentionPlan plan_tree(const mvr_paged_attention_args* a, size_t limi
         if (items <= target && bytes <= limit) break;
       }
       if (part >= longest) continue;
-      take(cost_of(items, part_longest) + 4.5 + 2 * bytes / 10e6, part, items, bytes);
+      take(cost_of(items, part_longest) + 4.5 + 2 * bytes / 4.05e6, part, items, bytes);
     }
   }
   return best;

@@ -28,16 +28,6 @@ constexpr int step_chunks() {
   return sizeof(typename Tr::elem) == 4 ? 1 : 2;
 }
 
-// Blocks per CU (wavefronts per SIMD): what the planner counts on, where the
-// registers allow it without scratch.  Rows with a page of their own (TP) hold an
-// address each.
-template <typename Tr, int D, int NB, bool TP>
-constexpr int stream_blocks() {
-  constexpr bool f16 = sizeof(typename Tr::elem) == 2;
-  constexpr int planned = draft_blocks_per_cu(16 * NB, f16, D);
-  return TP && f16 && D == 96 && NB == 2 ? 1 : planned;
-}
-
 // TP: page sizes that are not a multiple of 16, where every token row has a page
 // of its own to look up.
 template <typename Tr, int D, int NB, bool TP>
@@ -360,7 +350,7 @@ __device__ __forceinline__ void stream_item(const DraftAttentionParams& p, const
 typedef __attribute__((address_space(4))) DraftAttentionParams const_params;
 
 template <typename Tr, int D, int NB, bool TP>
-__global__ __launch_bounds__(kWaveSize* kDraftWaves, (stream_blocks<Tr, D, NB, TP>())) void draft_stream_kernel(
+__global__ __launch_bounds__(kWaveSize* kDraftWaves, (draft_blocks_per_cu(16 * NB, sizeof(typename Tr::elem) == 2, D))) void draft_stream_kernel(
     DraftAttentionParams) {
   constexpr int kTileRows = 16 * NB;
   constexpr size_t kTileBytes = (size_t)kDraftWaves * step_chunks<Tr>() * kChunkTokens * D * sizeof(typename Tr::elem);

@@ -22,8 +22,8 @@ constexpr bool draft_tile_supported(int tile_rows, int head_dim) {
 // Blocks that a CU holds at once, by registers (16- and 32-row tiles, whose
 // wavefronts keep K and V chunks in them) and LDS (64 and 128 rows).
 constexpr int draft_blocks_per_cu(int tile_rows, bool f16, int head_dim) {
-  if (tile_rows == 16) return f16 ? (head_dim <= 128 ? 3 : head_dim <= 160 ? 2 : 1) : head_dim <= 96 ? 2 : 1;
-  if (tile_rows == 32) return f16 ? 2 : head_dim <= 64 ? 2 : 1;
+  if (tile_rows == 16) return head_dim <= 64 ? 4 : head_dim <= (f16 ? 128 : 96) ? 3 : head_dim <= 160 ? 2 : 1;
+  if (tile_rows == 32) return head_dim <= 64 ? 3 : f16 || head_dim <= 96 ? 2 : 1;
   if (tile_rows == 64) return f16 || head_dim <= 64 ? 2 : 1;
   return head_dim <= 128 ? 2 : 1;
 }
