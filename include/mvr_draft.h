@@ -141,7 +141,7 @@ typedef struct mvr_compact_drafts_args {
   const int32_t* accepted;      /* device [num_seqs][max_accepted]: indices in [0, q_len), strictly ascending */
   const int32_t* accepted_lens; /* device [num_seqs], 0 .. min(q_len, max_accepted) */
   int32_t* new_seq_lens;        /* device [num_seqs], written: seq_len - q_len + accepted_lens; NULL: not wanted; must
-                                   not overlap seq_lens */
+                                   overlap none of the tables above */
   void* stream;
 } mvr_compact_drafts_args;
 

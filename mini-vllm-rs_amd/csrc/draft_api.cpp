@@ -8,6 +8,7 @@
 #include <stdlib.h>
 
 #include <algorithm>
+#include <exception>
 #include <memory>
 #include <new>
 #include <vector>
@@ -38,9 +39,27 @@ template <typename F>
 int run_checked(F check) {
   try {
     return check();
-  } catch (const std::bad_alloc&) {
+  } catch (const std::exception&) { // (bad_alloc, or more than a vector may hold)
     return fail(MVR_E_INVALID_ARGUMENT, "checked mode: out of host memory");
   }
+}
+
+// Threads of one launch, over all its blocks.
+constexpr int64_t kMaxThreads = UINT32_MAX;
+
+// Host tables of q_lens: starts that ascend from 0 and end by total_q (0: not given).
+// Whatever is read per token afterwards lies within them.
+int check_cu_q_lens(const int32_t* cu, int num_seqs, int32_t total_q, int32_t max_q_len = INT32_MAX) {
+  if (cu[0] != 0) return fail(MVR_E_INVALID_ARGUMENT, "cu_q_lens[0] must be 0");
+  for (int s = 0; s < num_seqs; s++)
+    if (cu[s + 1] < cu[s] || (int64_t)cu[s + 1] - cu[s] > max_q_len)
+      return max_q_len == INT32_MAX
+                 ? fail(MVR_E_INVALID_ARGUMENT, "cu_q_lens decreases at request %d", s)
+                 : fail(MVR_E_INVALID_ARGUMENT, "request %d has q_len %lld outside [0, max_q_len %d]", s,
+                        (long long)cu[s + 1] - cu[s], max_q_len);
+  if (total_q > 0 && cu[num_seqs] > total_q)
+    return fail(MVR_E_INVALID_ARGUMENT, "cu_q_lens[num_seqs] = %d exceeds total_q = %d", cu[num_seqs], total_q);
+  return MVR_OK;
 }
 
 int copy_failed() { return fail(MVR_E_HIP, "checked mode: copying the device tables to the host failed"); }
@@ -76,7 +95,7 @@ int check_tree(const mvr_paged_attention_args* a, const mvr_draft_trees* t) {
     return fail(MVR_E_UNSUPPORTED, "pools of over 2^31 pages, or pages of over 2^31 rows");
   const int64_t group = a->num_q_heads / a->num_kv_heads;
   const int64_t tiles = (int64_t)a->num_seqs * a->num_kv_heads * ((group * a->max_q_len + 15) / 16);
-  if (group * a->max_q_len > INT32_MAX || tiles * mvr::kDraftMaxParts > INT32_MAX)
+  if (group * a->max_q_len > INT32_MAX || tiles > kMaxThreads / 256)
     return fail(MVR_E_UNSUPPORTED, "%d requests of %d drafts are more than one call takes", a->num_seqs, a->max_q_len);
   return MVR_OK;
 }
@@ -203,6 +222,7 @@ mvr::DraftAttentionPlan plan_tree(const mvr_paged_attention_args* a, size_t limi
         if (items <= target && bytes <= limit) break;
       }
       if (part >= longest) continue;
+      if (a->num_seqs * hkv * ((longest_rows + 15) / 16) > kMaxThreads / 256 / 8) continue; // (the merge's threads)
       take(cost_of(items, part_longest) + 4.5 + 2 * bytes / 4.05e6, part, items, bytes);
     }
   }
@@ -224,20 +244,13 @@ int mvr_paged_attention_tree_validate(const mvr_paged_attention_args* a, const m
   mvr::api::clear_error();
   const int rc = check_tree(a, t);
   if (rc != MVR_OK) return rc;
-  if (cu_q_lens_host) {
-    if (cu_q_lens_host[0] != 0) return fail(MVR_E_INVALID_ARGUMENT, "cu_q_lens[0] must be 0");
-    if (a->total_q > 0 && cu_q_lens_host[a->num_seqs] > a->total_q)
-      return fail(MVR_E_INVALID_ARGUMENT, "cu_q_lens[num_seqs] = %d exceeds total_q = %d", cu_q_lens_host[a->num_seqs],
-                  a->total_q);
-  }
+  if (cu_q_lens_host && check_cu_q_lens(cu_q_lens_host, a->num_seqs, a->total_q, a->max_q_len) != MVR_OK)
+    return MVR_E_INVALID_ARGUMENT;
   for (int s = 0; s < a->num_seqs; s++) {
     int64_t q_len = a->num_seqs == 1 ? a->max_q_len : -1, at = 0;
     if (cu_q_lens_host) {
       at = cu_q_lens_host[s];
       q_len = (int64_t)cu_q_lens_host[s + 1] - at;
-      if (q_len < 0 || q_len > a->max_q_len)
-        return fail(MVR_E_INVALID_ARGUMENT, "request %d has q_len %lld outside [0, max_q_len %d]", s, (long long)q_len,
-                    a->max_q_len);
     }
     const int64_t seq_len = seq_lens_host ? seq_lens_host[s] : a->num_seqs == 1 ? a->max_seq_len : -1;
     if (seq_lens_host) {
@@ -355,8 +368,8 @@ static int check_norm_rope_append(const mvr_rope_append_args* a, const mvr_head_
   if (!a->q || !a->k || !a->v || !a->cos_table || !a->sin_table || !a->block_tables || !a->q_out || !a->key_pool ||
       !a->value_pool)
     return fail(MVR_E_INVALID_ARGUMENT, "null tensor, table or pool pointer");
-  // Blocks of 4 wavefronts, a row at least in each wavefront.
-  if ((int64_t)a->total_q * ((int64_t)a->num_q_heads + 2 * a->num_kv_heads) > INT32_MAX)
+  if (a->num_q_heads > INT32_MAX / 4 / 64 || // (rows of a token and their lanes, in 32 bits)
+      a->total_q > kMaxThreads / 64 / mvr::append_token_waves(a->num_q_heads + 2 * a->num_kv_heads, a->head_dim))
     return fail(MVR_E_UNSUPPORTED, "%d tokens of %d and 2 x %d heads are more than one call takes", a->total_q,
                 a->num_q_heads, a->num_kv_heads);
   if (!(n->eps >= 0.f) || !isfinite(n->eps)) return fail(MVR_E_INVALID_ARGUMENT, "eps must be finite and >= 0");
@@ -380,12 +393,8 @@ int mvr_norm_rope_append_validate(const mvr_rope_append_args* a, const mvr_head_
   mvr::api::clear_error();
   const int rc = check_norm_rope_append(a, n);
   if (rc != MVR_OK) return rc;
-  if (cu_q_lens_host) {
-    if (cu_q_lens_host[0] != 0) return fail(MVR_E_INVALID_ARGUMENT, "cu_q_lens[0] must be 0");
-    if (cu_q_lens_host[a->num_seqs] > a->total_q)
-      return fail(MVR_E_INVALID_ARGUMENT, "cu_q_lens[num_seqs] = %d exceeds total_q = %d", cu_q_lens_host[a->num_seqs],
-                  a->total_q);
-  }
+  if (cu_q_lens_host && check_cu_q_lens(cu_q_lens_host, a->num_seqs, a->total_q) != MVR_OK)
+    return MVR_E_INVALID_ARGUMENT;
   // Pages that an earlier request of this call writes (two writers would race).
   std::unique_ptr<uint8_t[]> written;
   if (block_tables_host) {
@@ -396,7 +405,6 @@ int mvr_norm_rope_append_validate(const mvr_rope_append_args* a, const mvr_head_
     if (!cu_q_lens_host && a->num_seqs > 1) break;
     const int64_t at = cu_q_lens_host ? cu_q_lens_host[s] : 0;
     const int64_t q_len = cu_q_lens_host ? (int64_t)cu_q_lens_host[s + 1] - at : a->total_q;
-    if (q_len < 0) return fail(MVR_E_INVALID_ARGUMENT, "cu_q_lens decreases at request %d", s);
     if (positions_host && n->positions)
       for (int64_t i = at; i < at + q_len; i++)
         if (positions_host[i] < 0 || positions_host[i] >= a->rope_len)
@@ -517,12 +525,18 @@ static int check_compact(const mvr_compact_drafts_args* a) {
                 a->max_pages_per_seq, a->max_seq_len, a->page_size);
   if (!a->block_tables || !a->seq_lens || !a->cu_q_lens || !a->accepted || !a->accepted_lens)
     return fail(MVR_E_INVALID_ARGUMENT, "null table pointer");
-  const uintptr_t old0 = (uintptr_t)a->seq_lens, new0 = (uintptr_t)a->new_seq_lens,
-                  bytes = (uintptr_t)a->num_seqs * sizeof(int32_t);
-  if (a->new_seq_lens && new0 < old0 + bytes && old0 < new0 + bytes)
-    return fail(MVR_E_INVALID_ARGUMENT, "new_seq_lens must not overlap seq_lens"); // read by every head's copy
-  if ((int64_t)a->num_layers * a->num_seqs > INT32_MAX / 2 / a->num_kv_heads)
+  if ((int64_t)a->num_layers * a->num_seqs > kMaxThreads / 64 / a->num_kv_heads)
     return fail(MVR_E_UNSUPPORTED, "more layers, requests and KV heads than one call takes");
+  // Every head and layer reads the tables, one writes the new lengths.
+  auto overlaps = [a](const int32_t* table, int64_t entries) {
+    return a->new_seq_lens && (uintptr_t)a->new_seq_lens < (uintptr_t)(table + entries) &&
+           (uintptr_t)table < (uintptr_t)(a->new_seq_lens + a->num_seqs);
+  };
+  if (overlaps(a->seq_lens, a->num_seqs)) return fail(MVR_E_INVALID_ARGUMENT, "new_seq_lens must not overlap seq_lens");
+  if (overlaps(a->cu_q_lens, (int64_t)a->num_seqs + 1) || overlaps(a->accepted_lens, a->num_seqs) ||
+      overlaps(a->accepted, (int64_t)a->num_seqs * a->max_accepted) ||
+      overlaps(a->block_tables, (int64_t)a->num_layers * a->num_seqs * a->max_pages_per_seq))
+    return fail(MVR_E_INVALID_ARGUMENT, "new_seq_lens must not overlap another table");
   return MVR_OK;
 }
 
@@ -532,7 +546,7 @@ int mvr_compact_drafts_validate(const mvr_compact_drafts_args* a, const int32_t*
   mvr::api::clear_error();
   const int rc = check_compact(a);
   if (rc != MVR_OK) return rc;
-  if (cu_q_lens_host && cu_q_lens_host[0] != 0) return fail(MVR_E_INVALID_ARGUMENT, "cu_q_lens[0] must be 0");
+  if (cu_q_lens_host && check_cu_q_lens(cu_q_lens_host, a->num_seqs, 0) != MVR_OK) return MVR_E_INVALID_ARGUMENT;
   std::unique_ptr<uint8_t[]> written;
   if (block_tables_host) {
     written.reset(new (std::nothrow) uint8_t[(size_t)a->num_pages]());
@@ -540,7 +554,6 @@ int mvr_compact_drafts_validate(const mvr_compact_drafts_args* a, const int32_t*
   }
   for (int s = 0; s < a->num_seqs; s++) {
     const int64_t q_len = cu_q_lens_host ? (int64_t)cu_q_lens_host[s + 1] - cu_q_lens_host[s] : -1;
-    if (cu_q_lens_host && q_len < 0) return fail(MVR_E_INVALID_ARGUMENT, "cu_q_lens decreases at request %d", s);
     if (seq_lens_host) {
       if (seq_lens_host[s] < 0 || seq_lens_host[s] > a->max_seq_len)
         return fail(MVR_E_INVALID_ARGUMENT, "request %d has seq_len %d outside [0, max_seq_len %d]", s, seq_lens_host[s],
@@ -633,9 +646,8 @@ static int check_copy(const mvr_copy_pages_args* a) {
   if (a->num_copies < 0) return fail(MVR_E_INVALID_ARGUMENT, "num_copies must not be negative");
   if (a->num_copies > 0 && (!a->src_pages || !a->dst_pages))
     return fail(MVR_E_INVALID_ARGUMENT, "null page list pointer");
-  // Blocks: one per 8 KiB (1 KiB of two-byte accesses) and pool.
-  const int64_t pieces = ((int64_t)a->num_kv_heads * a->page_size * a->head_dim + 1023) / 1024 + 1;
-  if (pieces * 2 * a->num_copies > INT32_MAX)
+  if (mvr::copy_pages_pieces(a->num_kv_heads * a->page_size, (int64_t)a->head_dim * es_of(a->dtype), a->key_pool,
+                             a->value_pool) * 2 * a->num_copies > kMaxThreads / 256)
     return fail(MVR_E_UNSUPPORTED, "%d copies of pages of this size are more than one call takes", a->num_copies);
   return MVR_OK;
 }

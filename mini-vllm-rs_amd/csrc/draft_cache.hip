@@ -145,10 +145,8 @@ __global__ __launch_bounds__(kThreads) void norm_rope_append_kernel(NormRopeAppe
 
 template <typename T>
 hipError_t launch_append(const NormRopeAppendParams& p, int rope_type, hipStream_t stream) {
-  int lanes_log2 = 0;
-  while ((1 << lanes_log2) < p.head_dim / kItem) lanes_log2++;
-  const int rows = p.num_q_heads + 2 * p.num_kv_heads;
-  const int token_waves = ((rows << lanes_log2) + kWave - 1) / kWave;
+  const int lanes_log2 = append_row_lanes_log2(p.head_dim);
+  const int token_waves = append_token_waves(p.num_q_heads + 2 * p.num_kv_heads, p.head_dim);
   const int64_t units = (int64_t)p.total_q * token_waves;
   const dim3 grid((unsigned)((units + kThreads / kWave - 1) / (kThreads / kWave)));
   if (rope_type == 0)
@@ -240,7 +238,7 @@ __global__ __launch_bounds__(kThreads) void compact_drafts_kernel(CompactDraftsP
 
 // Copies of pages.  A block per piece of kCopyVecs * 256 vectors of one page's
 // leading tokens, K and V in turn; all of a thread's loads before its stores.
-constexpr int kCopyVecs = 4;
+constexpr int kCopyVecs = kCopyPieceVecs / kThreads;
 
 template <typename V>
 __global__ __launch_bounds__(kThreads) void copy_pages_kernel(CopyPagesParams p, int row_vecs, int pieces) {
@@ -271,13 +269,12 @@ __global__ __launch_bounds__(kThreads) void copy_pages_kernel(CopyPagesParams p,
     if (v0 + u * kThreads < vecs) to[at[u]] = held[u];
 }
 
-// Widest vector that rows and pools allow.
 template <typename F>
 hipError_t with_vector(int64_t row_bytes, const void* a, const void* b, F launch) {
-  const uintptr_t align = (uintptr_t)a | (uintptr_t)b | (uintptr_t)row_bytes;
-  if (align % 16 == 0) return launch(u32x4{}, (int)(row_bytes / 16));
-  if (align % 4 == 0) return launch(uint32_t{}, (int)(row_bytes / 4));
-  return launch(uint16_t{}, (int)(row_bytes / 2));
+  const int bytes = cache_vector_bytes(row_bytes, a, b), row_vecs = (int)(row_bytes / bytes);
+  if (bytes == 16) return launch(u32x4{}, row_vecs);
+  if (bytes == 4) return launch(uint32_t{}, row_vecs);
+  return launch(uint16_t{}, row_vecs);
 }
 
 } // namespace
@@ -297,8 +294,8 @@ hipError_t launch_compact_drafts(const CompactDraftsParams& params, int64_t row_
 
 hipError_t launch_copy_pages(const CopyPagesParams& params, int64_t row_bytes, hipStream_t stream) {
   return with_vector(row_bytes, params.key_pool, params.value_pool, [&](auto v, int row_vecs) {
-    const int64_t vecs = (int64_t)params.num_kv_heads * params.page_size * row_vecs;
-    const int64_t pieces = (vecs + kCopyVecs * kThreads - 1) / (kCopyVecs * kThreads);
+    const int64_t pieces =
+        copy_pages_pieces((int64_t)params.num_kv_heads * params.page_size, row_bytes, params.key_pool, params.value_pool);
     hipLaunchKernelGGL(copy_pages_kernel<decltype(v)>, dim3((unsigned)(2 * pieces * params.num_copies)), dim3(kThreads),
                        0, stream, params, row_vecs, (int)pieces);
     return hipGetLastError();

@@ -34,6 +34,14 @@ struct NormRopeAppendParams {
   int32_t num_seqs, num_q_heads, num_kv_heads, head_dim, page_size, total_q;
 };
 
+// Lanes of a row, a power of two (8 elements each), and wavefronts of a token.
+inline int append_row_lanes_log2(int head_dim) {
+  int lanes_log2 = 0;
+  while ((8 << lanes_log2) < head_dim) lanes_log2++;
+  return lanes_log2;
+}
+inline int append_token_waves(int rows, int head_dim) { return ((rows << append_row_lanes_log2(head_dim)) + 63) / 64; }
+
 // dtype: 0 = F32, 1 = F16; rope_type: 0 = Neox, 1 = Interleaved.
 hipError_t launch_norm_rope_append(const NormRopeAppendParams& params, int dtype, int rope_type, hipStream_t stream);
 
@@ -62,6 +70,20 @@ struct CopyPagesParams {
   int64_t num_pages;
   int32_t num_copies, num_kv_heads, page_size;
 };
+
+// Bytes that one access moves: the widest that rows and pools allow.
+inline int cache_vector_bytes(int64_t row_bytes, const void* a, const void* b) {
+  const uintptr_t align = (uintptr_t)a | (uintptr_t)b | (uintptr_t)row_bytes;
+  return align % 16 == 0 ? 16 : align % 4 == 0 ? 4 : 2;
+}
+
+constexpr int kCopyPieceVecs = 4 * 256; // that a block copies
+
+// Blocks of one page's copy in one pool.
+inline int64_t copy_pages_pieces(int64_t rows, int64_t row_bytes, const void* a, const void* b) {
+  const int64_t vecs = rows * (row_bytes / cache_vector_bytes(row_bytes, a, b));
+  return (vecs + kCopyPieceVecs - 1) / kCopyPieceVecs;
+}
 
 hipError_t launch_copy_pages(const CopyPagesParams& params, int64_t row_bytes, hipStream_t stream);
 

@@ -177,7 +177,9 @@ def _pools(key_pool, value_pool):
 
 class Call:
     """One call of the library, its argument block (`args`, and `extra` where the entry point takes a second one) made
-    and its tensors kept.  Calling it launches on `stream`, or on the stream that is current then."""
+    and its tensors kept.  Calling it launches on `stream`, or on the stream that is current then.
+    One thread at a time may call it (another makes a Call of its own), and where there is a `workspace`, its launches must
+    not overlap in time, nor may those of Calls that share one."""
 
     def __init__(self, name, args, extra, tensors, device, stream, workspace=None):
         self._function = getattr(load_library(), name)

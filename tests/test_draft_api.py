@@ -159,6 +159,12 @@ def test_tree_validate():
             check(**kw)
         assert e.value.code == code and text in e.value.message, e.value.message
     check(block_tables_host=np.where(bt < 64, -1, bt))  # an empty request reads no page
+    # Starts that descend again: refused before a mask row behind the table's end (here, zeros) is read.
+    masks[10:] = 0
+    a.total_q = 10
+    with pytest.raises(M.MvrError) as e:
+        check(cu_q_lens_host=np.array([0, 40, 5]), masks_host=masks[:10])
+    assert "q_len -35" in e.value.message
 
 
 def test_tree_workspace_follows_the_hints():
@@ -223,6 +229,7 @@ def append_args(**kw):
     (dict(eps=float("inf")), M.MVR_E_INVALID_ARGUMENT, "eps"),
     (dict(k_weight=FAKE + 4), M.MVR_E_INVALID_ARGUMENT, "aligned"),
     (dict(k_stride_token=66), M.MVR_E_INVALID_ARGUMENT, "strides"),
+    (dict(total_q=1 << 26), M.MVR_E_UNSUPPORTED, "more than one call takes"),
 ])
 def test_append_refusals(change, code, text):
     rc, message = status("mvr_norm_rope_append", *append_args(**change))
@@ -240,6 +247,7 @@ def test_append_validate():
     for kw, code, text in (
             (dict(cu_q_lens_host=np.array([0, 5, 11])), M.MVR_E_INVALID_ARGUMENT, "total_q"),
             (dict(cu_q_lens_host=np.array([0, 5, 4])), M.MVR_E_INVALID_ARGUMENT, "decreases"),
+            (dict(cu_q_lens_host=np.array([0, 10, 5]), positions_host=np.full(10, -1)), M.MVR_E_INVALID_ARGUMENT, "decreases"),
             (dict(seq_lens_host=np.array([7, 129])), M.MVR_E_INVALID_ARGUMENT, "129"),
             (dict(seq_lens_host=np.array([7, 8])), M.MVR_E_LENGTH_MISMATCH, "after appending 9"),
             (dict(positions_host=np.full(10, 128)), M.MVR_E_INVALID_ARGUMENT, "position 128"),
@@ -278,6 +286,8 @@ def compact_args(**kw):
     (dict(accepted=None), M.MVR_E_INVALID_ARGUMENT, "null"),
     (dict(key_pool=FAKE + 1), M.MVR_E_INVALID_ARGUMENT, "aligned"),
     (dict(new_seq_lens=FAKE + 4), M.MVR_E_INVALID_ARGUMENT, "overlap"),
+    *((dict({table: 2 * FAKE + 4}), M.MVR_E_INVALID_ARGUMENT, "overlap")
+      for table in ("seq_lens", "cu_q_lens", "accepted", "accepted_lens", "block_tables")),
     (dict(num_layers=1 << 20, num_seqs=1 << 20, new_seq_lens=None), M.MVR_E_UNSUPPORTED, "more layers"),
 ])
 def test_compact_refusals(change, code, text):
@@ -324,6 +334,7 @@ def copy_args(**kw):
     (dict(src_pages=None), M.MVR_E_INVALID_ARGUMENT, "null"),
     (dict(value_pool=None), M.MVR_E_INVALID_ARGUMENT, "null"),
     (dict(num_copies=1 << 30, page_size=1 << 10), M.MVR_E_UNSUPPORTED, "more than one call takes"),
+    (dict(num_copies=1 << 23), M.MVR_E_UNSUPPORTED, "more than one call takes"),  # (2^24 blocks of 256 threads)
 ])
 def test_copy_refusals(change, code, text):
     rc, message = status("mvr_copy_pages", copy_args(**change))
