@@ -17,6 +17,9 @@ void clear_error();
 // MVR_ATTN_CHECKED=true: calls check their device tables on the host first.
 bool checked();
 
+// A positive integer from the environment.
+int env_int(const char* name, int fallback);
+
 // Host copy of `count` int32 device values (none when dev is null), after
 // waiting for the stream; false if the copy fails.
 bool copy_to_host(const int32_t* dev, size_t count, void* stream, std::vector<int32_t>& host);

@@ -165,12 +165,19 @@ mvr::DraftAttentionPlan plan_tree(const mvr_paged_attention_args* a, size_t limi
   const int64_t cus = mvr::api::compute_units(), hkv = a->num_kv_heads;
   const int64_t longest_rows = (int64_t)(a->num_q_heads / a->num_kv_heads) * a->max_q_len;
   const double key_us = 2.0 * mvr::kDraftUnitTokens * hkv * a->head_dim * es_of(a->dtype) / 5.9e6; // of a request's unit
+  // Overrides, for tests and tuning: a tile size that the head dimension has, and
+  // its parts.
+  static const int set_rows = mvr::api::env_int("MVR_DRAFT_TILE_ROWS", 0);
+  static const int set_units = mvr::api::env_int("MVR_DRAFT_PART_UNITS", 0);
+  bool rows_set = false;
+  for (const TileCost& tile : kF16Costs)
+    rows_set |= tile.rows == set_rows && mvr::draft_tile_supported(set_rows, a->head_dim);
   mvr::DraftAttentionPlan best{};
   double best_cost = INFINITY;
   for (const TileCost& tile : f16 ? kF16Costs : kF32Costs) {
     if (!mvr::draft_tile_supported(tile.rows, a->head_dim)) continue;
     // (A tile that no request fills half costs what the smaller one does, or more.)
-    if (tile.rows > 16 && longest_rows <= tile.rows / 2 && best_cost < INFINITY) break;
+    if (rows_set ? tile.rows != set_rows : longest_rows <= tile.rows / 2 && best_cost < INFINITY) continue;
     const int held = mvr::draft_blocks_per_cu(tile.rows, f16, a->head_dim);
     auto tiles_of = [&](const Request& r) { return r.count * hkv * ((r.rows + tile.rows - 1) / tile.rows); };
     int64_t tiles = 0, work = 0, longest = 0;
@@ -201,29 +208,44 @@ mvr::DraftAttentionPlan plan_tree(const mvr_paged_attention_args* a, size_t limi
       best.blocks = part ? (int)items : (int)(a->num_seqs * hkv * best.row_tiles);
       best.partial_bytes = bytes;
     };
+    int64_t items = 0, part_longest = 0;
+    size_t bytes = 0;
+    auto split_at = [&](int64_t part) {
+      items = part_longest = 0;
+      each_request(a, tables, [&](const Request& r) {
+        const int64_t parts = std::min<int64_t>((r.units + r.more + part - 1) / part + r.more, mvr::kDraftMaxParts);
+        if (parts == 0) return;
+        items += tiles_of(r) * parts;
+        part_longest = std::max(part_longest, (r.units + parts - 1) / parts);
+      });
+      bytes = align_up((size_t)items * tile.rows * a->head_dim * sizeof(float), 256) +
+              align_up((size_t)items * tile.rows * 2 * sizeof(float), 256);
+    };
+    auto take_split = [&](int64_t part) {
+      take(cost_of(items, part_longest) + 4.5 + 2 * bytes / 4.05e6, part, items, bytes);
+    };
+    // (The blocks of a split call and of its merge have to fit a launch each.)
+    const bool may_split = limit > 0 && longest > 1 &&
+                           a->num_seqs * hkv * ((longest_rows + 15) / 16) <= kMaxThreads / 256 / 64;
+    if (may_split && set_units && set_units < longest) {
+      split_at(set_units);
+      if (bytes <= limit) {
+        take_split(set_units);
+        continue;
+      }
+    }
     take(cost_of(tiles, longest), 0, 0, 0);
-    if (limit == 0) continue;
+    if (!may_split || set_units) continue;
     for (int64_t target = cus; target <= held * cus; target += cus) {
-      if (tiles >= target || longest < 2) continue;
+      if (tiles >= target) continue;
       // The shortest parts whose blocks are no more than `target`: from an estimate
       // (a request's last part is half full on average) upwards.
-      int64_t part = std::max<int64_t>(1, work / (target - tiles / 2)), items = 0, part_longest = 0;
-      size_t bytes = 0;
+      int64_t part = std::max<int64_t>(1, work / (target - tiles / 2));
       for (; part < longest; part += 1 + part / 16) {
-        items = part_longest = 0;
-        each_request(a, tables, [&](const Request& r) {
-          const int64_t parts = std::min<int64_t>((r.units + r.more + part - 1) / part + r.more, mvr::kDraftMaxParts);
-          if (parts == 0) return;
-          items += tiles_of(r) * parts;
-          part_longest = std::max(part_longest, (r.units + parts - 1) / parts);
-        });
-        bytes = align_up((size_t)items * tile.rows * a->head_dim * sizeof(float), 256) +
-                align_up((size_t)items * tile.rows * 2 * sizeof(float), 256);
+        split_at(part);
         if (items <= target && bytes <= limit) break;
       }
-      if (part >= longest) continue;
-      if (a->num_seqs * hkv * ((longest_rows + 15) / 16) > kMaxThreads / 256 / 8) continue; // (the merge's threads)
-      take(cost_of(items, part_longest) + 4.5 + 2 * bytes / 4.05e6, part, items, bytes);
+      if (part < longest) take_split(part);
     }
   }
   return best;

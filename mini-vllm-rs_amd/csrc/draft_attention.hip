@@ -410,7 +410,7 @@ __global__ __launch_bounds__(256) void draft_merge_kernel(DraftAttentionParams p
     float2v ml[kAhead];
     float4v o[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; u++) { // (past the last part: the last again, with no weight)
+    for (int u = 0; u < kAhead; u++) { // (past the last part: the last again, not counted)
       const int64_t row = row0 + min(j0 + u, parts - 1) * stride;
       ml[u] = *reinterpret_cast<const float2v*>(p.partial_ml + row * 2);
       o[u] = *reinterpret_cast<const float4v*>(p.partial_o + row * D + d);
@@ -424,7 +424,8 @@ __global__ __launch_bounds__(256) void draft_merge_kernel(DraftAttentionParams p
     sum *= alpha;
 #pragma unroll
     for (int u = 0; u < kAhead; u++) {
-      const float w = j0 + u < parts ? __builtin_amdgcn_exp2f(ml[u][0] - m_use) : 0.f;
+      if (j0 + u >= parts) continue; // (no weight of 0: its rows may hold an infinity)
+      const float w = __builtin_amdgcn_exp2f(ml[u][0] - m_use);
       sum += w * ml[u][1];
       acc += w * o[u];
     }

@@ -1251,6 +1251,8 @@ void clear_error() { g_last_error[0] = 0; }
 
 bool checked() { return checked_mode(); }
 
+int env_int(const char* name, int fallback) { return ::env_int(name, fallback); }
+
 bool copy_to_host(const int32_t* dev, size_t count, void* stream, std::vector<int32_t>& host) {
   return copy_table(dev, count, static_cast<hipStream_t>(stream), host);
 }
