@@ -64,7 +64,8 @@ __device__ __forceinline__ TokenRequest request_of(const int32_t* cu, int num_se
 // while its rows are on their way.
 //
 // Bound by that chain of dependent loads (request, length, page, store): 1,024
-// tokens of 36 rows take 7.6 us in F16 at D=128, where HBM needs 3.9.
+// tokens of 36 rows take 8.7 us in F16 at D=128, where HBM needs 3.9 and a launch
+// that does next to nothing 3.5.
 template <typename T, int ROPE>
 __global__ __launch_bounds__(kThreads) void norm_rope_append_kernel(NormRopeAppendParams p, int lanes_log2,
                                                                     int token_waves) {
@@ -162,6 +163,10 @@ hipError_t launch_append(const NormRopeAppendParams& p, int rope_type, hipStream
 // read before any of it is written.  Indices ascend, so a row's source lies at or
 // behind its destination, and behind every destination of the batches before:
 // whatever is written, its old content has been read.
+//
+// Rows of 256 bytes in random pages: 32 requests of 20..64 drafts in 32 layers (78
+// MB) take 21.5 us, 3.6 TB/s where a large copy reaches 4.9; all wavefronts are
+// resident at once, so the chain of lengths, path, pages and rows shows once.
 constexpr int kBatch = 4; // vectors per lane, pool and batch
 
 __device__ __forceinline__ int64_t shfl64(int64_t v, int src) {
@@ -238,6 +243,7 @@ __global__ __launch_bounds__(kThreads) void compact_drafts_kernel(CompactDraftsP
 
 // Copies of pages.  A block per piece of kCopyVecs * 256 vectors of one page's
 // leading tokens, K and V in turn; all of a thread's loads before its stores.
+// Bound by HBM: 3,500 pages of 32 KiB in 50.6 us, 4.5 TB/s.
 constexpr int kCopyVecs = kCopyPieceVecs / kThreads;
 
 template <typename V>
