@@ -58,6 +58,21 @@ def test_tree_sizes(dtype, hq, hkv, d, nodes):
                         note=masks)
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("hq,hkv", [(4, 4), (64, 1), (1, 1), (10, 2), (24, 8)])
+def test_head_layouts(dtype, hq, hkv):
+    """A KV head for every query head, one for all of them, and groups between."""
+    for nodes in ([3, 1], [40, 130]):
+        check_attention(run(b := Batch(hq + hkv, dtype, hq, hkv, 64, 16, [70, 200], nodes, "tree")), b, note=str(nodes))
+
+
+@pytest.mark.parametrize("dtype,cached,nodes", [(F16, [200_000, 3], [4, 2]), (F32, [70_001], [1]), (F16, [0, 900], [1100, 5]),
+                                                (F16, [120_000], [90])])
+def test_long(dtype, cached, nodes):
+    """Contexts of more keys than the most parts of the shortest units hold, and masks of tens of words."""
+    check_attention(run(b := Batch(sum(nodes), dtype, 4, 2, 64, 16, cached, nodes, "tree")), b)
+
+
 @pytest.mark.parametrize("cached", [0, 1, 15, 16, 17, 31, 33, 63, 64, 65, 127, 128, 129])
 @pytest.mark.parametrize("dtype", [F16, F32])
 def test_where_the_drafts_begin(dtype, cached):
