@@ -94,7 +94,8 @@ int check_tree(const mvr_paged_attention_args* a, const mvr_draft_trees* t) {
   if (a->num_pages > INT32_MAX || (int64_t)a->num_kv_heads * a->page_size > INT32_MAX)
     return fail(MVR_E_UNSUPPORTED, "pools of over 2^31 pages, or pages of over 2^31 rows");
   const int64_t group = a->num_q_heads / a->num_kv_heads;
-  const int64_t tiles = (int64_t)a->num_seqs * a->num_kv_heads * ((group * a->max_q_len + 15) / 16);
+  const int64_t pairs = (int64_t)a->num_seqs * a->num_kv_heads + mvr::kDraftXcds - 1;
+  const int64_t tiles = pairs * ((group * a->max_q_len + 15) / 16);
   if (group * a->max_q_len > INT32_MAX || tiles > kMaxThreads / 256)
     return fail(MVR_E_UNSUPPORTED, "%d requests of %d drafts are more than one call takes", a->num_seqs, a->max_q_len);
   return MVR_OK;
@@ -137,28 +138,29 @@ void each_request(const mvr_paged_attention_args* a, bool tables, F f) {
 }
 
 // What a block of one tile size costs, in us, for head_dim 128: `fixed` beside
-// its keys, `unit` per 64 keys with one to four blocks on its CU.  Fitted to 639
-// timed plans (tile sizes and splits of 40 calls: 1 to 64 requests on 100 to 16,000
+// its keys, `unit` per 64 keys with one to four blocks on its CU.  Fitted to 965
+// timed plans (tile sizes and splits of 53 calls: 1 to 64 requests on 100 to 16,000
 // tokens, 1 to 840 rows per KV head, head_dim 64 and 128, both types): the plan
-// that these costs make fastest takes 1.0% longer than the fastest of its call on
+// that these costs make fastest takes 1.1% longer than the fastest of its call on
 // average, 11% at most.  F32 products take 7 times as long as F16 ones.
 struct TileCost {
   int rows;
   double fixed, unit[4];
 };
 
-constexpr TileCost kF16Costs[] = {{16, 6.3, {0.60, 1.19, 1.79, 2.38}}, {32, 6.4, {0.77, 1.55, 2.19, 2.19}},
-                                  {64, 6.5, {1.07, 1.24, 1.24, 1.24}}, {128, 7.4, {1.43, 1.88, 1.88, 1.88}}};
-constexpr TileCost kF32Costs[] = {{16, 3.4, {1.93, 3.85, 5.46, 7.27}}, {32, 5.5, {3.13, 5.70, 7.58, 7.58}},
-                                  {64, 4.7, {5.39, 10.5, 10.5, 10.5}}, {128, 6.3, {7.62, 13.5, 13.5, 13.5}}};
+constexpr TileCost kF16Costs[] = {{16, 6.3, {0.57, 1.17, 1.81, 2.48}}, {32, 6.3, {0.75, 1.55, 2.33, 2.33}},
+                                  {64, 6.6, {1.02, 1.30, 1.30, 1.30}}, {128, 8.0, {1.32, 1.62, 1.62, 1.62}}};
+constexpr TileCost kF32Costs[] = {{16, 2.5, {1.97, 4.05, 6.23, 8.55}}, {32, 5.8, {3.06, 5.80, 7.43, 7.43}},
+                                  {64, 5.7, {4.73, 9.50, 9.50, 9.50}}, {128, 6.6, {7.61, 14.8, 14.8, 14.8}}};
 
 // The tile size and the split of its keys that these costs make fastest: every
 // tile whole, or in parts that give each CU one block, two, up to as many as it
-// holds.  A call takes its blocks' time (all of them in one round; in more rounds
-// the average load and most of a last block), joined with the time that its keys
-// take from HBM (as a 3-norm: 128 blocks of 126 units and a bound of 89 us ran in
-// 119, 256 of 63 in 98).  A split call scans the lengths and merges: 4.5 us, and
-// its partial results written and read at 4 TB/s.
+// holds, or two, three or four times that.  A call takes its blocks' time (all of
+// them in one round; in more rounds the average load and most of a last block, the
+// shortest where the longest start first), joined with the time that its keys take
+// from HBM (as a 3-norm: 128 blocks of 126 units and a bound of 89 us ran in 119,
+// 256 of 63 in 98).  A split call scans the lengths and merges: 4.5 us, and its
+// partial results written and read at 4.3 TB/s.
 mvr::DraftAttentionPlan plan_tree(const mvr_paged_attention_args* a, size_t limit) {
   const bool f16 = a->dtype == MVR_DTYPE_F16, tables = host_tables_fit(a);
   const double unit_scale = a->head_dim / 128.0;
@@ -180,21 +182,22 @@ mvr::DraftAttentionPlan plan_tree(const mvr_paged_attention_args* a, size_t limi
     if (rows_set ? tile.rows != set_rows : longest_rows <= tile.rows / 2 && best_cost < INFINITY) continue;
     const int held = mvr::draft_blocks_per_cu(tile.rows, f16, a->head_dim);
     auto tiles_of = [&](const Request& r) { return r.count * hkv * ((r.rows + tile.rows - 1) / tile.rows); };
-    int64_t tiles = 0, work = 0, longest = 0;
+    int64_t tiles = 0, work = 0, longest = 0, shortest = INT64_MAX;
     double hbm = 0;
     each_request(a, tables, [&](const Request& r) {
       if (r.units == 0) return;
       tiles += tiles_of(r);
       work += tiles_of(r) * r.units;
       longest = std::max(longest, r.units);
+      shortest = std::min(shortest, r.units);
       hbm += r.count * r.units * key_us;
     });
-    auto cost_of = [&](int64_t blocks, int64_t part) {
+    auto cost_of = [&](int64_t blocks, int64_t part, int64_t last) { // of `part` units at most, the last one of `last`
       double body;
       if (blocks <= held * cus)
         body = part * tile.unit[std::max<int64_t>(0, (blocks + cus - 1) / cus - 1)];
       else
-        body = work * tile.unit[held - 1] / (held * cus) + 0.73 * part * tile.unit[0] + 5.2;
+        body = std::max(work * tile.unit[held - 1] / (held * cus) + 0.87 * last * tile.unit[0], part * tile.unit[0]) + 6.1;
       body *= unit_scale;
       return tile.fixed + cbrt(body * body * body + hbm * hbm * hbm);
     };
@@ -205,7 +208,11 @@ mvr::DraftAttentionPlan plan_tree(const mvr_paged_attention_args* a, size_t limi
       best.row_tiles = (int)((longest_rows + tile.rows - 1) / tile.rows);
       best.part_units = (int)part;
       best.max_items = (int)items;
-      best.blocks = part ? (int)items : (int)(a->num_seqs * hkv * best.row_tiles);
+      // Not split: the pairs of request and KV head by eights.
+      const int64_t pairs = (a->num_seqs * hkv + mvr::kDraftXcds - 1) / mvr::kDraftXcds * mvr::kDraftXcds;
+      best.blocks = (int)(part ? items : pairs * best.row_tiles);
+      // (Finding a length's rank takes 0.3 us: not where all are alike, or start at once.)
+      best.by_length = part == 0 && best.blocks > cus && (!tables || shortest < longest);
       best.partial_bytes = bytes;
     };
     int64_t items = 0, part_longest = 0;
@@ -222,7 +229,7 @@ mvr::DraftAttentionPlan plan_tree(const mvr_paged_attention_args* a, size_t limi
               align_up((size_t)items * tile.rows * 2 * sizeof(float), 256);
     };
     auto take_split = [&](int64_t part) {
-      take(cost_of(items, part_longest) + 4.5 + 2 * bytes / 4.05e6, part, items, bytes);
+      take(cost_of(items, part_longest, part_longest) + 4.5 + 2 * bytes / 4.3e6, part, items, bytes);
     };
     // (The blocks of a split call and of its merge have to fit a launch each.)
     const bool may_split = limit > 0 && longest > 1 &&
@@ -234,9 +241,9 @@ mvr::DraftAttentionPlan plan_tree(const mvr_paged_attention_args* a, size_t limi
         continue;
       }
     }
-    take(cost_of(tiles, longest), 0, 0, 0);
+    take(cost_of(tiles, longest, longest ? shortest : 0), 0, 0, 0);
     if (!may_split || set_units) continue;
-    for (int64_t target = cus; target <= held * cus; target += cus) {
+    for (int64_t target = cus; target <= 4 * held * cus; target += target < held * cus ? cus : held * cus) {
       if (tiles >= target) continue;
       // The shortest parts whose blocks are no more than `target`: from an estimate
       // (a request's last part is half full on average) upwards.
@@ -343,6 +350,7 @@ int mvr_paged_attention_tree(const mvr_paged_attention_args* a, const mvr_draft_
   p.row_tiles = plan.row_tiles;
   p.part_units = plan.part_units;
   p.max_items = plan.max_items;
+  p.by_length = plan.by_length;
   if (plan.max_items) {
     p.partial_o = static_cast<float*>(a->workspace);
     p.partial_ml = reinterpret_cast<float*>(

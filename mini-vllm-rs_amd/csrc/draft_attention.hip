@@ -369,10 +369,11 @@ __global__ __launch_bounds__(kWaveSize* kDraftWaves, (draft_blocks_per_cu(16 * N
   // (One round, unless the device tables hold more than the host planned for.)
   // The parameters are read again each round: held over the loop, they and what is
   // worked out from them do not fit the registers.
-  for (int w = xcd_item(blockIdx.x, gridDim.x);; w += gridDim.x) {
+  for (int round = 0;; round++) {
     auto args = (const const_params*)__builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" : "+s"(args));
     const DraftAttentionParams& p = *(const DraftAttentionParams*)args;
+    const int w = first_item(p) + round * gridDim.x;
     const DraftItem it = find_item<kTileRows>(p, w);
     if (it.b >= p.num_seqs) break;
     if (it.rt < row_tiles_of<kTileRows>(p, it.s)) stream_item<Tr, D, NB, TP>(p, it, w, wave, lds_raw);

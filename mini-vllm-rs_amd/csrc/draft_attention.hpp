@@ -13,6 +13,7 @@ namespace mvr {
 constexpr int kDraftUnitTokens = 64;
 // Parts of one row tile, at most.
 constexpr int kDraftMaxParts = 64;
+constexpr int kDraftXcds = 8;
 
 // Row tiles: 16 rows for every head dimension, 128 too, 32 and 64 up to 128.
 constexpr bool draft_tile_supported(int tile_rows, int head_dim) {
@@ -50,12 +51,13 @@ struct DraftAttentionParams {
   uint64_t page_magic; // page of token t = t * page_magic >> page_magic_shift (page_divider)
   int32_t page_magic_shift;
   int32_t row_tiles; // of the longest request, per (request, KV head)
-  // 0: every row tile is one item, found from the block index.  Otherwise parts
+  // 0: every row tile is one item, found from the block index (of by_length: the
+  // longest requests first).  Otherwise parts
   // of at most part_units key units (longer ones where that makes more than
   // kDraftMaxParts), found by a scan of the length tables, whose items' partial
   // results lie in the slot of the item's number; max_items of them.  Where the
   // device tables hold more items than that, tiles are not split.
-  int32_t part_units, max_items;
+  int32_t part_units, max_items, by_length;
   float* partial_o;  // [max_items][tile_rows][head_dim]
   float* partial_ml; // [max_items][tile_rows][2]: maximum (log2 units), sum
   float scale_log2;
@@ -66,6 +68,7 @@ struct DraftAttentionPlan {
   int row_tiles;
   int part_units; // 0: not split
   int blocks;
+  int by_length;
   int max_items; // 0: no partials
   size_t partial_bytes;
 };

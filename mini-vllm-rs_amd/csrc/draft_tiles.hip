@@ -581,7 +581,7 @@ __global__ __launch_bounds__(kWaveSize* kDraftWaves, (draft_blocks_per_cu(32 * R
     DraftAttentionParams p) {
   constexpr int kTileRows = 32 * RW;
   // (One call of tile_item: its code, twice, would crowd the instruction cache.)
-  for (int w = xcd_item(blockIdx.x, gridDim.x);; w += gridDim.x) {
+  for (int w = first_item(p);; w += gridDim.x) {
     const DraftItem it = find_item<kTileRows>(p, w);
     if (it.b >= p.num_seqs) break;
     if (it.rt < row_tiles_of<kTileRows>(p, it.s)) tile_item<D, T, RW, PAGES, S>(p, it, w);

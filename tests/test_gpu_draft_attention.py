@@ -155,6 +155,22 @@ def test_many_requests():
     check_attention(run(few), few)
 
 
+@pytest.mark.parametrize("hkv", [1, 3, 8])
+@pytest.mark.parametrize("requests", [63, 64, 65, 150])
+def test_requests_of_all_lengths(requests, hkv):
+    """More blocks than CUs, which start by length: every request is found once, empty ones, equal ones and those of the
+    last, shorter batch of 64 among them."""
+    rng = np.random.default_rng(requests)
+    nodes = rng.choice([0, 1, 3, 9], requests)
+    b = Batch(requests, F16, 4 * hkv, hkv, 32, 16, rng.choice([0, 1, 30, 64, 200, 700], requests), nodes, "tree", tail=3)
+    for hints in (True, False):
+        t = b.device()
+        t["out"] = torch.full_like(t["q"], 7.0)
+        check_attention(out := run(b, t, hints, workspace=torch.empty(0, dtype=torch.uint8, device="cuda")), b,
+                        note=f"hints {hints}")
+        assert bool((out[:, int(b.cu[-1]):] == 7.0).all())
+
+
 def test_rows_that_see_nothing_are_zero():
     """Masks without a bit: with a cached prefix the rows see it, without one they see nothing."""
     for dtype in (F16, F32):
