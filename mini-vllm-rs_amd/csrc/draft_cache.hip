@@ -182,6 +182,9 @@ __global__ __launch_bounds__(kThreads) void compact_drafts_kernel(CompactDraftsP
   const int h = (int)(unit % p.num_kv_heads);
   const int64_t table = unit / p.num_kv_heads; // layer * num_seqs + request
   const int b = (int)(table % p.num_seqs);
+  // The path's first indices are on their way while the lengths are.
+  const int32_t* accepted = p.accepted + (int64_t)b * p.max_accepted;
+  int next = accepted[min(l, p.max_accepted - 1)], carry = -1;
   const const_i32* cu = (const const_i32*)p.cu_q_lens + b;
   const int seq_len = ((const const_i32*)p.seq_lens)[b], q_start = cu[0], q_end = cu[1];
   const int accepted_len = ((const const_i32*)p.accepted_lens)[b];
@@ -191,7 +194,6 @@ __global__ __launch_bounds__(kThreads) void compact_drafts_kernel(CompactDraftsP
   if (first < 0 || q_len <= 0 || seq_len > p.max_seq_len) return; // (a broken table)
   V* const kpool = static_cast<V*>(p.key_pool);
   V* const vpool = static_cast<V*>(p.value_pool);
-  const int32_t* accepted = p.accepted + (int64_t)b * p.max_accepted;
   const int32_t* bt = p.block_tables + table * p.block_table_stride;
   // First vector of the row at cache slot t, or -1.
   auto row_at = [&](int t) -> int64_t {
@@ -202,7 +204,9 @@ __global__ __launch_bounds__(kThreads) void compact_drafts_kernel(CompactDraftsP
   const int batch_rows = max(1, kWave * kBatch / row_vecs);
   for (int j0 = 0; j0 < count; j0 += kWave) {
     const int j = j0 + l;
-    const int s = j < count ? accepted[j] : -1, before = j > 0 && j < count ? accepted[j - 1] : -1;
+    const int s = j < count ? next : -1, up = __shfl_up(s, 1), before = l > 0 ? up : carry;
+    carry = __builtin_amdgcn_readlane(s, kWave - 1);
+    if (j0 + kWave < count) next = accepted[min(j + kWave, count - 1)];
     int64_t from = -1, to = -1;
     if (s > j && s < q_len && s > before) { // (s == j is in place)
       from = row_at(first + s);
