@@ -165,7 +165,7 @@ hipError_t launch_append(const NormRopeAppendParams& p, int rope_type, hipStream
 // whatever is written, its old content has been read.
 //
 // Rows of 256 bytes in random pages: 32 requests of 20..64 drafts in 32 layers (78
-// MB) take 21.5 us, 3.6 TB/s where a large copy reaches 4.9; all wavefronts are
+// MB) take 21.8 us, 3.6 TB/s where a large copy reaches 4.9; all wavefronts are
 // resident at once, so the chain of lengths, path, pages and rows shows once.
 constexpr int kBatch = 4; // vectors per lane, pool and batch
 
