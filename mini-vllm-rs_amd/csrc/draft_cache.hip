@@ -96,12 +96,29 @@ __global__ __launch_bounds__(kThreads) void norm_rope_append_kernel(NormRopeAppe
     }
   }
 
+  // The rotation's factors go out as soon as the position is known: with positions
+  // now, without them beside the page's look-up.
+  float4v c = {0.f, 0.f, 0.f, 0.f}, s = c;
+  auto load_factors = [&](int pos) {
+    if (!active || kind == 2) return;
+    const int64_t at = (int64_t)min(max(pos, 0), p.rope_len - 1) * (D / 2) + 4 * j;
+    c = load4(static_cast<const T*>(p.cos_table) + at);
+    s = load4(static_cast<const T*>(p.sin_table) + at);
+  };
+  int pos = 0;
+  if (p.positions) {
+    pos = ((const const_i32*)p.positions)[n];
+    load_factors(pos);
+  }
   TokenRequest r = {0, 0, p.total_q};
   if (p.cu_q_lens) r = request_of(p.cu_q_lens, p.num_seqs, n);
   if (r.b < 0 || r.b >= p.num_seqs) return; // behind the last request (a padded batch)
   const int seq_len = p.seq_lens ? ((const const_i32*)p.seq_lens)[r.b] : p.max_seq_len;
   const int slot = seq_len - (r.end - r.start) + (n - r.start);
-  const int pos = p.positions ? ((const const_i32*)p.positions)[n] : slot;
+  if (!p.positions) {
+    pos = slot;
+    load_factors(pos);
+  }
   // Only tables that break the contract hold such values: nothing is written.
   if (slot < 0 || slot >= p.max_seq_len || pos < 0 || pos >= p.rope_len) return;
   const int64_t page = ((const const_i32*)p.block_tables)[(int64_t)r.b * p.block_table_stride + slot / p.page_size];
@@ -122,8 +139,6 @@ __global__ __launch_bounds__(kThreads) void norm_rope_append_kernel(NormRopeAppe
          : kind == 1 ? static_cast<T*>(p.key_pool) + at
                      : static_cast<T*>(p.value_pool) + at;
   if (kind != 2) {
-    const float4v c = load4(static_cast<const T*>(p.cos_table) + (int64_t)pos * (D / 2) + 4 * j);
-    const float4v s = load4(static_cast<const T*>(p.sin_table) + (int64_t)pos * (D / 2) + 4 * j);
     float4v ylo, yhi;
     if (ROPE == 0) {
       ylo = lo * c - hi * s;
