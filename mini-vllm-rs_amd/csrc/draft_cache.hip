@@ -64,8 +64,9 @@ __device__ __forceinline__ TokenRequest request_of(const int32_t* cu, int num_se
 // while its rows are on their way.
 //
 // Bound by that chain of dependent loads (request, length, page, store): 1,024
-// tokens of 36 rows take 8.7 us in F16 at D=128, where HBM needs 3.9 and a launch
-// that does next to nothing 3.5.
+// tokens of 36 rows take 8.3 us in F16 at D=128, where HBM needs 3.9 and a launch
+// that does next to nothing 3.5.  Two row groups per wavefront: 8.2, and 1 us more
+// for 64 tokens.
 template <typename T, int ROPE>
 __global__ __launch_bounds__(kThreads) void norm_rope_append_kernel(NormRopeAppendParams p, int lanes_log2,
                                                                     int token_waves) {
@@ -180,7 +181,7 @@ hipError_t launch_append(const NormRopeAppendParams& p, int rope_type, hipStream
 // whatever is written, its old content has been read.
 //
 // Rows of 256 bytes in random pages: 32 requests of 20..64 drafts in 32 layers (78
-// MB) take 21.8 us, 3.6 TB/s where a large copy reaches 4.9; all wavefronts are
+// MB) take 21.7 us, 3.6 TB/s where a large copy reaches 4.9; all wavefronts are
 // resident at once, so the chain of lengths, path, pages and rows shows once.
 constexpr int kBatch = 4; // vectors per lane, pool and batch
 
