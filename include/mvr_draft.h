@@ -52,9 +52,11 @@ typedef struct mvr_draft_trees {
 
 /* mvr_paged_attention with the drafts' own masks in place of the causal one.
    Same arguments, layouts, dtypes, head dimensions (multiples of 32 up to
-   256), page sizes (any; nothing is repacked), hints and numerics: 32-bit
-   scores, softmax state and sums; the probabilities are rounded to the
-   activation dtype for the product with V.  Differences:
+   256), page sizes (any; nothing is repacked) and hints.  Scores, softmax state
+   and sums are held in 32 bits.  F16 probabilities enter the product with V with
+   20 bits; where requests have more than 32 rows (query heads per KV head x
+   drafts) the plan may round them to F16, and the sum is then that of the
+   rounded ones.  Differences to mvr_paged_attention:
      - a request may have q_len 0 (no drafts this step): nothing is computed
        for it, so total_q, where given, lies in [0, num_seqs * max_q_len];
      - rows of q and out from cu_q_lens[num_seqs] on are neither read nor

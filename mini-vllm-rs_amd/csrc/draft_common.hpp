@@ -194,6 +194,8 @@ __device__ __forceinline__ uint32_t visible_bits(const RowMask& m, int off) {
 // 0 for a row without a key (its sum is 0: no exponential was added), else 1 / sum.
 __device__ __forceinline__ float inverse_sum(float sum) { return __float_as_uint(sum) == 0 ? 0.f : 1.f / sum; }
 
+typedef half_t half2v __attribute__((ext_vector_type(2)));
+
 // Maximum and sum over the lanes l, l ^ 16, l ^ 32, l ^ 48, which hold one query row.
 __device__ __forceinline__ float row_max(float v) {
   const uint32_t x = __float_as_uint(v);
