@@ -179,14 +179,20 @@ class Call:
     """One call of the library, its argument block (`args`, and `extra` where the entry point takes a second one) made
     and its tensors kept.  Calling it launches on `stream`, or on the stream that is current then.
     One thread at a time may call it (another makes a Call of its own), and where there is a `workspace`, its launches must
-    not overlap in time, nor may those of Calls that share one."""
+    not overlap in time, nor may those of Calls that share one.  A graph that recorded a launch reads the argument block's
+    tensors and writes the workspace at every replay: keep the Call as long as the graph.
+    workspace_stream: handle of the stream whose memory the workspace is, where this module made it; None: the caller's."""
 
-    def __init__(self, name, args, extra, tensors, device, stream, workspace=None):
+    def __init__(self, name, args, extra, tensors, device, stream, workspace=None, workspace_stream=None):
         self._function = getattr(load_library(), name)
         self.args, self.extra, self.workspace = args, extra, workspace
         self._refs = (ctypes.byref(args),) if extra is None else (ctypes.byref(args), ctypes.byref(extra))
         self._tensors = tuple(t for t in tensors if t is not None)
+        if workspace is not None and workspace_stream is None:
+            self._tensors += (workspace,)
         self._device, self._stream = device, stream
+        # Streams that the workspace made here is known to be used on (the allocator's record lasts until it is freed).
+        self._known = None if workspace_stream is None else {workspace_stream}
         self._cuda = M._torch().cuda
         if stream is not None and stream.device != device:
             _refuse(f"a stream of {stream.device} for tensors of {device}")
@@ -197,16 +203,15 @@ class Call:
             with cuda.device(self._device):
                 return self()
         current = _raw_current_stream(index)
-        if self._stream is None:
-            self.args.stream = current
-        else:
-            self.args.stream = self._stream.cuda_stream
-            if self._stream.cuda_stream != current:
-                # Freed on their own stream before the kernels ran, their memory must not be handed out meanwhile.
-                for t in self._tensors:
-                    t.record_stream(self._stream)
-                if self.workspace is not None:
-                    self.workspace.record_stream(self._stream)
+        launch = current if self._stream is None else self._stream.cuda_stream
+        self.args.stream = launch
+        # Memory that is freed while kernels of another stream than its own still use it must not be handed out meanwhile.
+        if launch != current:
+            for t in self._tensors:
+                t.record_stream(self._stream)
+        if self._known is not None and launch not in self._known:
+            self.workspace.record_stream(self._stream or cuda.current_stream(index))
+            self._known.add(launch)
         _check(self._function(*self._refs))
 
 
@@ -256,12 +261,14 @@ def make_tree_call(q, key_pool, value_pool, block_tables, seq_lens, cu_q_lens, m
         if a.total_q > a.num_seqs * max_q_len:  # rows behind the last request (a padded batch)
             a.total_q = 0
         need = int(load_library().mvr_paged_attention_tree_workspace_size(ctypes.byref(a), ctypes.byref(t)))
+        made_on = None
         if need and workspace is None:
-            workspace = M.new_workspace(need, device)
+            workspace, made_on = M.new_workspace(need, device), _raw_current_stream(device.index)
         if workspace is not None:
             a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     return Call("mvr_paged_attention_tree", a, t,
-                (q, key_pool, value_pool, block_tables, seq_lens, cu_q_lens, masks, out), device, stream, workspace)
+                (q, key_pool, value_pool, block_tables, seq_lens, cu_q_lens, masks, out), device, stream, workspace=workspace,
+                workspace_stream=made_on)
 
 
 def paged_attention_tree(q, key_pool, value_pool, block_tables, seq_lens, cu_q_lens, masks, out=None, *,
