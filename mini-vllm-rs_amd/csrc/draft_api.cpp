@@ -101,41 +101,130 @@ int check_tree(const mvr_paged_attention_args* a, const mvr_draft_trees* t) {
   return MVR_OK;
 }
 
-// The requests as the planner sees them: the host tables where they are given
-// and within the call's bounds, else every request at those bounds.
-struct Request {
-  int64_t count, rows, units; // requests alike: grouped rows per KV head, key units
-  int64_t more;               // units and parts that one may have beyond these
-};
-
-bool host_tables_fit(const mvr_paged_attention_args* a) {
-  const int32_t* cu = a->cu_q_lens_host;
-  const int32_t* sl = a->seq_lens_host;
-  if (!cu || !sl) return false;
-  for (int s = 0; s < a->num_seqs; s++) {
-    const int64_t q = (int64_t)cu[s + 1] - cu[s];
-    if (q < 0 || q > a->max_q_len || sl[s] < q || sl[s] > a->max_seq_len) return false;
-  }
-  return true;
-}
-
 int64_t units_of(int64_t tokens) { return (tokens + mvr::kDraftUnitTokens - 1) / mvr::kDraftUnitTokens; }
 
-template <typename F>
-void each_request(const mvr_paged_attention_args* a, bool tables, F f) {
-  const int64_t group = a->num_q_heads / a->num_kv_heads;
-  if (!tables) {
-    // sum_seq_lens alone tells the average context: requests of other lengths round
-    // up to a unit and a part more each.
-    const int64_t tokens = a->sum_seq_lens > 0 ? (a->sum_seq_lens + a->num_seqs - 1) / a->num_seqs : a->max_seq_len;
-    f(Request{a->num_seqs, group * a->max_q_len, units_of(tokens), tokens < a->max_seq_len});
-    return;
+constexpr int kTileSizes = 4;
+constexpr int kTileRowsLog2[kTileSizes] = {4, 5, 6, 7};
+
+// The requests as the planner sees them: the host tables where they are given and
+// within the call's bounds, else every request at those bounds.  Two passes over the
+// tables, whatever is planned on them afterwards: they leave, for each tile size, the
+// row tiles of requests of each length, from whose sums over the longer lengths a
+// split's parts are counted in a few look-ups (64 at most, a request's most parts).
+class Requests {
+ public:
+  explicit Requests(const mvr_paged_attention_args* a) : hkv_(a->num_kv_heads) {
+    const int64_t group = a->num_q_heads / a->num_kv_heads;
+    tables_ = read_bounds(a);
+    if (!tables_) {
+      // sum_seq_lens alone tells the average context: requests of other lengths round
+      // up to a unit and a part more each.
+      const int64_t tokens = a->sum_seq_lens > 0 ? (a->sum_seq_lens + a->num_seqs - 1) / a->num_seqs : a->max_seq_len;
+      const int64_t rows = group * a->max_q_len;
+      longest = shortest = units_of(tokens);
+      more_ = tokens < a->max_seq_len;
+      all_units = a->num_seqs * longest;
+      for (int t = 0; t < kTileSizes; t++) {
+        tiles[t] = a->num_seqs * hkv_ * tiles_of(rows, t);
+        work[t] = tiles[t] * longest;
+      }
+      return;
+    }
+    while (longest >> scale_ >= kBuckets) scale_++;
+    const int top = bucket(longest);
+    std::fill(longest_in_, longest_in_ + top + 1, 0);
+    for (int t = 0; t < kTileSizes; t++) std::fill(from_[t], from_[t] + top + 2, 0);
+    for (int s = 0; s < a->num_seqs; s++) {
+      const int64_t rows = group * (a->cu_q_lens_host[s + 1] - a->cu_q_lens_host[s]);
+      if (rows == 0) continue;
+      const int64_t units = units_of(a->seq_lens_host[s]);
+      const int b = bucket(units);
+      all_units += units;
+      longest_in_[b] = b;
+      for (int t = 0; t < kTileSizes; t++) {
+        const int64_t n = tiles_of(rows, t);
+        from_[t][b] += (int32_t)n;
+        tiles[t] += n;
+        work[t] += n * units;
+      }
+    }
+    for (int b = 1; b <= top; b++) longest_in_[b] = std::max(longest_in_[b], longest_in_[b - 1]);
+    for (int t = 0; t < kTileSizes; t++) {
+      for (int b = top - 1; b >= 1; b--) from_[t][b] += from_[t][b + 1];
+      tiles[t] *= hkv_;
+      work[t] *= hkv_;
+    }
   }
-  for (int s = 0; s < a->num_seqs; s++) {
-    const int64_t q = a->cu_q_lens_host[s + 1] - a->cu_q_lens_host[s];
-    if (q > 0) f(Request{1, group * q, units_of(a->seq_lens_host[s]), 0});
+
+  // Items of the tile size where every request is split in parts of at most `part`
+  // units (kDraftMaxParts parts at most).  (Lengths of kBuckets units or more count as
+  // rounded up by 1 / 512 at most.)
+  int64_t items(int t, int64_t part) const {
+    if (!tables_) return tiles[t] * uniform_parts(part);
+    const int64_t end = longest_counted();
+    int64_t n = 0, at = 0; // a request has a k-th part where it is longer than k parts
+    for (int k = 0; k < mvr::kDraftMaxParts && at < end; k++, at += part) n += from_[t][(at >> scale_) + 1];
+    return n * hkv_;
   }
-}
+
+  // Units of the longest part then.
+  int64_t longest_part(int64_t part) const {
+    if (!tables_) return (longest + uniform_parts(part) - 1) / uniform_parts(part);
+    const int64_t end = longest_counted();
+    const int64_t most = std::min<int64_t>((end + part - 1) / part, mvr::kDraftMaxParts);
+    int64_t best = (end + most - 1) / most;
+    for (int64_t k = 1; k < most && best < part; k++) { // the longest request of k parts
+      const int64_t units = (int64_t)longest_in_[(k * part) >> scale_] << scale_;
+      if (units > (k - 1) * part) best = std::max(best, (units + k - 1) / k);
+    }
+    return best;
+  }
+
+  bool from_tables() const { return tables_; }
+
+  int64_t longest = 0, shortest = 0;           // units; 0: no request has drafts
+  int64_t all_units = 0;                       // of all requests
+  int64_t tiles[kTileSizes] = {};              // row tiles, over the KV heads
+  int64_t work[kTileSizes] = {};               // tiles x units
+
+ private:
+  static constexpr int kBuckets = 1024; // of units, 2^scale_ each
+
+  static int64_t tiles_of(int64_t rows, int t) { return (rows + (1 << kTileRowsLog2[t]) - 1) >> kTileRowsLog2[t]; }
+  int bucket(int64_t units) const { return (int)((units + ((int64_t)1 << scale_) - 1) >> scale_); }
+  int64_t longest_counted() const { return (int64_t)bucket(longest) << scale_; }
+  int64_t uniform_parts(int64_t part) const {
+    return std::min<int64_t>((longest + more_ + part - 1) / part + more_, mvr::kDraftMaxParts);
+  }
+
+  // Longest and shortest of the requests with drafts; false where the tables are not
+  // given or leave the call's bounds.
+  bool read_bounds(const mvr_paged_attention_args* a) {
+    const int32_t* cu = a->cu_q_lens_host;
+    const int32_t* sl = a->seq_lens_host;
+    if (!cu || !sl) return false;
+    int32_t most = 0, least = INT32_MAX;
+    for (int s = 0; s < a->num_seqs; s++) {
+      const int64_t q = (int64_t)cu[s + 1] - cu[s];
+      if (q < 0 || q > a->max_q_len || sl[s] < q || sl[s] > a->max_seq_len) return false;
+      if (q == 0) continue;
+      most = std::max(most, sl[s]);
+      least = std::min(least, sl[s]);
+    }
+    if (most > 0) {
+      longest = units_of(most);
+      shortest = units_of(least);
+    }
+    return true;
+  }
+
+  int64_t hkv_;
+  bool tables_;
+  int64_t more_ = 0; // units and parts that a request may have beyond the average
+  int scale_ = 0;
+  int32_t from_[kTileSizes][kBuckets + 2]; // [t][b]: row tiles (of a KV head) of the requests of bucket b or longer
+  int32_t longest_in_[kBuckets + 2];       // [b]: the longest bucket up to b that holds a request, or 0
+};
 
 // What a block of one tile size costs, in us, for head_dim 128: `fixed` beside
 // its keys, `unit` per 64 keys with one to four blocks on its CU.  Fitted to 965
@@ -162,11 +251,13 @@ constexpr TileCost kF32Costs[] = {{16, 2.5, {1.97, 4.05, 6.23, 8.55}}, {32, 5.8,
 // 256 of 63 in 98).  A split call scans the lengths and merges: 4.5 us, and its
 // partial results written and read at 4.3 TB/s.
 mvr::DraftAttentionPlan plan_tree(const mvr_paged_attention_args* a, size_t limit) {
-  const bool f16 = a->dtype == MVR_DTYPE_F16, tables = host_tables_fit(a);
+  const bool f16 = a->dtype == MVR_DTYPE_F16;
+  const Requests requests(a);
+  const int64_t longest = requests.longest, shortest = requests.shortest;
   const double unit_scale = a->head_dim / 128.0;
   const int64_t cus = mvr::api::compute_units(), hkv = a->num_kv_heads;
   const int64_t longest_rows = (int64_t)(a->num_q_heads / a->num_kv_heads) * a->max_q_len;
-  const double key_us = 2.0 * mvr::kDraftUnitTokens * hkv * a->head_dim * es_of(a->dtype) / 5.9e6; // of a request's unit
+  const double hbm = requests.all_units * (2.0 * mvr::kDraftUnitTokens * hkv * a->head_dim * es_of(a->dtype) / 5.9e6);
   // Overrides, for tests and tuning: a tile size that the head dimension has, and
   // its parts.
   static const int set_rows = mvr::api::env_int("MVR_DRAFT_TILE_ROWS", 0);
@@ -176,22 +267,13 @@ mvr::DraftAttentionPlan plan_tree(const mvr_paged_attention_args* a, size_t limi
     rows_set |= tile.rows == set_rows && mvr::draft_tile_supported(set_rows, a->head_dim);
   mvr::DraftAttentionPlan best{};
   double best_cost = INFINITY;
-  for (const TileCost& tile : f16 ? kF16Costs : kF32Costs) {
+  for (int t = 0; t < kTileSizes; t++) {
+    const TileCost& tile = f16 ? kF16Costs[t] : kF32Costs[t];
     if (!mvr::draft_tile_supported(tile.rows, a->head_dim)) continue;
     // (A tile that no request fills half costs what the smaller one does, or more.)
     if (rows_set ? tile.rows != set_rows : longest_rows <= tile.rows / 2 && best_cost < INFINITY) continue;
     const int held = mvr::draft_blocks_per_cu(tile.rows, f16, a->head_dim);
-    auto tiles_of = [&](const Request& r) { return r.count * hkv * ((r.rows + tile.rows - 1) / tile.rows); };
-    int64_t tiles = 0, work = 0, longest = 0, shortest = INT64_MAX;
-    double hbm = 0;
-    each_request(a, tables, [&](const Request& r) {
-      if (r.units == 0) return;
-      tiles += tiles_of(r);
-      work += tiles_of(r) * r.units;
-      longest = std::max(longest, r.units);
-      shortest = std::min(shortest, r.units);
-      hbm += r.count * r.units * key_us;
-    });
+    const int64_t tiles = requests.tiles[t], work = requests.work[t];
     auto cost_of = [&](int64_t blocks, int64_t part, int64_t last) { // of `part` units at most, the last one of `last`
       double body;
       if (blocks <= held * cus)
@@ -212,47 +294,55 @@ mvr::DraftAttentionPlan plan_tree(const mvr_paged_attention_args* a, size_t limi
       const int64_t pairs = (a->num_seqs * hkv + mvr::kDraftXcds - 1) / mvr::kDraftXcds * mvr::kDraftXcds;
       best.blocks = (int)(part ? items : pairs * best.row_tiles);
       // (Finding a length's rank takes 0.3 us: not where all are alike, or start at once.)
-      best.by_length = part == 0 && best.blocks > cus && (!tables || shortest < longest);
+      best.by_length = part == 0 && best.blocks > cus && (!requests.from_tables() || shortest < longest);
       best.partial_bytes = bytes;
     };
-    int64_t items = 0, part_longest = 0;
-    size_t bytes = 0;
-    auto split_at = [&](int64_t part) {
-      items = part_longest = 0;
-      each_request(a, tables, [&](const Request& r) {
-        const int64_t parts = std::min<int64_t>((r.units + r.more + part - 1) / part + r.more, mvr::kDraftMaxParts);
-        if (parts == 0) return;
-        items += tiles_of(r) * parts;
-        part_longest = std::max(part_longest, (r.units + parts - 1) / parts);
-      });
-      bytes = align_up((size_t)items * tile.rows * a->head_dim * sizeof(float), 256) +
-              align_up((size_t)items * tile.rows * 2 * sizeof(float), 256);
+    auto bytes_of = [&](int64_t items) {
+      return align_up((size_t)items * tile.rows * a->head_dim * sizeof(float), 256) +
+             align_up((size_t)items * tile.rows * 2 * sizeof(float), 256);
     };
     auto take_split = [&](int64_t part) {
+      const int64_t items = requests.items(t, part), part_longest = requests.longest_part(part);
+      const size_t bytes = bytes_of(items);
       take(cost_of(items, part_longest, part_longest) + 4.5 + 2 * bytes / 4.3e6, part, items, bytes);
     };
     // (The blocks of a split call and of its merge have to fit a launch each.)
     const bool may_split = limit > 0 && longest > 1 &&
                            a->num_seqs * hkv * ((longest_rows + 15) / 16) <= kMaxThreads / 256 / 64;
-    if (may_split && set_units && set_units < longest) {
-      split_at(set_units);
-      if (bytes <= limit) {
-        take_split(set_units);
-        continue;
-      }
+    if (may_split && set_units && set_units < longest && bytes_of(requests.items(t, set_units)) <= limit) {
+      take_split(set_units);
+      continue;
     }
-    take(cost_of(tiles, longest, longest ? shortest : 0), 0, 0, 0);
+    take(cost_of(tiles, longest, shortest), 0, 0, 0);
     if (!may_split || set_units) continue;
+    int64_t last = 0;
     for (int64_t target = cus; target <= 4 * held * cus; target += target < held * cus ? cus : held * cus) {
       if (tiles >= target) continue;
-      // The shortest parts whose blocks are no more than `target`: from an estimate
-      // (a request's last part is half full on average) upwards.
+      // The shortest parts whose blocks are no more than `target`, in steps of 1/16: from
+      // an estimate (a request's last part is half full on average) upwards.  Longer
+      // parts are fewer: bisected, from the length whose parts are few enough even where
+      // every request's last one holds a single unit.
+      auto fits = [&](int64_t part) {
+        const int64_t items = requests.items(t, part);
+        return items <= target && bytes_of(items) <= limit;
+      };
       int64_t part = std::max<int64_t>(1, work / (target - tiles / 2));
-      for (; part < longest; part += 1 + part / 16) {
-        split_at(part);
-        if (items <= target && bytes <= limit) break;
+      if (part >= longest) continue;
+      if (!fits(part)) {
+        int64_t below = part, above = std::min(longest - 1, std::max(part + 1, work / (target - tiles) + 1));
+        if (!fits(above)) {
+          below = above;
+          above = longest - 1;
+          if (below >= above || !fits(above)) continue;
+        }
+        while (above - below > 1) {
+          const int64_t middle = below + (above - below) / 2;
+          (fits(middle) ? above : below) = middle;
+        }
+        while (part < above) part += 1 + part / 16;
       }
-      if (part < longest) take_split(part);
+      if (part < longest && part != last) take_split(part);
+      last = part;
     }
   }
   return best;
