@@ -58,7 +58,9 @@ typedef struct mvr_draft_trees {
    drafts) the plan may round them to F16, and the sum is then that of the
    rounded ones.  Differences to mvr_paged_attention:
      - a request may have q_len 0 (no drafts this step): nothing is computed
-       for it, so total_q, where given, lies in [0, num_seqs * max_q_len];
+       for it, so total_q, where given, lies in [0, num_seqs * max_q_len].  All
+       of them may; max_q_len is 1 at least and q, out and masks are there even
+       so (a step without any token can leave the call out);
      - rows of q and out from cu_q_lens[num_seqs] on are neither read nor
        written;
      - a device q_len above max_q_len is clamped to it;
@@ -101,8 +103,10 @@ typedef struct mvr_head_norms {
    rounding follows the reference's kernels, rounds every product and sum).
    The row of token i of request b goes to slot seq_len - q_len + i, wherever
    it is rotated to.  Arguments are mvr_rope_append's; here
-     - a request may have q_len 0, and total_q may exceed cu_q_lens[num_seqs]
-       (a padded batch): rows from there on do not matter and are not written;
+     - a request may have q_len 0, and total_q, 1 at least, may exceed
+       cu_q_lens[num_seqs] (a padded batch): rows from there on do not matter
+       and are not written.  A step without any token makes no call, or one on
+       a padded batch;
      - rope_len need only cover the positions: rows whose position is outside
        [0, rope_len), or whose slot is outside [0, max_seq_len), or whose page
        is outside the pool, are left out. */

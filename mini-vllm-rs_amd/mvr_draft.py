@@ -12,6 +12,7 @@ and per step, over the block tables of all layers:
 make_*_call(...) builds the argument block (and workspace) of one call once: the object that it returns makes the call,
 on the stream that is current then unless it was given one, as a runner repeats it step by step or records it into a
 graph.  The functions above build one and call it.  Tensors are torch tensors on one GPU; errors are mvr_attn.MvrError.
+A call on tensors without rows (no request has a draft this step) launches nothing.
 """
 from __future__ import annotations
 
@@ -181,16 +182,17 @@ class Call:
     One thread at a time may call it (another makes a Call of its own), and where there is a `workspace`, its launches must
     not overlap in time, nor may those of Calls that share one.  A graph that recorded a launch reads the argument block's
     tensors and writes the workspace at every replay: keep the Call as long as the graph.
-    workspace_stream: handle of the stream whose memory the workspace is, where this module made it; None: the caller's."""
+    workspace_stream: handle of the stream whose memory the workspace is, where this module made it; None: the caller's.
+    empty: its tensors have no rows, there is nothing to launch."""
 
-    def __init__(self, name, args, extra, tensors, device, stream, workspace=None, workspace_stream=None):
+    def __init__(self, name, args, extra, tensors, device, stream, workspace=None, workspace_stream=None, empty=False):
         self._function = getattr(load_library(), name)
         self.args, self.extra, self.workspace = args, extra, workspace
         self._refs = (ctypes.byref(args),) if extra is None else (ctypes.byref(args), ctypes.byref(extra))
         self._tensors = tuple(t for t in tensors if t is not None)
         if workspace is not None and workspace_stream is None:
             self._tensors += (workspace,)
-        self._device, self._stream = device, stream
+        self._device, self._stream, self._empty = device, stream, empty
         # Streams that the workspace made here is known to be used on (the allocator's record lasts until it is freed).
         self._known = None if workspace_stream is None else {workspace_stream}
         self._cuda = M._torch().cuda
@@ -198,6 +200,8 @@ class Call:
             _refuse(f"a stream of {stream.device} for tensors of {device}")
 
     def __call__(self):
+        if self._empty:
+            return
         cuda, index = self._cuda, self._device.index
         if cuda.current_device() != index:
             with cuda.device(self._device):
@@ -268,7 +272,7 @@ def make_tree_call(q, key_pool, value_pool, block_tables, seq_lens, cu_q_lens, m
             a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     return Call("mvr_paged_attention_tree", a, t,
                 (q, key_pool, value_pool, block_tables, seq_lens, cu_q_lens, masks, out), device, stream, workspace=workspace,
-                workspace_stream=made_on)
+                workspace_stream=made_on, empty=q.shape[1] == 0)
 
 
 def paged_attention_tree(q, key_pool, value_pool, block_tables, seq_lens, cu_q_lens, masks, out=None, *,
@@ -315,7 +319,7 @@ def make_norm_rope_append_call(q, k, v, q_weight, k_weight, cos_table, sin_table
                                     value_pool, q_out, max_seq_len=max_seq_len, rope_type=rope_type, stream=stream)
     return Call("mvr_norm_rope_append", a, n,
                 (q, k, v, q_weight, k_weight, cos_table, sin_table, block_tables, seq_lens, cu_q_lens, key_pool,
-                 value_pool, q_out, positions), device, stream)
+                 value_pool, q_out, positions), device, stream, empty=q.shape[1] == 0)
 
 
 def norm_rope_append(q, k, v, q_weight, k_weight, cos_table, sin_table, block_tables, seq_lens, cu_q_lens, key_pool,
