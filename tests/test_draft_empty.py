@@ -14,6 +14,7 @@ import mvr_draft as D  # noqa: E402
 def no_gpu(monkeypatch):
     """CPU tensors pass for a GPU's, and nothing may be launched on them."""
     monkeypatch.setattr(D, "_same_device", lambda *t: torch.device("cuda", 0))
+    monkeypatch.setattr(M, "_stream_handle", lambda stream: 0)
     monkeypatch.setattr(D, "_scope", lambda device, stream: contextlib.nullcontext())
 
 
