@@ -392,48 +392,73 @@ def copy_pages(key_pool, value_pool, src_pages, dst_pages, tokens=None, *, strea
     make_copy_pages_call(key_pool, value_pool, src_pages, dst_pages, tokens, stream=stream)()
 
 
-def _host(keep, x, dtype="int32"):
+def _host_table(keep, x, name, entries, dtype="int32"):
+    """Address of a host table of at least `entries` entries, as the library reads it."""
     if x is None:
         return None
     import numpy as np
 
     x = np.ascontiguousarray(x, dtype=dtype)
+    if x.size < entries:
+        _refuse(f"{name} must hold {entries} entries, not {x.size}")
     keep.append(x)
     return x.ctypes.data
+
+
+def _rows_read(args, cu_q_lens_host, alone):
+    """Rows of a per-token table that a check reads: the requests' tokens; `alone` of one request without cu_q_lens."""
+    if cu_q_lens_host is None:
+        return alone if args.num_seqs == 1 else 0
+    rows = max((int(x) for x in cu_q_lens_host), default=0)  # (starts that do not ascend are refused before any row is read)
+    return min(rows, args.total_q) if args.total_q > 0 else rows
 
 
 def validate_tree(args: M.PagedAttentionArgs, trees: DraftTrees, block_tables_host=None, seq_lens_host=None,
                   cu_q_lens_host=None, masks_host=None) -> None:
     """Host-side checks of a tree call's tables (numpy arrays or None); raises MvrError."""
-    keep = []
-    _check(load_library().mvr_paged_attention_tree_validate(
-        ctypes.byref(args), ctypes.byref(trees), _host(keep, block_tables_host), _host(keep, seq_lens_host),
-        _host(keep, cu_q_lens_host), None if masks_host is None else _host(keep, masks_host.view("uint32"), "uint32")))
+    keep, n = [], args.num_seqs
+    tables = (_host_table(keep, block_tables_host, "block_tables_host", n * args.max_pages_per_seq),
+              _host_table(keep, seq_lens_host, "seq_lens_host", n),
+              _host_table(keep, cu_q_lens_host, "cu_q_lens_host", n + 1))
+    if masks_host is not None:
+        if masks_host.dtype.itemsize != 4:
+            _refuse(f"masks_host must hold 32-bit words, not {masks_host.dtype}")
+        masks_host = masks_host.view("uint32")
+    masks = _host_table(keep, masks_host, "masks_host",
+                        _rows_read(args, cu_q_lens_host, args.max_q_len) * trees.mask_words, "uint32")
+    _check(load_library().mvr_paged_attention_tree_validate(ctypes.byref(args), ctypes.byref(trees), *tables, masks))
 
 
 def validate_norm_rope_append(args: M.RopeAppendArgs, norms: HeadNorms, block_tables_host=None, seq_lens_host=None,
                               cu_q_lens_host=None, positions_host=None, page_writable_host=None) -> None:
     """Host-side checks of an append's tables (numpy arrays or None); raises MvrError."""
-    keep = []
-    _check(load_library().mvr_norm_rope_append_validate(
-        ctypes.byref(args), ctypes.byref(norms), _host(keep, block_tables_host), _host(keep, seq_lens_host),
-        _host(keep, cu_q_lens_host), _host(keep, positions_host), _host(keep, page_writable_host, "uint8")))
+    keep, n = [], args.num_seqs
+    tables = (_host_table(keep, block_tables_host, "block_tables_host", n * args.max_pages_per_seq),
+              _host_table(keep, seq_lens_host, "seq_lens_host", n),
+              _host_table(keep, cu_q_lens_host, "cu_q_lens_host", n + 1),
+              _host_table(keep, positions_host, "positions_host", _rows_read(args, cu_q_lens_host, args.total_q)),
+              _host_table(keep, page_writable_host, "page_writable_host", args.num_pages, "uint8"))
+    _check(load_library().mvr_norm_rope_append_validate(ctypes.byref(args), ctypes.byref(norms), *tables))
 
 
 def validate_compact_drafts(args: CompactDraftsArgs, block_tables_host=None, seq_lens_host=None, cu_q_lens_host=None,
                             accepted_host=None, accepted_lens_host=None) -> None:
     """Host-side checks of a compaction's tables (numpy arrays or None); raises MvrError."""
-    keep = []
-    _check(load_library().mvr_compact_drafts_validate(
-        ctypes.byref(args), _host(keep, block_tables_host), _host(keep, seq_lens_host), _host(keep, cu_q_lens_host),
-        _host(keep, accepted_host), _host(keep, accepted_lens_host)))
+    keep, n = [], args.num_seqs
+    tables = (_host_table(keep, block_tables_host, "block_tables_host", args.num_layers * n * args.max_pages_per_seq),
+              _host_table(keep, seq_lens_host, "seq_lens_host", n),
+              _host_table(keep, cu_q_lens_host, "cu_q_lens_host", n + 1),
+              _host_table(keep, accepted_host, "accepted_host", n * args.max_accepted),
+              _host_table(keep, accepted_lens_host, "accepted_lens_host", n))
+    _check(load_library().mvr_compact_drafts_validate(ctypes.byref(args), *tables))
 
 
 def validate_copy_pages(args: CopyPagesArgs, src_pages_host=None, dst_pages_host=None, tokens_host=None) -> None:
     """Host-side checks of a copy's lists (numpy arrays or None); raises MvrError."""
-    keep = []
-    _check(load_library().mvr_copy_pages_validate(ctypes.byref(args), _host(keep, src_pages_host),
-                                                  _host(keep, dst_pages_host), _host(keep, tokens_host)))
+    keep, n = [], args.num_copies
+    _check(load_library().mvr_copy_pages_validate(ctypes.byref(args), _host_table(keep, src_pages_host, "src_pages_host", n),
+                                                  _host_table(keep, dst_pages_host, "dst_pages_host", n),
+                                                  _host_table(keep, tokens_host, "tokens_host", n)))
 
 
 def tree_masks(parents, cu_q_lens, mask_words: Optional[int] = None):
