@@ -147,7 +147,7 @@ int check_scalars(const mvr_paged_attention_args* a) {
   if (a->num_seqs == 1 && !a->cu_q_lens && a->total_q > 0 && a->total_q < a->max_q_len)
     return fail(MVR_E_INVALID_ARGUMENT, "total_q %d is smaller than max_q_len %d, the q_len of a call without cu_q_lens",
                 a->total_q, a->max_q_len);
-  const int64_t pages_needed = (a->max_seq_len + a->page_size - 1) / a->page_size;
+  const int64_t pages_needed = (a->max_seq_len + (int64_t)a->page_size - 1) / a->page_size;
   if (a->max_pages_per_seq < pages_needed)
     return fail(MVR_E_PAGES_UNCOVERED,
                 "paged KV cache contains fewer pages than its sequence length, leaving %lld tokens uncovered",
