@@ -229,9 +229,12 @@ class Requests {
 // What a block of one tile size costs, in us, for head_dim 128: `fixed` beside
 // its keys, `unit` per 64 keys with one to four blocks on its CU.  Fitted to 965
 // timed plans (tile sizes and splits of 53 calls: 1 to 64 requests on 100 to 16,000
-// tokens, 1 to 840 rows per KV head, head_dim 64 and 128, both types): the plan
-// that these costs make fastest takes 1.1% longer than the fastest of its call on
-// average, 11% at most.  F32 products take 7 times as long as F16 ones.
+// tokens, 1 to 840 rows per KV head, head_dim 64 and 128, both types).  Timed again
+// since, the plan that these costs make fastest takes 0.9% longer than the fastest of
+// 989 plans of those calls on average, 12% at most (4 drafts on 4,000 keys); on 20
+// calls of other head dimensions and page sizes 6%, and 28 to 44% on F16 calls of many
+// rows on 5-token pages and of head_dim 32: neither has costs of its own.  F32 products
+// take 7 times as long as F16 ones.
 struct TileCost {
   int rows;
   double fixed, unit[4];

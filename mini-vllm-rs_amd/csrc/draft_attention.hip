@@ -187,8 +187,8 @@ __device__ __forceinline__ void stream_item(const DraftAttentionParams& p, const
   // towards 0, p - hi is exact in 32 bits.  With hi alone, off by up to 2^-11 p, calls
   // of few rows came out 1.4 times as far from the formula as a form that holds 32
   // bits, and up to 1.8 times.  The second product is free where HBM is the bound (64
-  // requests of 1 token on 500..3,500 keys 110.6 -> 110.5 us), and costs 0 to 4% where
-  // a block's steps are (1 x 16 on 1,000 9.3 -> 9.7).
+  // requests of 1 token on 500..3,500 keys 110.6 -> 110.5 us), and costs 0 to 5% where
+  // a block's steps are (1 x 16 on 1,000 9.2 -> 9.7).
   auto pv = [&](int le, const float4v (&pr)[NB][C]) {
     if constexpr (sizeof(T) == 2) {
       half8 hi[NB], lo[NB];

@@ -116,8 +116,8 @@ __device__ __forceinline__ int request_of_rank(const DraftAttentionParams& p, in
 // run on one XCD, take the (request, KV head) pairs that are w % 8 modulo 8, row
 // tile by row tile.  Requests of unequal lengths load the XCDs alike that way, and
 // with by_length the longest start first (F16, 64 requests of 60 drafts on
-// 300..4,000 keys, 28 / 4 heads of 128: 196 -> 180 us; F32, 40 of 10 on 100..1,500,
-// 24 / 8 heads: 111 -> 82).
+// 300..4,000 keys, 28 / 4 heads of 128: 190 -> 164 us; F32, 40 of 10 on 100..1,500,
+// 24 / 8 heads: 96 -> 81).
 template <int kTileRows>
 __device__ __forceinline__ DraftItem find_item(const DraftAttentionParams& p, int w) {
   if (p.part_units == 0) {

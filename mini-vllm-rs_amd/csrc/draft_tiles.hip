@@ -16,10 +16,11 @@
 // more than 2^8: P stays below 2^8 in F16, and sums are 32 bits.
 //
 // Bound by HBM on long contexts (64 requests of 32 drafts on 8,192 keys, 32 / 8
-// heads of 128, F16: 392 us, 5.6 TB/s, the matrix pipe 38% busy), else by a step's
-// chain of product, softmax, product: a block of 128 rows takes 1.43 us per 64 keys
-// alone on its CU, two take 1.9 (1.1 PFLOP/s over the card), which is why two
-// blocks share a CU rather than one with deeper stages.  Beside its steps a block
+// heads of 128, F16: 398 us in a loop of calls, 5.5 TB/s, 380 to 450 with the card's
+// state; the matrix pipe is 38% busy), else by a step's chain of product, softmax,
+// product: a block of 128 rows takes 1.38 us per 64 keys alone on its CU, 448 blocks
+// on 256 CUs take 2.02 (0.93 PFLOP/s), which is why two blocks share a CU rather
+// than one with deeper stages.  Beside its steps a block
 // takes some 5 us more than a launch: scan, Q and masks, first loads, draft steps,
 // stores.
 #include "draft_common.hpp"
