@@ -21,48 +21,7 @@
 
 namespace {
 
-using mvr::api::fail;
-
-size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
-
-int es_of(int32_t dtype) { return dtype == MVR_DTYPE_F16 ? 2 : 4; }
-
-int launch_status(hipError_t err) {
-  return err == hipSuccess ? MVR_OK : fail(MVR_E_HIP, "kernel launch failed: %s", hipGetErrorString(err));
-}
-
-const int32_t* data_or_null(const std::vector<int32_t>& v) { return v.empty() ? nullptr : v.data(); }
-
-// Checked mode: runs `check` on host copies of the device tables; the host
-// memory that they take may not be there.
-template <typename F>
-int run_checked(F check) {
-  try {
-    return check();
-  } catch (const std::exception&) { // (bad_alloc, or more than a vector may hold)
-    return fail(MVR_E_INVALID_ARGUMENT, "checked mode: out of host memory");
-  }
-}
-
-// Threads of one launch, over all its blocks.
-constexpr int64_t kMaxThreads = UINT32_MAX;
-
-// Host tables of q_lens: starts that ascend from 0 and end by total_q (0: not given).
-// Whatever is read per token afterwards lies within them.
-int check_cu_q_lens(const int32_t* cu, int num_seqs, int32_t total_q, int32_t max_q_len = INT32_MAX) {
-  if (cu[0] != 0) return fail(MVR_E_INVALID_ARGUMENT, "cu_q_lens[0] must be 0");
-  for (int s = 0; s < num_seqs; s++)
-    if (cu[s + 1] < cu[s] || (int64_t)cu[s + 1] - cu[s] > max_q_len)
-      return max_q_len == INT32_MAX
-                 ? fail(MVR_E_INVALID_ARGUMENT, "cu_q_lens decreases at request %d", s)
-                 : fail(MVR_E_INVALID_ARGUMENT, "request %d has q_len %lld outside [0, max_q_len %d]", s,
-                        (long long)cu[s + 1] - cu[s], max_q_len);
-  if (total_q > 0 && cu[num_seqs] > total_q)
-    return fail(MVR_E_INVALID_ARGUMENT, "cu_q_lens[num_seqs] = %d exceeds total_q = %d", cu[num_seqs], total_q);
-  return MVR_OK;
-}
-
-int copy_failed() { return fail(MVR_E_HIP, "checked mode: copying the device tables to the host failed"); }
+using namespace mvr::api;
 
 // ---------------------------------------------------------------------------
 // Tree attention
@@ -617,21 +576,6 @@ int mvr_norm_rope_append(const mvr_rope_append_args* a, const mvr_head_norms* n)
 // ---------------------------------------------------------------------------
 // Compaction
 // ---------------------------------------------------------------------------
-
-static int check_pool(int32_t dtype, int32_t num_kv_heads, int32_t head_dim, int32_t page_size, int64_t num_pages,
-                      const void* key_pool, const void* value_pool) {
-  if (dtype != MVR_DTYPE_F32 && dtype != MVR_DTYPE_F16)
-    return fail(MVR_E_UNSUPPORTED, "dtype %d is not F32 (0) or F16 (1)", dtype);
-  if (num_kv_heads < 1 || page_size < 1 || head_dim < 1 || num_pages < 1)
-    return fail(MVR_E_INVALID_ARGUMENT, "invalid pool geometry");
-  // A page's elements are counted in 32 bits.
-  if ((int64_t)num_kv_heads * page_size > INT32_MAX / head_dim)
-    return fail(MVR_E_UNSUPPORTED, "pages of 2^31 elements or more");
-  if (!key_pool || !value_pool) return fail(MVR_E_INVALID_ARGUMENT, "null pool pointer");
-  if (((uintptr_t)key_pool | (uintptr_t)value_pool) % es_of(dtype))
-    return fail(MVR_E_INVALID_ARGUMENT, "pools must be aligned to their elements");
-  return MVR_OK;
-}
 
 static int check_compact(const mvr_compact_drafts_args* a) {
   if (!a) return fail(MVR_E_INVALID_ARGUMENT, "args is null");
