@@ -66,7 +66,7 @@ typedef struct mvr_score_rules {
    dimensions (multiples of 32 up to 256), page sizes (any; nothing is repacked) and
    hints.  Scores, softmax state and sums are held in 32 bits.  F16 probabilities
    enter the product with V with 20 bits; calls of many rows round them to F16, and
-   the sum is then that of the rounded ones (the log-sum-exp too).  Differences to
+   the sum that divides them is then of the rounded ones.  Differences to
    mvr_paged_attention:
      - a request may have q_len 0: nothing is computed for it, so total_q, where
        given, lies in [0, num_seqs * max_q_len];
@@ -129,9 +129,9 @@ int mvr_attention_weights_validate(const mvr_paged_attention_args* args, const m
 /* ---- Which tokens stay ------------------------------------------------------ */
 
 /* Every layer and KV head of a request chooses its own keep_lens[b] tokens: those
-   whose position is below `first` or among the last `recent` ones before all others,
-   then by descending weight (NaN counts as -infinity), and at equal weights the
-   lower slot.  Tokens that stay and lie below the new length stay where they are; the
+   whose position is below `first` or among the last `recent` ones before all others
+   (where they are too many, those in the lower slots), the others by descending weight
+   (NaN counts as -infinity), at equal weights those in the lower slots.  Tokens that stay and lie below the new length stay where they are; the
    others move into the slots there that become free, both in ascending order, which
    is as few rows as can be moved, and in any order of execution the same.
    positions holds the position of each token in slots below kept_lens (what an

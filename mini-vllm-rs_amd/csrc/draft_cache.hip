@@ -4,7 +4,7 @@
 // All three move rows once: they are bound by HBM where a call has many rows,
 // and by the chain of dependent table loads (request, lengths, page, row) where
 // it has few.
-#include "draft_cache.hpp"
+#include "cache_rows.hpp"
 
 #include <math.h>
 
@@ -14,7 +14,6 @@ namespace {
 typedef _Float16 half_t;
 typedef half_t half4 __attribute__((ext_vector_type(4)));
 typedef float float4v __attribute__((ext_vector_type(4)));
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(4))) int32_t const_i32;
 
 constexpr int kThreads = 256;
@@ -293,14 +292,6 @@ __global__ __launch_bounds__(kThreads) void copy_pages_kernel(CopyPagesParams p,
 #pragma unroll
   for (int u = 0; u < kCopyVecs; u++)
     if (v0 + u * kThreads < vecs) to[at[u]] = held[u];
-}
-
-template <typename F>
-hipError_t with_vector(int64_t row_bytes, const void* a, const void* b, F launch) {
-  const int bytes = cache_vector_bytes(row_bytes, a, b), row_vecs = (int)(row_bytes / bytes);
-  if (bytes == 16) return launch(u32x4{}, row_vecs);
-  if (bytes == 4) return launch(uint32_t{}, row_vecs);
-  return launch(uint16_t{}, row_vecs);
 }
 
 } // namespace

@@ -1,0 +1,637 @@
+// C ABI of the calls on scores: argument checks, planning, dispatch.
+// Declared in include/mvr_score.h.
+#include "mvr_score.h"
+
+#include <hip/hip_runtime.h>
+
+#include <math.h>
+
+#include <algorithm>
+#include <memory>
+#include <new>
+#include <vector>
+
+#include "api_common.hpp"
+#include "paged_attention_kernels.hpp" // kChunkTokens
+#include "paged_prefill.hpp"           // page_divider
+#include "score_attention.hpp"
+
+namespace {
+
+using namespace mvr::api;
+
+constexpr double kLog2e = 1.4426950408889634;
+
+float scale_of(const mvr_paged_attention_args* a) {
+  return a->scale > 0.f ? a->scale : (float)(1.0 / sqrt((double)a->head_dim));
+}
+
+// ---------------------------------------------------------------------------
+// Attention with bent and masked scores
+// ---------------------------------------------------------------------------
+
+int check_rules(const mvr_paged_attention_args* a, const mvr_score_rules* r) {
+  if (!r) return fail(MVR_E_INVALID_ARGUMENT, "rules is null");
+  if (!(r->cap >= 0.f) || !isfinite(r->cap)) return fail(MVR_E_INVALID_ARGUMENT, "cap must be finite and >= 0");
+  if (r->cap > 0.f && (r->cap > 1e30f || !(scale_of(a) / r->cap < 1e30f)))
+    return fail(MVR_E_UNSUPPORTED, "cap %g is out of range for scores in 32 bits", r->cap);
+  if (r->window < 0) return fail(MVR_E_INVALID_ARGUMENT, "window must not be negative");
+  if (((uintptr_t)r->slopes | (uintptr_t)r->first_keys | (uintptr_t)r->prefix_lens | (uintptr_t)r->lse) % 4)
+    return fail(MVR_E_INVALID_ARGUMENT, "slopes, first_keys, prefix_lens and lse must be 4-byte aligned");
+  if (r->lse && r->lse_stride_head < a->total_q)
+    return fail(MVR_E_INVALID_ARGUMENT, "lse_stride_head %lld is smaller than total_q %d", (long long)r->lse_stride_head,
+                a->total_q);
+  return MVR_OK;
+}
+
+// The checks that attention and weights share.
+int check_scored(const mvr_paged_attention_args* a, const mvr_score_rules* r) {
+  if (!a) return fail(MVR_E_INVALID_ARGUMENT, "args is null");
+  mvr_paged_attention_args b = *a;
+  b.total_q = 0; // empty requests make its lower bound 0
+  int rc = check_attention_scalars(&b);
+  if (rc != MVR_OK) return rc;
+  if (a->total_q < 0 || a->total_q > (int64_t)a->num_seqs * a->max_q_len)
+    return fail(MVR_E_INVALID_ARGUMENT, "total_q %d is outside [0, num_seqs * max_q_len]", a->total_q);
+  if (a->num_seqs == 1 && !a->cu_q_lens && a->total_q > 0 && a->total_q < a->max_q_len)
+    return fail(MVR_E_INVALID_ARGUMENT, "total_q %d is smaller than max_q_len %d, the q_len of a call without cu_q_lens",
+                a->total_q, a->max_q_len);
+  rc = check_rules(a, r);
+  if (rc != MVR_OK) return rc;
+  if (a->max_seq_len > INT32_MAX - 1024) // (positions of whole key tiles are counted in 32 bits)
+    return fail(MVR_E_UNSUPPORTED, "max_seq_len %d is too close to 2^31", a->max_seq_len);
+  if (a->page_size % mvr::kChunkTokens != 0 && (int64_t)a->page_size * a->head_dim * es_of(a->dtype) > INT32_MAX)
+    return fail(MVR_E_UNSUPPORTED, "pages of 2 GiB per KV head whose size is not a multiple of %d tokens",
+                mvr::kChunkTokens);
+  // The kernels count a page's rows, a head's rows and work items in 32 bits.
+  if (a->num_pages > INT32_MAX || (int64_t)a->num_kv_heads * a->page_size > INT32_MAX)
+    return fail(MVR_E_UNSUPPORTED, "pools of over 2^31 pages, or pages of over 2^31 rows");
+  const int64_t group = a->num_q_heads / a->num_kv_heads;
+  const int64_t pairs = (int64_t)a->num_seqs * a->num_kv_heads + mvr::kScoreXcds - 1;
+  const int64_t tiles = pairs * ((group * a->max_q_len + 15) / 16);
+  if (group * a->max_q_len > INT32_MAX - 1024 || tiles > kMaxThreads / 256 / 2)
+    return fail(MVR_E_UNSUPPORTED, "%d requests of %d tokens are more than one call takes", a->num_seqs, a->max_q_len);
+  return MVR_OK;
+}
+
+mvr::ScoreTables tables_of(const mvr_paged_attention_args* a) {
+  mvr::ScoreTables t{};
+  t.q = a->q;
+  t.q_stride_head = a->q_stride_head;
+  t.q_stride_token = a->q_stride_token;
+  t.key_pool = a->key_pool;
+  t.block_tables = a->block_tables;
+  t.block_table_stride = a->max_pages_per_seq;
+  t.seq_lens = a->seq_lens;
+  t.cu_q_lens = a->cu_q_lens;
+  t.max_seq_len = a->max_seq_len;
+  t.max_q_len = a->max_q_len;
+  t.num_seqs = a->num_seqs;
+  t.num_kv_heads = a->num_kv_heads;
+  t.group_size = a->num_q_heads / a->num_kv_heads;
+  t.page_size = a->page_size;
+  t.last_page = (uint32_t)(a->num_pages - 1);
+  mvr::page_divider(a->page_size, t.page_magic, t.page_magic_shift);
+  return t;
+}
+
+mvr::ScoreRules rules_of(const mvr_paged_attention_args* a, const mvr_score_rules* r) {
+  mvr::ScoreRules k{};
+  const float scale = scale_of(a);
+  k.scale_log2 = (float)(scale * kLog2e);
+  if (r->cap > 0.f) {
+    k.cap_log2 = (float)(r->cap * kLog2e);
+    k.cap_scale = scale / r->cap;
+  }
+  k.window = r->window;
+  k.slopes = r->slopes;
+  k.first_keys = r->first_keys;
+  k.prefix_lens = r->prefix_lens;
+  k.lse = r->lse;
+  k.lse_stride_head = r->lse_stride_head;
+  return k;
+}
+
+int64_t units_of(int64_t tokens) { return (tokens + mvr::kScoreUnitTokens - 1) / mvr::kScoreUnitTokens; }
+
+// Row tiles of 16 and the split of their keys: into as many parts as give every CU the
+// blocks that it holds, where there are fewer row tiles.
+mvr::ScoreAttentionPlan plan_scored(const mvr_paged_attention_args* a, const mvr_score_rules* r, size_t limit) {
+  mvr::ScoreAttentionPlan plan{};
+  const int64_t group = a->num_q_heads / a->num_kv_heads, hkv = a->num_kv_heads;
+  plan.tile_rows = 16;
+  plan.row_tiles = (int)((group * a->max_q_len + plan.tile_rows - 1) / plan.tile_rows);
+  plan.parts = 1;
+  plan.part_units = INT32_MAX;
+  // Units of one row tile's keys at most.
+  int64_t bound = units_of(a->max_seq_len);
+  if (r->window > 0 && !r->prefix_lens)
+    bound = std::min(bound, units_of((int64_t)r->window + (plan.tile_rows + group - 1) / group) + 1);
+  // Row tiles and units of all of them: by the host tables, or as if all requests were alike.
+  int64_t tiles = 0, work = 0;
+  const int32_t *cu = a->cu_q_lens_host, *sl = a->seq_lens_host;
+  for (int s = 0; s < a->num_seqs && cu && sl; s++) {
+    const int64_t q = std::min<int64_t>(std::max<int64_t>(0, (int64_t)cu[s + 1] - cu[s]), a->max_q_len);
+    const int64_t n = (group * q + plan.tile_rows - 1) / plan.tile_rows;
+    tiles += n;
+    work += n * std::min(bound, std::max<int64_t>(units_of(sl[s]), 0));
+  }
+  if (!cu || !sl) {
+    const int64_t tokens = a->sum_seq_lens > 0 ? (a->sum_seq_lens + a->num_seqs - 1) / a->num_seqs : a->max_seq_len;
+    tiles = (int64_t)a->num_seqs * plan.row_tiles;
+    work = tiles * std::min(bound, units_of(tokens));
+  }
+  tiles *= hkv;
+  work *= hkv;
+  const int64_t all_tiles = a->num_seqs * hkv * plan.row_tiles;
+  const int64_t target = 3 * (int64_t)compute_units();
+  if (tiles == 0 || tiles >= target || bound < 2 || limit == 0) return plan;
+  const int64_t part = std::max<int64_t>(1, (work + target - 1) / target);
+  int64_t parts = std::min<int64_t>((bound + part - 1) / part, mvr::kScoreMaxParts);
+  parts = std::min(parts, kMaxThreads / 256 / (all_tiles + mvr::kScoreXcds * plan.row_tiles));
+  auto bytes_of = [&](int64_t n) {
+    return align_up((size_t)all_tiles * n * plan.tile_rows * a->head_dim * sizeof(float), 256) +
+           align_up((size_t)all_tiles * n * plan.tile_rows * 2 * sizeof(float), 256) +
+           align_up((size_t)all_tiles * sizeof(int32_t), 256);
+  };
+  while (parts > 1 && bytes_of(parts) > limit) parts--;
+  if (parts <= 1) return plan;
+  plan.parts = (int)parts;
+  plan.part_units = (int)std::max(part, (bound + parts - 1) / parts);
+  plan.partial_bytes = bytes_of(parts);
+  return plan;
+}
+
+int copy_floats(const float* dev, size_t count, void* stream, std::vector<float>& host) {
+  if (!dev) return MVR_OK;
+  std::vector<int32_t> bits;
+  if (!copy_to_host(reinterpret_cast<const int32_t*>(dev), count, stream, bits)) return copy_failed();
+  host.resize(count);
+  for (size_t i = 0; i < count; i++) host[i] = __builtin_bit_cast(float, bits[i]);
+  return MVR_OK;
+}
+
+const float* floats_or_null(const std::vector<float>& v) { return v.empty() ? nullptr : v.data(); }
+
+// Host copies of the tables that attention and weights read.
+struct HostTables {
+  std::vector<int32_t> bt, sl, cu, first, prefix;
+  std::vector<float> slopes;
+
+  int read(const mvr_paged_attention_args* a, const mvr_score_rules* r) {
+    if (!copy_to_host(a->block_tables, (size_t)a->num_seqs * a->max_pages_per_seq, a->stream, bt) ||
+        !copy_to_host(a->seq_lens, a->num_seqs, a->stream, sl) ||
+        !copy_to_host(a->cu_q_lens, (size_t)a->num_seqs + 1, a->stream, cu) ||
+        !copy_to_host(r->prefix_lens, a->num_seqs, a->stream, prefix))
+      return copy_failed();
+    // (Packed tokens: as many as the starts say, once those are known to be sound.)
+    if (!cu.empty() && check_cu_q_lens(cu.data(), a->num_seqs, a->total_q, a->max_q_len) != MVR_OK)
+      return MVR_E_INVALID_ARGUMENT;
+    const int64_t tokens = cu.empty() ? a->max_q_len : cu[a->num_seqs];
+    if (!copy_to_host(r->first_keys, (size_t)tokens, a->stream, first)) return copy_failed();
+    return copy_floats(r->slopes, a->num_q_heads, a->stream, slopes);
+  }
+};
+
+int validate_scored(const mvr_paged_attention_args* a, const int32_t* block_tables_host, const int32_t* seq_lens_host,
+                    const int32_t* cu_q_lens_host, const int32_t* first_keys_host, const int32_t* prefix_lens_host,
+                    const float* slopes_host) {
+  if (cu_q_lens_host && check_cu_q_lens(cu_q_lens_host, a->num_seqs, a->total_q, a->max_q_len) != MVR_OK)
+    return MVR_E_INVALID_ARGUMENT;
+  for (int h = 0; slopes_host && h < a->num_q_heads; h++)
+    if (!isfinite(slopes_host[h])) return fail(MVR_E_INVALID_ARGUMENT, "slope of head %d is not finite", h);
+  for (int s = 0; s < a->num_seqs; s++) {
+    int64_t q_len = a->num_seqs == 1 ? a->max_q_len : -1, at = 0;
+    if (cu_q_lens_host) {
+      at = cu_q_lens_host[s];
+      q_len = (int64_t)cu_q_lens_host[s + 1] - at;
+    }
+    const int64_t seq_len = seq_lens_host ? seq_lens_host[s] : a->num_seqs == 1 ? a->max_seq_len : -1;
+    if (seq_lens_host) {
+      if (seq_len < 0 || seq_len > a->max_seq_len)
+        return fail(MVR_E_INVALID_ARGUMENT, "request %d has seq_len %lld outside [0, max_seq_len %d]", s,
+                    (long long)seq_len, a->max_seq_len);
+      if (q_len >= 0 && seq_len < q_len)
+        return fail(MVR_E_LENGTH_MISMATCH, "paged KV cache reports sequence length %lld, expected at least %lld",
+                    (long long)seq_len, (long long)q_len);
+    }
+    if (prefix_lens_host && prefix_lens_host[s] < 0)
+      return fail(MVR_E_INVALID_ARGUMENT, "request %d has a prefix of %d tokens", s, prefix_lens_host[s]);
+    if (block_tables_host && seq_len >= 0 && q_len != 0)
+      for (int64_t pi = 0; pi < (seq_len + a->page_size - 1) / a->page_size; pi++) {
+        const int32_t id = block_tables_host[(int64_t)s * a->max_pages_per_seq + pi];
+        if (id < 0 || id >= a->num_pages)
+          return fail(MVR_E_PAGE_ID, "request %d page %lld has id %d outside a pool of %lld pages", s, (long long)pi, id,
+                      (long long)a->num_pages);
+      }
+    if (first_keys_host && q_len > 0)
+      for (int64_t n = at; n < at + q_len; n++)
+        if (first_keys_host[n] < 0)
+          return fail(MVR_E_INVALID_ARGUMENT, "token %lld has first key %d", (long long)n, first_keys_host[n]);
+  }
+  return MVR_OK;
+}
+
+} // namespace
+
+extern "C" {
+
+size_t mvr_paged_attention_scored_workspace_size(const mvr_paged_attention_args* a, const mvr_score_rules* r) {
+  if (check_scored(a, r) != MVR_OK) return 0;
+  return plan_scored(a, r, SIZE_MAX).partial_bytes;
+}
+
+int mvr_paged_attention_scored_validate(const mvr_paged_attention_args* a, const mvr_score_rules* r,
+                                        const int32_t* block_tables_host, const int32_t* seq_lens_host,
+                                        const int32_t* cu_q_lens_host, const int32_t* first_keys_host,
+                                        const int32_t* prefix_lens_host, const float* slopes_host) {
+  clear_error();
+  const int rc = check_scored(a, r);
+  if (rc != MVR_OK) return rc;
+  return validate_scored(a, block_tables_host, seq_lens_host, cu_q_lens_host, first_keys_host, prefix_lens_host,
+                         slopes_host);
+}
+
+int mvr_paged_attention_scored(const mvr_paged_attention_args* a, const mvr_score_rules* r) {
+  Range range("attn"); // trace.rs:64
+  clear_error();
+  int rc = check_scored(a, r);
+  if (rc != MVR_OK) return rc;
+  if (checked()) {
+    rc = run_checked([&] {
+      HostTables h;
+      const int read = h.read(a, r);
+      if (read != MVR_OK) return read;
+      return validate_scored(a, data_or_null(h.bt), data_or_null(h.sl), data_or_null(h.cu), data_or_null(h.first),
+                             data_or_null(h.prefix), floats_or_null(h.slopes));
+    });
+    if (rc != MVR_OK) return rc;
+  }
+  if (a->workspace && ((uintptr_t)a->workspace & 255u))
+    return fail(MVR_E_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
+  const mvr::ScoreAttentionPlan plan = plan_scored(a, r, a->workspace ? a->workspace_bytes : 0);
+  mvr::ScoreAttentionParams p{};
+  p.t = tables_of(a);
+  p.r = rules_of(a, r);
+  p.value_pool = a->value_pool;
+  p.out = a->out;
+  p.out_stride_head = a->out_stride_head;
+  p.out_stride_token = a->out_stride_token;
+  p.row_tiles = plan.row_tiles;
+  p.parts = plan.parts;
+  p.part_units = plan.part_units;
+  if (plan.parts > 1) {
+    const size_t rows = (size_t)a->num_seqs * a->num_kv_heads * plan.row_tiles * plan.parts * plan.tile_rows;
+    char* at = static_cast<char*>(a->workspace);
+    p.partial_o = reinterpret_cast<float*>(at);
+    at += align_up(rows * a->head_dim * sizeof(float), 256);
+    p.partial_ml = reinterpret_cast<float*>(at);
+    at += align_up(rows * 2 * sizeof(float), 256);
+    p.tile_parts = reinterpret_cast<int32_t*>(at);
+  }
+  Range launch("attn-paged-fused");
+  return launch_status(
+      mvr::launch_score_attention(plan, p, a->dtype, a->head_dim, static_cast<hipStream_t>(a->stream)));
+}
+
+// ---------------------------------------------------------------------------
+// The weight that keys get
+// ---------------------------------------------------------------------------
+
+static int check_weights(const mvr_paged_attention_args* a, const mvr_score_rules* r, const mvr_key_weights* w) {
+  if (!a) return fail(MVR_E_INVALID_ARGUMENT, "args is null");
+  mvr_paged_attention_args b = *a; // (what this call does not use need not be there)
+  b.value_pool = a->key_pool;
+  b.out = const_cast<void*>(a->q);
+  b.out_stride_head = a->q_stride_head;
+  b.out_stride_token = a->q_stride_token;
+  const int rc = check_scored(&b, r);
+  if (rc != MVR_OK) return rc;
+  if (!r->lse) return fail(MVR_E_INVALID_ARGUMENT, "weights need the rows' log-sum-exps");
+  if (!w) return fail(MVR_E_INVALID_ARGUMENT, "weights is null");
+  if (!w->weights) return fail(MVR_E_INVALID_ARGUMENT, "null weights pool pointer");
+  if (((uintptr_t)w->weights | (uintptr_t)w->fresh_from) % 4)
+    return fail(MVR_E_INVALID_ARGUMENT, "the weights pool and fresh_from must be 4-byte aligned");
+  if (!(w->decay >= 0.f) || !isfinite(w->decay)) return fail(MVR_E_INVALID_ARGUMENT, "decay must be finite and >= 0");
+  const int64_t unit = mvr::weights_unit_tokens(es_of(a->dtype), a->head_dim);
+  const int64_t blocks = (a->max_seq_len + 4 * unit - 1) / (4 * unit);
+  if ((int64_t)a->num_seqs * a->num_kv_heads > kMaxThreads / 256 / blocks)
+    return fail(MVR_E_UNSUPPORTED, "%d requests of %d tokens are more than one call takes", a->num_seqs, a->max_seq_len);
+  return MVR_OK;
+}
+
+// Marks a page as written; an error where it was before.
+static int mark_page(uint8_t* written, int32_t id, const char* what) {
+  if (written[id]) return fail(MVR_E_INVALID_ARGUMENT, "page %d %s more than one request or layer", id, what);
+  written[id] = 1;
+  return MVR_OK;
+}
+
+static int validate_weights(const mvr_paged_attention_args* a, const int32_t* block_tables_host,
+                            const int32_t* seq_lens_host, const int32_t* cu_q_lens_host, const int32_t* first_keys_host,
+                            const int32_t* prefix_lens_host, const float* slopes_host, const int32_t* fresh_from_host) {
+  int rc = validate_scored(a, block_tables_host, seq_lens_host, cu_q_lens_host, first_keys_host, prefix_lens_host,
+                           slopes_host);
+  if (rc != MVR_OK) return rc;
+  for (int s = 0; fresh_from_host && s < a->num_seqs; s++)
+    if (fresh_from_host[s] < 0) return fail(MVR_E_INVALID_ARGUMENT, "request %d has fresh_from %d", s, fresh_from_host[s]);
+  if (!block_tables_host || (a->num_seqs > 1 && (!seq_lens_host || !cu_q_lens_host))) return MVR_OK;
+  std::unique_ptr<uint8_t[]> written(new (std::nothrow) uint8_t[(size_t)a->num_pages]());
+  if (!written) return fail(MVR_E_INVALID_ARGUMENT, "out of host memory");
+  for (int s = 0; s < a->num_seqs; s++) {
+    if (cu_q_lens_host && cu_q_lens_host[s + 1] == cu_q_lens_host[s]) continue;
+    const int64_t seq_len = seq_lens_host ? seq_lens_host[s] : a->max_seq_len;
+    for (int64_t pi = 0; pi < (seq_len + a->page_size - 1) / a->page_size && rc == MVR_OK; pi++)
+      rc = mark_page(written.get(), block_tables_host[(int64_t)s * a->max_pages_per_seq + pi],
+                     "holds the weights of");
+    if (rc != MVR_OK) return rc;
+  }
+  return MVR_OK;
+}
+
+int mvr_attention_weights_validate(const mvr_paged_attention_args* a, const mvr_score_rules* r, const mvr_key_weights* w,
+                                   const int32_t* block_tables_host, const int32_t* seq_lens_host,
+                                   const int32_t* cu_q_lens_host, const int32_t* first_keys_host,
+                                   const int32_t* prefix_lens_host, const float* slopes_host,
+                                   const int32_t* fresh_from_host) {
+  clear_error();
+  const int rc = check_weights(a, r, w);
+  if (rc != MVR_OK) return rc;
+  return validate_weights(a, block_tables_host, seq_lens_host, cu_q_lens_host, first_keys_host, prefix_lens_host,
+                          slopes_host, fresh_from_host);
+}
+
+int mvr_attention_weights(const mvr_paged_attention_args* a, const mvr_score_rules* r, const mvr_key_weights* w) {
+  Range range("attn-cache operation=weigh");
+  clear_error();
+  int rc = check_weights(a, r, w);
+  if (rc != MVR_OK) return rc;
+  if (checked()) {
+    rc = run_checked([&] {
+      HostTables h;
+      std::vector<int32_t> fresh;
+      const int read = h.read(a, r);
+      if (read != MVR_OK) return read;
+      if (!copy_to_host(w->fresh_from, a->num_seqs, a->stream, fresh)) return copy_failed();
+      return validate_weights(a, data_or_null(h.bt), data_or_null(h.sl), data_or_null(h.cu), data_or_null(h.first),
+                              data_or_null(h.prefix), floats_or_null(h.slopes), data_or_null(fresh));
+    });
+    if (rc != MVR_OK) return rc;
+  }
+  mvr::ScoreWeightsParams p{};
+  p.t = tables_of(a);
+  p.r = rules_of(a, r);
+  p.weights = w->weights;
+  p.decay = w->decay;
+  p.fresh_from = w->fresh_from;
+  return launch_status(mvr::launch_score_weights(p, a->dtype, a->head_dim, static_cast<hipStream_t>(a->stream)));
+}
+
+// ---------------------------------------------------------------------------
+// Which tokens stay
+// ---------------------------------------------------------------------------
+
+constexpr int64_t kMaxSlots = (int64_t)1 << 40;
+
+// Geometry of a call over the tables of several layers.
+static int check_layers(int32_t num_layers, int32_t num_seqs, int32_t num_kv_heads, int32_t page_size, int64_t num_pages,
+                        int64_t threads_per_row, int32_t max_moves) {
+  if (num_layers < 1) return fail(MVR_E_INVALID_ARGUMENT, "num_layers must be positive");
+  if (num_seqs < 1) return fail(MVR_E_INVALID_ARGUMENT, "forward requires at least one request");
+  if (max_moves < 1) return fail(MVR_E_INVALID_ARGUMENT, "max_moves must be positive");
+  if (num_pages > INT32_MAX || num_pages > kMaxSlots / num_kv_heads / page_size)
+    return fail(MVR_E_UNSUPPORTED, "pools of over 2^31 pages, or 2^40 tokens and heads");
+  if ((int64_t)num_layers * num_seqs > kMaxThreads / threads_per_row / num_kv_heads)
+    return fail(MVR_E_UNSUPPORTED, "more layers, requests and KV heads than one call takes");
+  return MVR_OK;
+}
+
+struct Extent {
+  const void* at;
+  int64_t bytes;
+  bool overlaps(const Extent& o) const {
+    return at && o.at && (uintptr_t)at < (uintptr_t)o.at + o.bytes && (uintptr_t)o.at < (uintptr_t)at + bytes;
+  }
+};
+
+static int check_select(const mvr_select_tokens_args* a) {
+  if (!a) return fail(MVR_E_INVALID_ARGUMENT, "args is null");
+  int rc = check_pool(MVR_DTYPE_F32, a->num_kv_heads, 1, a->page_size, a->num_pages, a->weights, a->positions);
+  if (rc != MVR_OK) return rc;
+  rc = check_layers(a->num_layers, a->num_seqs, a->num_kv_heads, a->page_size, a->num_pages, 1024, a->max_moves);
+  if (rc != MVR_OK) return rc;
+  if (a->max_seq_len < 1) return fail(MVR_E_INVALID_ARGUMENT, "max_seq_len must be positive");
+  if (a->max_seq_len > INT32_MAX - 2048)
+    return fail(MVR_E_UNSUPPORTED, "max_seq_len %d is too close to 2^31", a->max_seq_len);
+  if (a->recent < 0 || a->first < 0) return fail(MVR_E_INVALID_ARGUMENT, "recent and first must not be negative");
+  const int64_t pages_needed = (a->max_seq_len + (int64_t)a->page_size - 1) / a->page_size;
+  if (a->max_pages_per_seq < pages_needed)
+    return fail(MVR_E_PAGES_UNCOVERED, "block table rows of %d pages cannot hold %d tokens of %d-token pages",
+                a->max_pages_per_seq, a->max_seq_len, a->page_size);
+  if (!a->block_tables || !a->seq_lens || !a->keep_lens || !a->moves || !a->num_moves)
+    return fail(MVR_E_INVALID_ARGUMENT, "null table pointer");
+  if ((uintptr_t)a->moves % 8) return fail(MVR_E_INVALID_ARGUMENT, "moves must be 8-byte aligned");
+  // Every block reads the tables while others write.
+  const int64_t rows = (int64_t)a->num_layers * a->num_seqs * a->num_kv_heads;
+  const int64_t slots = a->num_pages * a->num_kv_heads * a->page_size;
+  const Extent written[] = {{a->positions, slots * 4}, {a->moves, rows * a->max_moves * 8}, {a->num_moves, rows * 4},
+                            {a->new_seq_lens, (int64_t)a->num_seqs * 4}};
+  const Extent read[] = {{a->weights, slots * 4},
+                         {a->block_tables, (int64_t)a->num_layers * a->num_seqs * a->max_pages_per_seq * 4},
+                         {a->seq_lens, (int64_t)a->num_seqs * 4},
+                         {a->next_positions, (int64_t)a->num_seqs * 4},
+                         {a->kept_lens, (int64_t)a->num_seqs * 4},
+                         {a->keep_lens, (int64_t)a->num_seqs * 4}};
+  for (const Extent& w : written) {
+    for (const Extent& x : read)
+      if (w.overlaps(x)) return fail(MVR_E_INVALID_ARGUMENT, "a written array overlaps a table or the weights");
+    for (const Extent& x : written)
+      if (&x != &w && w.overlaps(x)) return fail(MVR_E_INVALID_ARGUMENT, "written arrays overlap each other");
+  }
+  return MVR_OK;
+}
+
+int mvr_select_tokens_validate(const mvr_select_tokens_args* a, const int32_t* block_tables_host,
+                               const int32_t* seq_lens_host, const int32_t* next_positions_host,
+                               const int32_t* kept_lens_host, const int32_t* keep_lens_host) {
+  clear_error();
+  int rc = check_select(a);
+  if (rc != MVR_OK) return rc;
+  std::unique_ptr<uint8_t[]> written;
+  if (block_tables_host && seq_lens_host) {
+    written.reset(new (std::nothrow) uint8_t[(size_t)a->num_pages]());
+    if (!written) return fail(MVR_E_INVALID_ARGUMENT, "out of host memory");
+  }
+  for (int s = 0; s < a->num_seqs; s++) {
+    const int64_t n = seq_lens_host ? seq_lens_host[s] : -1;
+    if (seq_lens_host && (n < 0 || n > a->max_seq_len))
+      return fail(MVR_E_INVALID_ARGUMENT, "request %d has seq_len %lld outside [0, max_seq_len %d]", s, (long long)n,
+                  a->max_seq_len);
+    if (n >= 0 && next_positions_host && next_positions_host[s] < n)
+      return fail(MVR_E_LENGTH_MISMATCH, "request %d has next position %d before its %lld tokens", s,
+                  next_positions_host[s], (long long)n);
+    if (kept_lens_host && (kept_lens_host[s] < 0 || (n >= 0 && kept_lens_host[s] > n)))
+      return fail(MVR_E_LENGTH_MISMATCH, "request %d has kept_len %d outside its tokens", s, kept_lens_host[s]);
+    if (keep_lens_host) {
+      const int64_t keep = keep_lens_host[s];
+      if (keep < 0) return fail(MVR_E_INVALID_ARGUMENT, "request %d has keep_len %lld", s, (long long)keep);
+      if (n > keep) {
+        if ((int64_t)a->first + a->recent > keep)
+          return fail(MVR_E_INVALID_ARGUMENT, "request %d keeps %lld tokens, fewer than the first %d and the last %d", s,
+                      (long long)keep, a->first, a->recent);
+        if (std::min(keep, n - keep) > a->max_moves)
+          return fail(MVR_E_INVALID_ARGUMENT, "request %d may need %lld moves, more than max_moves %d", s,
+                      (long long)std::min(keep, n - keep), a->max_moves);
+      }
+    }
+    for (int layer = 0; written && layer < a->num_layers; layer++)
+      for (int64_t pi = 0; pi < (n + a->page_size - 1) / a->page_size; pi++) {
+        const int32_t id = block_tables_host[((int64_t)layer * a->num_seqs + s) * a->max_pages_per_seq + pi];
+        if (id < 0 || id >= a->num_pages)
+          return fail(MVR_E_PAGE_ID, "layer %d request %d page %lld has id %d outside a pool of %lld pages", layer, s,
+                      (long long)pi, id, (long long)a->num_pages);
+        rc = mark_page(written.get(), id, "holds the tokens of");
+        if (rc != MVR_OK) return rc;
+      }
+  }
+  return MVR_OK;
+}
+
+int mvr_select_tokens(const mvr_select_tokens_args* a) {
+  Range range("attn-cache operation=select");
+  clear_error();
+  int rc = check_select(a);
+  if (rc != MVR_OK) return rc;
+  if (checked()) {
+    rc = run_checked([&] {
+      std::vector<int32_t> bt, sl, next, kept, keep;
+      if (!copy_to_host(a->block_tables, (size_t)a->num_layers * a->num_seqs * a->max_pages_per_seq, a->stream, bt) ||
+          !copy_to_host(a->seq_lens, a->num_seqs, a->stream, sl) ||
+          !copy_to_host(a->next_positions, a->num_seqs, a->stream, next) ||
+          !copy_to_host(a->kept_lens, a->num_seqs, a->stream, kept) ||
+          !copy_to_host(a->keep_lens, a->num_seqs, a->stream, keep))
+        return copy_failed();
+      return mvr_select_tokens_validate(a, bt.data(), sl.data(), data_or_null(next), data_or_null(kept), keep.data());
+    });
+    if (rc != MVR_OK) return rc;
+  }
+  mvr::SelectTokensParams p{};
+  p.weights = a->weights;
+  p.positions = a->positions;
+  p.block_tables = a->block_tables;
+  p.block_table_stride = a->max_pages_per_seq;
+  p.seq_lens = a->seq_lens;
+  p.next_positions = a->next_positions;
+  p.kept_lens = a->kept_lens;
+  p.keep_lens = a->keep_lens;
+  p.moves = a->moves;
+  p.num_moves = a->num_moves;
+  p.new_seq_lens = a->new_seq_lens;
+  p.num_pages = a->num_pages;
+  p.num_layers = a->num_layers;
+  p.num_seqs = a->num_seqs;
+  p.num_kv_heads = a->num_kv_heads;
+  p.page_size = a->page_size;
+  p.max_seq_len = a->max_seq_len;
+  p.max_moves = a->max_moves;
+  p.recent = a->recent;
+  p.first = a->first;
+  mvr::page_divider(a->page_size, p.page_magic, p.page_magic_shift);
+  return launch_status(mvr::launch_select_tokens(p, static_cast<hipStream_t>(a->stream)));
+}
+
+// ---------------------------------------------------------------------------
+// Moves of tokens
+// ---------------------------------------------------------------------------
+
+static int check_move(const mvr_move_tokens_args* a) {
+  if (!a) return fail(MVR_E_INVALID_ARGUMENT, "args is null");
+  int rc = check_pool(a->dtype, a->num_kv_heads, a->head_dim, a->page_size, a->num_pages, a->key_pool, a->value_pool);
+  if (rc != MVR_OK) return rc;
+  rc = check_layers(a->num_layers, a->num_seqs, a->num_kv_heads, a->page_size, a->num_pages, 256, a->max_moves);
+  if (rc != MVR_OK) return rc;
+  if (a->max_pages_per_seq < 1) return fail(MVR_E_INVALID_ARGUMENT, "max_pages_per_seq must be positive");
+  if (!a->block_tables || !a->moves || !a->num_moves) return fail(MVR_E_INVALID_ARGUMENT, "null table pointer");
+  if ((uintptr_t)a->moves % 8) return fail(MVR_E_INVALID_ARGUMENT, "moves must be 8-byte aligned");
+  if (((uintptr_t)a->weights | (uintptr_t)a->positions) % 4)
+    return fail(MVR_E_INVALID_ARGUMENT, "weights and positions must be 4-byte aligned");
+  return MVR_OK;
+}
+
+int mvr_move_tokens_validate(const mvr_move_tokens_args* a, const int32_t* block_tables_host, const int32_t* moves_host,
+                             const int32_t* num_moves_host) {
+  clear_error();
+  const int rc = check_move(a);
+  if (rc != MVR_OK) return rc;
+  if (!moves_host || !num_moves_host) return MVR_OK;
+  const int64_t slots = (int64_t)a->max_pages_per_seq * a->page_size;
+  return run_checked([&]() -> int {
+    std::vector<int32_t> used; // slots of one row of moves: targets, then sources among them
+    for (int64_t row = 0; row < (int64_t)a->num_layers * a->num_seqs * a->num_kv_heads; row++) {
+      const int32_t count = num_moves_host[row], *moves = moves_host + row * a->max_moves * 2;
+      if (count < 0 || count > a->max_moves)
+        return fail(MVR_E_INVALID_ARGUMENT, "row %lld has %d moves, outside [0, max_moves %d]", (long long)row, count,
+                    a->max_moves);
+      used.clear();
+      for (int64_t j = 0; j < 2 * (int64_t)count; j++) {
+        const int32_t slot = moves[j];
+        if (slot < 0 || slot >= slots)
+          return fail(MVR_E_INVALID_ARGUMENT, "row %lld moves slot %d, outside its pages", (long long)row, slot);
+        if (block_tables_host) {
+          const int32_t id = block_tables_host[row / a->num_kv_heads * a->max_pages_per_seq + slot / a->page_size];
+          if (id < 0 || id >= a->num_pages)
+            return fail(MVR_E_PAGE_ID, "row %lld page %d has id %d outside a pool of %lld pages", (long long)row,
+                        slot / a->page_size, id, (long long)a->num_pages);
+        }
+        if (j % 2) used.push_back(slot);
+      }
+      std::sort(used.begin(), used.end());
+      for (size_t i = 1; i < used.size(); i++)
+        if (used[i] == used[i - 1])
+          return fail(MVR_E_INVALID_ARGUMENT, "row %lld moves to slot %d twice", (long long)row, used[i]);
+      for (int32_t j = 0; j < count; j++)
+        if (std::binary_search(used.begin(), used.end(), moves[2 * (int64_t)j]))
+          return fail(MVR_E_INVALID_ARGUMENT, "row %lld moves both to and from slot %d", (long long)row,
+                      moves[2 * (int64_t)j]);
+    }
+    return MVR_OK;
+  });
+}
+
+int mvr_move_tokens(const mvr_move_tokens_args* a) {
+  Range range("attn-cache operation=move");
+  clear_error();
+  int rc = check_move(a);
+  if (rc != MVR_OK) return rc;
+  if (checked()) {
+    rc = run_checked([&] {
+      std::vector<int32_t> bt, moves, counts;
+      const size_t rows = (size_t)a->num_layers * a->num_seqs * a->num_kv_heads;
+      if (!copy_to_host(a->block_tables, (size_t)a->num_layers * a->num_seqs * a->max_pages_per_seq, a->stream, bt) ||
+          !copy_to_host(a->moves, rows * a->max_moves * 2, a->stream, moves) ||
+          !copy_to_host(a->num_moves, rows, a->stream, counts))
+        return copy_failed();
+      return mvr_move_tokens_validate(a, bt.data(), moves.data(), counts.data());
+    });
+    if (rc != MVR_OK) return rc;
+  }
+  mvr::MoveTokensParams p{};
+  p.key_pool = a->key_pool;
+  p.value_pool = a->value_pool;
+  p.weights = a->weights;
+  p.positions = a->positions;
+  p.block_tables = a->block_tables;
+  p.block_table_stride = a->max_pages_per_seq;
+  p.moves = a->moves;
+  p.num_moves = a->num_moves;
+  p.num_pages = a->num_pages;
+  p.num_layers = a->num_layers;
+  p.num_seqs = a->num_seqs;
+  p.num_kv_heads = a->num_kv_heads;
+  p.page_size = a->page_size;
+  p.max_moves = a->max_moves;
+  return launch_status(
+      mvr::launch_move_tokens(p, (int64_t)a->head_dim * es_of(a->dtype), static_cast<hipStream_t>(a->stream)));
+}
+
+} // extern "C"

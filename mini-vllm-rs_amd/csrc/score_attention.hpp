@@ -1,0 +1,124 @@
+// Internal launch interface of the kernels of mvr_score.h (score_attention.hip,
+// score_weights.hip, score_evict.hip).  Not part of the public ABI.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace mvr {
+
+// Keys are split between parts in units of 64 tokens.
+constexpr int kScoreUnitTokens = 64;
+// Parts of one row tile, at most.
+constexpr int kScoreMaxParts = 64;
+constexpr int kScoreXcds = 8;
+
+// Where queries, keys and lengths are.
+struct ScoreTables {
+  const void* q;
+  int64_t q_stride_head, q_stride_token;
+  const void* key_pool;
+  const int32_t* block_tables;
+  int32_t block_table_stride;
+  const int32_t* seq_lens;  // may be null: max_seq_len
+  const int32_t* cu_q_lens; // may be null: max_q_len
+  int32_t max_seq_len, max_q_len;
+  int32_t num_seqs, num_kv_heads, group_size, page_size;
+  uint32_t last_page;  // num_pages - 1
+  uint64_t page_magic; // page of token t = t * page_magic >> page_magic_shift (page_divider)
+  int32_t page_magic_shift;
+};
+
+struct ScoreRules {
+  float scale_log2; // scale * log2(e)
+  float cap_log2;   // cap * log2(e); 0: none
+  float cap_scale;  // scale / cap
+  int32_t window;   // 0: none
+  const float* slopes;
+  const int32_t* first_keys;
+  const int32_t* prefix_lens;
+  float* lse;
+  int64_t lse_stride_head;
+};
+
+// Attention.  A row tile holds tile_rows rows rho = i * group_size + r of one
+// (request, KV head): i the query token, r the query head within its group.  Its
+// keys, from the first that any of its rows sees to the last, are split into parts of
+// at least part_units units, `parts` at most.
+struct ScoreAttentionParams {
+  ScoreTables t;
+  ScoreRules r;
+  const void* value_pool;
+  void* out;
+  int64_t out_stride_head, out_stride_token;
+  int32_t row_tiles; // of the longest request, per (request, KV head)
+  int32_t parts, part_units;
+  float* partial_o;    // [pair][row tile][part][tile_rows][head_dim]
+  float* partial_ml;   // [pair][row tile][part][tile_rows][2]: maximum (log2 units), sum
+  int32_t* tile_parts; // [pair][row tile]: parts that it was split into
+};
+
+struct ScoreAttentionPlan {
+  int tile_rows;
+  int row_tiles;
+  int parts, part_units;
+  size_t partial_bytes; // 0: not split
+};
+
+hipError_t launch_score_attention(const ScoreAttentionPlan& plan, const ScoreAttentionParams& params, int dtype,
+                                  int head_dim, hipStream_t stream);
+
+// Weights of keys.
+struct ScoreWeightsParams {
+  ScoreTables t;
+  ScoreRules r;
+  float* weights;
+  float decay;
+  const int32_t* fresh_from; // may be null: seq_len - q_len
+};
+
+// Keys of one wavefront: as many as 64 registers hold the rows of (64 at most).
+constexpr int weights_unit_tokens(int elem_bytes, int head_dim) {
+  return head_dim * elem_bytes <= 256 ? 64 : head_dim * elem_bytes <= 512 ? 32 : 16;
+}
+
+hipError_t launch_score_weights(const ScoreWeightsParams& params, int dtype, int head_dim, hipStream_t stream);
+
+// Which tokens stay.
+struct SelectTokensParams {
+  const float* weights;
+  int32_t* positions;
+  const int32_t* block_tables; // [num_layers][num_seqs][block_table_stride]
+  int32_t block_table_stride;
+  const int32_t* seq_lens;
+  const int32_t* next_positions; // may be null: seq_lens
+  const int32_t* kept_lens;      // may be null: 0
+  const int32_t* keep_lens;
+  int32_t* moves;
+  int32_t* num_moves;
+  int32_t* new_seq_lens; // may be null
+  int64_t num_pages;
+  int32_t num_layers, num_seqs, num_kv_heads, page_size, max_seq_len, max_moves, recent, first;
+  uint64_t page_magic;
+  int32_t page_magic_shift;
+};
+
+hipError_t launch_select_tokens(const SelectTokensParams& params, hipStream_t stream);
+
+// Moves.
+struct MoveTokensParams {
+  void* key_pool;
+  void* value_pool;
+  float* weights;     // may be null
+  int32_t* positions; // may be null
+  const int32_t* block_tables;
+  int32_t block_table_stride;
+  const int32_t* moves;
+  const int32_t* num_moves;
+  int64_t num_pages;
+  int32_t num_layers, num_seqs, num_kv_heads, page_size, max_moves;
+};
+
+hipError_t launch_move_tokens(const MoveTokensParams& params, int64_t row_bytes, hipStream_t stream);
+
+} // namespace mvr

@@ -177,8 +177,8 @@ def _pools(key_pool, value_pool):
 
 
 class Call:
-    """One call of the library, its argument block (`args`, and `extra` where the entry point takes a second one) made
-    and its tensors kept.  Calling it launches on `stream`, or on the stream that is current then.
+    """One call of the library, its argument block (`args`, and `extra` where the entry point takes a second one, or a
+    tuple of more) made and its tensors kept.  Calling it launches on `stream`, or on the stream that is current then.
     One thread at a time may call it (another makes a Call of its own), and where there is a `workspace`, its launches must
     not overlap in time, nor may those of Calls that share one.  A graph that recorded a launch reads the argument block's
     tensors and writes the workspace at every replay: keep the Call as long as the graph.
@@ -188,7 +188,8 @@ class Call:
     def __init__(self, name, args, extra, tensors, device, stream, workspace=None, workspace_stream=None, empty=False):
         self._function = getattr(load_library(), name)
         self.args, self.extra, self.workspace = args, extra, workspace
-        self._refs = (ctypes.byref(args),) if extra is None else (ctypes.byref(args), ctypes.byref(extra))
+        extras = extra if isinstance(extra, tuple) else () if extra is None else (extra,)
+        self._refs = tuple(ctypes.byref(block) for block in (args, *extras))
         self._tensors = tuple(t for t in tensors if t is not None)
         if workspace is not None and workspace_stream is None:
             self._tensors += (workspace,)
