@@ -102,6 +102,9 @@ mvr::ScoreRules rules_of(const mvr_paged_attention_args* a, const mvr_score_rule
   if (r->cap > 0.f) {
     k.cap_log2 = (float)(r->cap * kLog2e);
     k.cap_scale = scale / r->cap;
+    const double y = (double)scale / r->cap; // y^2k, k <= 5, has to be a normal number
+    k.cap_poly_limit = y > 2e-4 && y < 2e3 ? (float)(mvr::kTanhPolynomial / y) : -1.f;
+    for (int i = 0; i < 6; i++) k.cap_poly[i] = (float)(mvr::kTanhCoefficients[i] * scale * kLog2e * pow(y, 2 * i));
   }
   k.window = r->window;
   k.slopes = r->slopes;
@@ -314,7 +317,7 @@ static int check_weights(const mvr_paged_attention_args* a, const mvr_score_rule
     return fail(MVR_E_INVALID_ARGUMENT, "the weights pool and fresh_from must be 4-byte aligned");
   if (!(w->decay >= 0.f) || !isfinite(w->decay)) return fail(MVR_E_INVALID_ARGUMENT, "decay must be finite and >= 0");
   const int64_t unit = mvr::weights_unit_tokens(es_of(a->dtype), a->head_dim);
-  const int64_t blocks = (a->max_seq_len + 4 * unit - 1) / (4 * unit);
+  const int64_t blocks = (a->max_seq_len + unit - 1) / unit;
   if ((int64_t)a->num_seqs * a->num_kv_heads > kMaxThreads / 256 / blocks)
     return fail(MVR_E_UNSUPPORTED, "%d requests of %d tokens are more than one call takes", a->num_seqs, a->max_seq_len);
   return MVR_OK;
@@ -384,7 +387,9 @@ int mvr_attention_weights(const mvr_paged_attention_args* a, const mvr_score_rul
   p.weights = w->weights;
   p.decay = w->decay;
   p.fresh_from = w->fresh_from;
-  return launch_status(mvr::launch_score_weights(p, a->dtype, a->head_dim, static_cast<hipStream_t>(a->stream)));
+  const int64_t rows = (int64_t)(a->num_q_heads / a->num_kv_heads) * a->max_q_len;
+  const bool split = rows > 64;
+  return launch_status(mvr::launch_score_weights(p, a->dtype, a->head_dim, split, static_cast<hipStream_t>(a->stream)));
 }
 
 // ---------------------------------------------------------------------------
@@ -630,6 +635,7 @@ int mvr_move_tokens(const mvr_move_tokens_args* a) {
   p.num_kv_heads = a->num_kv_heads;
   p.page_size = a->page_size;
   p.max_moves = a->max_moves;
+  mvr::page_divider(a->page_size, p.page_magic, p.page_magic_shift);
   return launch_status(
       mvr::launch_move_tokens(p, (int64_t)a->head_dim * es_of(a->dtype), static_cast<hipStream_t>(a->stream)));
 }

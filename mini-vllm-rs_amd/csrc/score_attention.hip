@@ -89,7 +89,7 @@ __global__ __launch_bounds__(kWaveSize* kWaves, (stream_blocks_per_cu(sizeof(typ
   const ScoreRow row = score_row(t, p.r, s, b, head, i);
   KeyRange range = no_rows();
   if (valid) add_row(range, row);
-  range = wave_range(range);
+  range = row_tile_range(range);
 
   // The part's chunks, and the wavefront's.
   const int units = units_of(range), unit0 = range.begin / kScoreUnitTokens;
@@ -272,7 +272,7 @@ __global__ __launch_bounds__(kWaveSize* kWaves, (stream_blocks_per_cu(sizeof(typ
     }
     load_v(k + C, vbuf);
     const int first = k * kChunkTokens + 4 * g; // key of element e: first + 16 (e / 4) + e % 4
-    to_scores(p.r, row, x, [&](int e) { return first + 16 * (e >> 2) + (e & 3); });
+    to_scores(p.r, row, 0.f, x, [&](int e) { return first + 16 * (e >> 2) + (e & 3); });
     if constexpr (kMasked) {
 #pragma unroll
       for (int e = 0; e < 4 * C; e++) x[e] = sees(mine, first + 16 * (e >> 2) + (e & 3)) ? x[e] : -INFINITY;

@@ -29,10 +29,23 @@ struct ScoreTables {
   int32_t page_magic_shift;
 };
 
+// tanh(y) = y * sum_k c_k y^2k for |y| <= kTanhPolynomial.
+constexpr float kTanhPolynomial = 0.625f;
+constexpr float kTanhCoefficients[6] = {1.0f,
+                                        -0.3333328068256378f,
+                                        0.13331441581249237f,
+                                        -0.05373971164226532f,
+                                        0.020639080554246902f,
+                                        -0.005704979412257671f};
+
 struct ScoreRules {
   float scale_log2; // scale * log2(e)
   float cap_log2;   // cap * log2(e); 0: none
   float cap_scale;  // scale / cap
+  // Of a dot product s up to cap_poly_limit in size, the capped score in log2 units is
+  // s * sum_k cap_poly[k] s^2k.  (Limit below 0: the coefficients leave the range of 32
+  // bits.)
+  float cap_poly_limit, cap_poly[6];
   int32_t window;   // 0: none
   const float* slopes;
   const int32_t* first_keys;
@@ -82,7 +95,8 @@ constexpr int weights_unit_tokens(int elem_bytes, int head_dim) {
   return head_dim * elem_bytes <= 256 ? 64 : head_dim * elem_bytes <= 512 ? 32 : 16;
 }
 
-hipError_t launch_score_weights(const ScoreWeightsParams& params, int dtype, int head_dim, hipStream_t stream);
+// split: the rows are shared out among a block's wavefronts, not the keys.
+hipError_t launch_score_weights(const ScoreWeightsParams& params, int dtype, int head_dim, bool split, hipStream_t stream);
 
 // Which tokens stay.
 struct SelectTokensParams {
@@ -117,6 +131,8 @@ struct MoveTokensParams {
   const int32_t* num_moves;
   int64_t num_pages;
   int32_t num_layers, num_seqs, num_kv_heads, page_size, max_moves;
+  uint64_t page_magic;
+  int32_t page_magic_shift;
 };
 
 hipError_t launch_move_tokens(const MoveTokensParams& params, int64_t row_bytes, hipStream_t stream);

@@ -7,6 +7,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 namespace mvr {
 namespace {
 
@@ -58,16 +60,24 @@ __device__ __forceinline__ bool sees(const ScoreRow& row, int key) {
   return (uint32_t)(key - row.lo) < (uint32_t)row.width;
 }
 
-// Smallest, largest over the 64 lanes.
-__device__ __forceinline__ int wave_min(int v) {
-#pragma unroll
-  for (int x = 32; x; x >>= 1) v = min(v, __shfl_xor(v, x));
-  return __builtin_amdgcn_readfirstlane(v);
+// Over the 16 lanes of a DPP row, by rotations: every lane gets the result.
+template <typename Op>
+__device__ __forceinline__ int row16_reduce(int v, Op op) {
+  v = op(v, __builtin_amdgcn_update_dpp(v, v, 0x128, 0xf, 0xf, false)); // row_ror:8
+  v = op(v, __builtin_amdgcn_update_dpp(v, v, 0x124, 0xf, 0xf, false));
+  v = op(v, __builtin_amdgcn_update_dpp(v, v, 0x122, 0xf, 0xf, false));
+  return op(v, __builtin_amdgcn_update_dpp(v, v, 0x121, 0xf, 0xf, false));
 }
-__device__ __forceinline__ int wave_max(int v) {
-#pragma unroll
-  for (int x = 32; x; x >>= 1) v = max(v, __shfl_xor(v, x));
-  return __builtin_amdgcn_readfirstlane(v);
+
+__device__ __forceinline__ float row16_sum(float v) {
+  auto turned = [](float x, auto by) {
+    const int bits = __float_as_int(x);
+    return __int_as_float(__builtin_amdgcn_update_dpp(bits, bits, decltype(by)::value, 0xf, 0xf, false));
+  };
+  v += turned(v, std::integral_constant<int, 0x128>()); // row_ror:8
+  v += turned(v, std::integral_constant<int, 0x124>());
+  v += turned(v, std::integral_constant<int, 0x122>());
+  return v + turned(v, std::integral_constant<int, 0x121>());
 }
 
 // The keys that any row of a wavefront sees, [begin, end), and those that all do,
@@ -87,25 +97,27 @@ __device__ __forceinline__ void add_row(KeyRange& k, const ScoreRow& row) {
 
 __device__ __forceinline__ KeyRange no_rows() { return {INT32_MAX, 0, 0, INT32_MAX}; }
 
-// Over the wavefront's lanes; nothing seen: begin = end = 0.
-__device__ __forceinline__ KeyRange wave_range(const KeyRange& mine) {
-  KeyRange k = {wave_min(mine.begin), wave_max(mine.end), wave_max(mine.all_begin), wave_min(mine.all_end)};
+// Over the query rows of 16 lanes (the other groups of 16 hold the same ones); nothing
+// seen: begin = end = 0.
+__device__ __forceinline__ KeyRange row_tile_range(const KeyRange& mine) {
+  auto least = [](int a, int b) { return min(a, b); };
+  auto most = [](int a, int b) { return max(a, b); };
+  auto first = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  KeyRange k = {first(row16_reduce(mine.begin, least)), first(row16_reduce(mine.end, most)),
+                first(row16_reduce(mine.all_begin, most)), first(row16_reduce(mine.all_end, least))};
   if (k.end == 0) k.begin = 0;
   return k;
 }
 
-// tanh(y) / y for |y| <= kTanhPolynomial as a polynomial in u = y^2 that is off by
-// 4.4e-9 of it at most (least squares, reweighted towards the largest error); in 32
-// bits y * P(u) is within 1.0e-7.  A form with exponentials takes an e^x and a
-// reciprocal, 16 cycles each, and loses the small values to cancellation.
-constexpr float kTanhPolynomial = 0.625f;
+// tanh(y) / y for |y| <= kTanhPolynomial is a polynomial in y^2 (kTanhCoefficients) but
+// for 4.4e-9 of it (least squares, reweighted towards the largest error); y times it, in
+// 32 bits, is within 1.0e-7.  A form with exponentials takes an e^x and a reciprocal, 16
+// cycles each, and loses the small values to cancellation.
 __device__ __forceinline__ float tanh_over(float u) {
-  float p = -0.005704979412257671f;
-  p = fmaf(p, u, 0.020639080554246902f);
-  p = fmaf(p, u, -0.05373971164226532f);
-  p = fmaf(p, u, 0.13331441581249237f);
-  p = fmaf(p, u, -0.3333328068256378f);
-  return fmaf(p, u, 1.0f);
+  float p = kTanhCoefficients[5];
+#pragma unroll
+  for (int k = 4; k >= 0; k--) p = fmaf(p, u, kTanhCoefficients[k]);
+  return p;
 }
 
 // tanh(y), any y: past the polynomial's range 1 - 2 / (e^2|y| + 1), there 0.55 at
@@ -117,30 +129,34 @@ __device__ __forceinline__ float tanh_any(float y) {
   return a <= kTanhPolynomial ? y * tanh_over(y * y) : big; // (a NaN: big, which is one)
 }
 
-// N dot products q . k of one row to scores in log2 units, x = score * log2(e);
-// key(e): the key of element e.  What the rules lack is left out by branches that all
-// lanes take alike.
+// N dot products q . k of one row to scores in log2 units less `minus`,
+// x = score * log2(e) - minus; key(e): the key of element e.  What the rules lack is left
+// out by branches that all lanes take alike.  A cap costs 7 operations a score while all
+// of them lie in the polynomial's range (those of a model that caps them mostly do): its
+// coefficients hold scale, cap and log2(e).
 template <int N, typename Key>
-__device__ __forceinline__ void to_scores(const ScoreRules& r, const ScoreRow& row, float (&x)[N], Key key) {
+__device__ __forceinline__ void to_scores(const ScoreRules& r, const ScoreRow& row, float minus, float (&x)[N], Key key) {
   if (r.cap_log2 > 0.f) {
     float top = 0.f;
 #pragma unroll
     for (int e = 0; e < N; e++) top = fmaxf(top, fabsf(x[e]));
-    // (Most scores of a model that caps them are far below the cap.  A NaN among
-    // finite scores takes either way as a NaN.)
-    if (__any(!(top * r.cap_scale <= kTanhPolynomial))) {
+    // (A NaN among scores in range takes either way as a NaN.)
+    if (__any(!(top <= r.cap_poly_limit))) {
 #pragma unroll
-      for (int e = 0; e < N; e++) x[e] = r.cap_log2 * tanh_any(x[e] * r.cap_scale);
+      for (int e = 0; e < N; e++) x[e] = fmaf(r.cap_log2, tanh_any(x[e] * r.cap_scale), -minus);
     } else {
 #pragma unroll
       for (int e = 0; e < N; e++) {
-        const float y = x[e] * r.cap_scale;
-        x[e] = x[e] * r.scale_log2 * tanh_over(y * y);
+        const float u = x[e] * x[e];
+        float p = r.cap_poly[5];
+#pragma unroll
+        for (int k = 4; k >= 0; k--) p = fmaf(p, u, r.cap_poly[k]);
+        x[e] = fmaf(x[e], p, -minus);
       }
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < N; e++) x[e] *= r.scale_log2;
+    for (int e = 0; e < N; e++) x[e] = fmaf(x[e], r.scale_log2, -minus);
   }
   if (r.slopes) {
 #pragma unroll

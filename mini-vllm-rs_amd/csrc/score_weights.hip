@@ -19,34 +19,67 @@ namespace {
 
 constexpr int kWaves = 4; // wavefronts per block
 
-template <typename Tr, int D>
-__global__ __launch_bounds__(kWaveSize* kWaves) void score_weights_kernel(ScoreWeightsParams p, int blocks_per_pair) {
+// Wavefronts per SIMD.  (F32 rows from 512 bytes on hold their queries twice, with the next
+// tile's, in up to 128 registers.)
+template <typename T, int D>
+constexpr int weights_waves() {
+  return sizeof(T) == 4 && D >= 128 ? 2 : 3;
+}
+
+// SPLIT: the block's wavefronts hold the same keys and take every fourth row tile each
+// (their sums add up in LDS); else they hold keys of their own.
+template <typename Tr, int D, bool SPLIT>
+__global__ __launch_bounds__(kWaveSize* kWaves, (weights_waves<typename Tr::elem, D>())) void score_weights_kernel(
+    ScoreWeightsParams p, int blocks_per_pair) {
   typedef typename Tr::elem T;
   constexpr int kUnit = weights_unit_tokens(sizeof(T), D), kChunks = kUnit / kChunkTokens;
+  constexpr int kRowStep = SPLIT ? 16 * kWaves : 16;
   const ScoreTables& t = p.t;
   const int l = lane_id(), g = l >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
-  const int pair = (int)(blockIdx.x / (unsigned)blocks_per_pair);
-  const int unit = (int)(blockIdx.x - (unsigned)pair * blocks_per_pair) * kWaves + wave;
+  const int pair = (int)(blockIdx.x / (unsigned)blocks_per_pair), block = (int)(blockIdx.x - (unsigned)pair * blocks_per_pair);
+  const int key0 = (SPLIT ? block : block * kWaves + wave) * kUnit;
   const int b = pair / t.num_kv_heads, h = pair - b * t.num_kv_heads;
   const ScoreSeq s = load_score_seq(t, b);
-  const int key0 = unit * kUnit;
-  if (key0 >= s.seq_len) return;
+  if (key0 >= s.seq_len) return; // (SPLIT: the whole block)
   const int rows = t.group_size * s.q_len;
 
   // Lane l holds the page entry of key key0 + l (lanes past the last key that key's).
   const int my_key = min(key0 + l % kUnit, s.seq_len - 1);
   auto page_div = [&](int x) { return (int)(((uint64_t)(uint32_t)x * t.page_magic) >> t.page_magic_shift); };
   const uint32_t entry = (uint32_t)t.block_tables[(int64_t)b * t.block_table_stride + page_div(my_key)];
+
+  // The next row tile's queries and rows are on their way while one is computed.
+  struct Rows {
+    typename Tr::qreg_t q[Tr::kQRegs];
+    ScoreRow row;
+    float lse;
+    bool valid;
+  };
+  int token = (16 * (SPLIT ? wave : 0) + (l & 15)) / t.group_size; // the lane's row of the next tile: token and head
+  int in_group = 16 * (SPLIT ? wave : 0) + (l & 15) - token * t.group_size;
+  const int token_step = kRowStep / t.group_size, group_step = kRowStep - token_step * t.group_size;
+  auto load_rows = [&](Rows& r) {
+    r.valid = token < s.q_len;
+    const int i = r.valid ? token : 0, head = h * t.group_size + (r.valid ? in_group : 0);
+    token += token_step;
+    in_group += group_step;
+    if (in_group >= t.group_size) {
+      in_group -= t.group_size;
+      token++;
+    }
+    r.lse = p.r.lse[(int64_t)head * p.r.lse_stride_head + s.q_start + i];
+    r.row = score_row(t, p.r, s, b, head, i);
+    Tr::load_q(static_cast<const T*>(t.q) + (int64_t)head * t.q_stride_head + (int64_t)(s.q_start + i) * t.q_stride_token,
+               r.valid, g, r.q);
+  };
+  Rows next;
+  int rho0 = SPLIT ? 16 * wave : 0;
+  if (rho0 < rows) load_rows(next);
+
   const uint32_t page = min(entry, t.last_page);
   const uint32_t in_page = (uint32_t)(my_key - page_div(my_key) * t.page_size);
   const uint64_t slot = ((uint64_t)page * t.num_kv_heads + h) * (uint32_t)t.page_size + in_page; // of all pools' slots
-  // What the key had, and whether it is the lane's to write.
-  const bool writes = l < kUnit && key0 + l < s.seq_len && entry <= t.last_page;
-  const int fresh = p.fresh_from ? ((const const_i32*)p.fresh_from)[b] : s.seq_len - s.q_len;
-  const bool keeps = writes && my_key < fresh && p.decay != 0.f;
-  const float had = keeps ? p.weights[slot] : 0.f;
-
   typename Tr::kreg_t k[kChunks][Tr::kLoads];
 #pragma unroll
   for (int c = 0; c < kChunks; c++) {
@@ -55,92 +88,92 @@ __global__ __launch_bounds__(kWaveSize* kWaves) void score_weights_kernel(ScoreW
     const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)(uint32_t)(slot >> 32));
     Tr::load_k_row(static_cast<const T*>(t.key_pool) + (((uint64_t)hi << 32) | lo) * D, l, k[c]);
   }
+  // What the key had, and whether it is the lane's to write.
+  const bool writes = l < kUnit && key0 + l < s.seq_len && entry <= t.last_page && (!SPLIT || wave == 0);
+  const int fresh = p.fresh_from ? ((const const_i32*)p.fresh_from)[b] : s.seq_len - s.q_len;
+  const bool keeps = writes && my_key < fresh && p.decay != 0.f;
+  const float had = keeps ? p.weights[slot] : 0.f;
 
-  float acc[kChunks][4];
+  float acc[4 * kChunks];
 #pragma unroll
-  for (int c = 0; c < kChunks; c++)
-#pragma unroll
-    for (int e = 0; e < 4; e++) acc[c][e] = 0.f;
+  for (int v = 0; v < 4 * kChunks; v++) acc[v] = 0.f;
 
-  for (int rho0 = 0; rho0 < rows; rho0 += 16) {
-    const int rho = rho0 + (l & 15);
-    const bool valid = rho < rows;
-    const int i = valid ? rho / t.group_size : 0, head = h * t.group_size + (valid ? rho - i * t.group_size : 0);
-    ScoreRow row = score_row(t, p.r, s, b, head, i);
-    const float lse = valid ? p.r.lse[(int64_t)head * p.r.lse_stride_head + s.q_start + i] : 0.f;
-    if (!valid || lse == -INFINITY) row.width = 0;
-    const float lse_log2 = lse * 1.4426950408889634f;
+  for (; rho0 < rows; rho0 += kRowStep) {
+    Rows r = next;
+    if (rho0 + kRowStep < rows) load_rows(next);
+    if (!r.valid || r.lse == -INFINITY) r.row.width = 0;
+    const float lse_log2 = r.lse * 1.4426950408889634f;
     KeyRange range = no_rows();
-    add_row(range, row);
-    range = wave_range(range);
+    add_row(range, r.row);
+    range = row_tile_range(range);
     if (range.end <= key0 || range.begin >= key0 + kUnit) continue;
-    typename Tr::qreg_t q[Tr::kQRegs];
-    Tr::load_q(static_cast<const T*>(t.q) + (int64_t)head * t.q_stride_head + (int64_t)(s.q_start + i) * t.q_stride_token,
-               valid, g, q);
     const bool masked = range.all_begin > key0 || range.all_end < key0 + kUnit;
+    float x[4 * kChunks];
 #pragma unroll
     for (int c = 0; c < kChunks; c++) {
-      const float4v sc = Tr::qk(k[c], q);
-      float x[4] = {sc[0], sc[1], sc[2], sc[3]};
-      const int first = key0 + 16 * c + 4 * g;
-      to_scores(p.r, row, x, [&](int e) { return first + e; });
+      const float4v sc = Tr::qk(k[c], r.q);
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        float w = __builtin_amdgcn_exp2f(x[e] - lse_log2);
-        if (masked) w = sees(row, first + e) ? w : 0.f;
-        acc[c][e] += w;
-      }
+      for (int e = 0; e < 4; e++) x[4 * c + e] = sc[e];
     }
+    auto key_of = [&](int e) { return key0 + 4 * g + 16 * (e >> 2) + (e & 3); };
+    to_scores(p.r, r.row, lse_log2, x, key_of);
+    if (masked) {
+#pragma unroll
+      for (int e = 0; e < 4 * kChunks; e++) x[e] = sees(r.row, key_of(e)) ? x[e] : -INFINITY;
+    }
+#pragma unroll
+    for (int e = 0; e < 4 * kChunks; e++) acc[e] += __builtin_amdgcn_exp2f(x[e]);
   }
 
-  // acc[c][e] of lane 16 g + n: key 16 c + 4 g + e, rows n modulo 16.  Four steps, each
-  // of which adds one half of the values to the other lane's half, leave lane 16 g + n
-  // with the sum of value n.
-  float sum[16];
+  // acc[4 c + e] of lane 16 g + n: key 16 c + 4 g + e, rows n modulo 16.  Summed over a
+  // group's lanes, the lane l takes key l's.
+  const int want = 4 * (l >> 4) + (l & 3); // (of group (l & 15) / 4)
+  float mine = 0.f;
 #pragma unroll
-  for (int v = 0; v < 16; v++) sum[v] = v < 4 * kChunks ? acc[v / 4 % kChunks][v % 4] : 0.f;
-#pragma unroll
-  for (int half = 8; half; half >>= 1) {
-    const bool upper = l & half;
-#pragma unroll
-    for (int v = 0; v < half; v++) {
-      const float give = upper ? sum[v] : sum[v + half], keep = upper ? sum[v + half] : sum[v];
-      sum[v] = keep + __shfl_xor(give, half);
-    }
+  for (int v = 0; v < 4 * kChunks; v++) {
+    const float sum = row16_sum(acc[v]);
+    mine = (l & 15) == v ? sum : mine;
   }
-  // Value n = 4 c + e of lane group g is key 16 c + 4 g + e.
-  const int c = l >> 4, in_chunk = l & 15;
-  const float got = __shfl(sum[0], 16 * (in_chunk >> 2) + 4 * c + (in_chunk & 3));
+  float got = __shfl(mine, 16 * ((l & 15) >> 2) + want);
+  if constexpr (SPLIT) {
+    __shared__ float sums[kWaves][kWaveSize];
+    sums[wave][l] = got;
+    __syncthreads();
+    got = ((sums[0][l] + sums[1][l]) + sums[2][l]) + sums[3][l];
+  }
   if (writes) p.weights[slot] = (keeps ? p.decay * had : 0.f) + got;
 }
 
 template <typename Tr, int D>
-hipError_t launch(const ScoreWeightsParams& p, hipStream_t stream) {
+hipError_t launch(const ScoreWeightsParams& p, bool split, hipStream_t stream) {
   constexpr int kUnit = weights_unit_tokens(sizeof(typename Tr::elem), D);
   const int64_t units = ((int64_t)p.t.max_seq_len + kUnit - 1) / kUnit, blocks = (units + kWaves - 1) / kWaves;
   const int64_t pairs = (int64_t)p.t.num_seqs * p.t.num_kv_heads;
-  hipLaunchKernelGGL((score_weights_kernel<Tr, D>), dim3((unsigned)(pairs * blocks)), dim3(kWaveSize * kWaves), 0, stream,
-                     p, (int)blocks);
+  const dim3 block(kWaveSize * kWaves);
+  if (split)
+    hipLaunchKernelGGL((score_weights_kernel<Tr, D, true>), dim3((unsigned)(pairs * units)), block, 0, stream, p, (int)units);
+  else
+    hipLaunchKernelGGL((score_weights_kernel<Tr, D, false>), dim3((unsigned)(pairs * blocks)), block, 0, stream, p, (int)blocks);
   return hipGetLastError();
 }
 
 template <int D>
-hipError_t launch_type(const ScoreWeightsParams& p, int dtype, hipStream_t stream) {
-  return dtype == 1 ? launch<F16Traits<D>, D>(p, stream) : launch<F32Traits<D>, D>(p, stream);
+hipError_t launch_type(const ScoreWeightsParams& p, int dtype, bool split, hipStream_t stream) {
+  return dtype == 1 ? launch<F16Traits<D>, D>(p, split, stream) : launch<F32Traits<D>, D>(p, split, stream);
 }
 
 } // namespace
 
-hipError_t launch_score_weights(const ScoreWeightsParams& params, int dtype, int head_dim, hipStream_t stream) {
+hipError_t launch_score_weights(const ScoreWeightsParams& params, int dtype, int head_dim, bool split, hipStream_t stream) {
   switch (head_dim) {
-  case 32: return launch_type<32>(params, dtype, stream);
-  case 64: return launch_type<64>(params, dtype, stream);
-  case 96: return launch_type<96>(params, dtype, stream);
-  case 128: return launch_type<128>(params, dtype, stream);
-  case 160: return launch_type<160>(params, dtype, stream);
-  case 192: return launch_type<192>(params, dtype, stream);
-  case 224: return launch_type<224>(params, dtype, stream);
-  case 256: return launch_type<256>(params, dtype, stream);
+  case 32: return launch_type<32>(params, dtype, split, stream);
+  case 64: return launch_type<64>(params, dtype, split, stream);
+  case 96: return launch_type<96>(params, dtype, split, stream);
+  case 128: return launch_type<128>(params, dtype, split, stream);
+  case 160: return launch_type<160>(params, dtype, split, stream);
+  case 192: return launch_type<192>(params, dtype, split, stream);
+  case 224: return launch_type<224>(params, dtype, split, stream);
+  case 256: return launch_type<256>(params, dtype, split, stream);
   default: return hipErrorInvalidValue;
   }
 }
