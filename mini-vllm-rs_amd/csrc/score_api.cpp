@@ -101,10 +101,25 @@ mvr::ScoreRules rules_of(const mvr_paged_attention_args* a, const mvr_score_rule
   k.scale_log2 = (float)(scale * kLog2e);
   if (r->cap > 0.f) {
     k.cap_log2 = (float)(r->cap * kLog2e);
-    k.cap_scale = scale / r->cap;
-    const double y = (double)scale / r->cap; // y^2k, k <= 5, has to be a normal number
-    k.cap_poly_limit = y > 2e-4 && y < 2e3 ? (float)(mvr::kTanhPolynomial / y) : -1.f;
-    for (int i = 0; i < 6; i++) k.cap_poly[i] = (float)(mvr::kTanhCoefficients[i] * scale * kLog2e * pow(y, 2 * i));
+    const double y = (double)scale / r->cap; // of a dot product of 1
+    k.cap_exp_scale = (float)(2 * kLog2e * y);
+    // Where y is so small that a coefficient leaves the normal numbers, it and those after
+    // it are left out, and the range ends where they would be 2^-25 of the result.  Where
+    // it is so large that one overflows, there is no range.
+    double limit = mvr::kTanhPolynomial;
+    for (int i = 0; i < 6; i++) {
+      const double c = mvr::kTanhCoefficients[i], folded = c * scale * kLog2e * pow(y, 2 * i);
+      if (fabs(folded) < 1e-37 && i > 0) {
+        limit = std::min(limit, pow(0x1p-25 / fabs(c), 1.0 / (2 * i)));
+        break;
+      }
+      if (!(fabs(folded) < 1e37)) {
+        limit = -1;
+        break;
+      }
+      k.cap_poly[i] = (float)folded;
+    }
+    k.cap_poly_limit = (float)std::min(limit / y, 1e18); // (its square is a number)
   }
   k.window = r->window;
   k.slopes = r->slopes;
@@ -117,52 +132,128 @@ mvr::ScoreRules rules_of(const mvr_paged_attention_args* a, const mvr_score_rule
 
 int64_t units_of(int64_t tokens) { return (tokens + mvr::kScoreUnitTokens - 1) / mvr::kScoreUnitTokens; }
 
-// Row tiles of 16 and the split of their keys: into as many parts as give every CU the
-// blocks that it holds, where there are fewer row tiles.
+// Row tiles of one size, as the planner sees them: by the host tables, or as if all
+// requests were alike.
+struct TileWork {
+  int64_t tiles = 0, units = 0; // row tiles; units of 64 keys over all of them
+  int64_t longest = 0;          // units of one
+
+  TileWork(const mvr_paged_attention_args* a, const mvr_score_rules* r, int tile_rows) {
+    const int64_t group = a->num_q_heads / a->num_kv_heads;
+    int64_t bound = INT64_MAX; // units that a window leaves a row tile
+    if (r->window > 0 && !r->prefix_lens) bound = units_of((int64_t)r->window + (tile_rows + group - 1) / group) + 1;
+    const int32_t *cu = a->cu_q_lens_host, *sl = a->seq_lens_host;
+    auto add = [&](int64_t q, int64_t keys, int64_t requests) {
+      const int64_t n = (group * q + tile_rows - 1) / tile_rows;
+      tiles += requests * n;
+      // (A causal mask leaves the request's queries half of its new tokens on average.)
+      units += requests * n * std::min(bound, units_of(std::max<int64_t>(keys - q / 2, 1)));
+      if (n) longest = std::max(longest, std::min(bound, units_of(keys)));
+    };
+    if (cu && sl) {
+      for (int s = 0; s < a->num_seqs; s++)
+        add(std::min<int64_t>(std::max<int64_t>(0, (int64_t)cu[s + 1] - cu[s]), a->max_q_len),
+            std::min(std::max(sl[s], 0), a->max_seq_len), 1);
+    } else {
+      add(a->max_q_len, a->sum_seq_lens > 0 ? (a->sum_seq_lens + a->num_seqs - 1) / a->num_seqs : a->max_seq_len,
+          a->num_seqs);
+    }
+    tiles *= a->num_kv_heads;
+    units *= a->num_kv_heads;
+  }
+};
+
+// What a block of one tile size costs, in us, for head_dim 128: `fixed` beside its keys,
+// `unit` per 64 keys with one to four blocks on its CU.
+struct TileCost {
+  int rows;
+  double fixed, unit[4];
+};
+
+constexpr TileCost kF16Costs[] = {{16, 6.3, {0.57, 1.17, 1.81, 2.48}}, {64, 6.6, {1.02, 1.30, 1.30, 1.30}},
+                                  {128, 8.0, {1.32, 1.62, 1.62, 1.62}}};
+constexpr TileCost kF32Costs[] = {{16, 2.5, {1.97, 4.05, 6.23, 8.55}}, {64, 5.7, {4.73, 9.50, 9.50, 9.50}},
+                                  {128, 6.6, {7.61, 14.8, 14.8, 14.8}}};
+
+// The tile size and the split of its keys that these costs make fastest: every tile
+// whole, or in parts that give each CU one block, two, up to as many as it holds, or
+// two, three or four times that.  A call takes its blocks' time (all of them in one
+// round; in more rounds the average load and most of a last block), joined with the time
+// that its keys take from HBM (as a 3-norm).  A split call merges: a launch, and its
+// partial results written and read at 4.3 TB/s.
 mvr::ScoreAttentionPlan plan_scored(const mvr_paged_attention_args* a, const mvr_score_rules* r, size_t limit) {
-  mvr::ScoreAttentionPlan plan{};
-  const int64_t group = a->num_q_heads / a->num_kv_heads, hkv = a->num_kv_heads;
-  plan.tile_rows = 16;
-  plan.row_tiles = (int)((group * a->max_q_len + plan.tile_rows - 1) / plan.tile_rows);
-  plan.parts = 1;
-  plan.part_units = INT32_MAX;
-  // Units of one row tile's keys at most.
-  int64_t bound = units_of(a->max_seq_len);
-  if (r->window > 0 && !r->prefix_lens)
-    bound = std::min(bound, units_of((int64_t)r->window + (plan.tile_rows + group - 1) / group) + 1);
-  // Row tiles and units of all of them: by the host tables, or as if all requests were alike.
-  int64_t tiles = 0, work = 0;
-  const int32_t *cu = a->cu_q_lens_host, *sl = a->seq_lens_host;
-  for (int s = 0; s < a->num_seqs && cu && sl; s++) {
-    const int64_t q = std::min<int64_t>(std::max<int64_t>(0, (int64_t)cu[s + 1] - cu[s]), a->max_q_len);
-    const int64_t n = (group * q + plan.tile_rows - 1) / plan.tile_rows;
-    tiles += n;
-    work += n * std::min(bound, std::max<int64_t>(units_of(sl[s]), 0));
+  const bool f16 = a->dtype == MVR_DTYPE_F16;
+  const int64_t group = a->num_q_heads / a->num_kv_heads, longest_rows = group * a->max_q_len;
+  const int64_t cus = compute_units(), pairs = (int64_t)a->num_seqs * a->num_kv_heads;
+  const double unit_scale = a->head_dim / 128.0;
+  // Overrides, for tests and tuning: a tile size that the head dimension has, and its parts.
+  static const int set_rows = env_int("MVR_SCORE_TILE_ROWS", 0);
+  static const int set_units = env_int("MVR_SCORE_PART_UNITS", 0);
+  bool rows_set = false;
+  for (const TileCost& tile : kF16Costs) rows_set |= tile.rows == set_rows && mvr::score_tile_supported(set_rows, a->head_dim);
+  mvr::ScoreAttentionPlan best{};
+  double best_cost = INFINITY;
+  for (const TileCost& tile : f16 ? kF16Costs : kF32Costs) {
+    if (!mvr::score_tile_supported(tile.rows, a->head_dim)) continue;
+    // (A tile that no request fills half costs what the smaller one does, or more.)
+    if (rows_set ? tile.rows != set_rows : longest_rows <= tile.rows / 2 && best_cost < INFINITY) continue;
+    const int held = mvr::score_blocks_per_cu(tile.rows, f16, a->head_dim);
+    const TileWork w(a, r, tile.rows);
+    const int64_t row_tiles = (longest_rows + tile.rows - 1) / tile.rows, all_tiles = pairs * row_tiles;
+    // (Row tiles of one KV head read the same keys, which the caches keep.)
+    const double hbm = (double)w.units / std::max<int64_t>(1, row_tiles) *
+                       (2.0 * mvr::kScoreUnitTokens * a->head_dim * es_of(a->dtype) / 5.9e6);
+    auto cost_of = [&](int64_t blocks, double longest) { // of `longest` units at most
+      double body;
+      if (blocks <= held * cus)
+        body = longest * tile.unit[std::max<int64_t>(0, (blocks + cus - 1) / cus - 1)];
+      else
+        body = std::max(w.units * tile.unit[held - 1] / (held * cus) + 0.5 * longest * tile.unit[0], longest * tile.unit[0]);
+      body *= unit_scale;
+      return tile.fixed + cbrt(body * body * body + hbm * hbm * hbm);
+    };
+    auto take = [&](double cost, int64_t parts, int64_t part_units, size_t bytes) {
+      if (!(cost < best_cost)) return;
+      best_cost = cost;
+      best.tile_rows = tile.rows;
+      best.row_tiles = (int)row_tiles;
+      best.parts = (int)parts;
+      best.part_units = (int)std::min<int64_t>(part_units, INT32_MAX / 2); // (units are added to it)
+      best.partial_bytes = bytes;
+    };
+    auto take_split = [&](int64_t part) { // parts of `part` units
+      const int64_t parts = std::min<int64_t>((w.longest + part - 1) / part, mvr::kScoreMaxParts);
+      if (parts < 2 || parts > kMaxThreads / 256 / ((pairs + mvr::kScoreXcds) * row_tiles)) return;
+      const int64_t rows = all_tiles * parts * tile.rows;
+      const size_t bytes = align_up((size_t)rows * a->head_dim * sizeof(float), 256) +
+                           align_up((size_t)rows * 2 * sizeof(float), 256) +
+                           align_up((size_t)all_tiles * sizeof(int32_t), 256);
+      if (bytes > limit) return;
+      part = std::max(part, (w.longest + parts - 1) / parts);
+      const int64_t blocks = std::max(w.tiles, w.units / part + w.tiles / 2);
+      // (The partials that are written: the others' slots are left alone.)
+      const double moved = 2.0 * blocks * tile.rows * (a->head_dim + 2) * sizeof(float) / 4.3e6;
+      take(cost_of(blocks, part) + 4.5 + moved, parts, part, bytes);
+    };
+    take(cost_of(w.tiles, w.longest), 1, INT32_MAX, 0);
+    if (w.tiles == 0 || w.longest < 2 || limit == 0) continue;
+    if (set_units) {
+      if (set_units < w.longest) best_cost = rows_set ? INFINITY : best_cost, take_split(set_units);
+      continue;
+    }
+    int64_t last = 0;
+    for (int64_t target = cus; target <= 4 * held * cus; target += target < held * cus ? cus : held * cus) {
+      if (w.tiles >= target) continue;
+      // (A tile's last part is half full on average.)
+      const int64_t part = std::max<int64_t>(1, (w.units + target - w.tiles / 2 - 1) / (target - w.tiles / 2));
+      if (part < w.longest && part != last) take_split(part);
+      last = part;
+    }
+    // Where a workspace is too small for all of these, the fewest parts that fit.
+    if (limit != SIZE_MAX && best.parts <= 1)
+      for (int64_t parts = 2; parts <= 8; parts++) take_split((w.longest + parts - 1) / parts);
   }
-  if (!cu || !sl) {
-    const int64_t tokens = a->sum_seq_lens > 0 ? (a->sum_seq_lens + a->num_seqs - 1) / a->num_seqs : a->max_seq_len;
-    tiles = (int64_t)a->num_seqs * plan.row_tiles;
-    work = tiles * std::min(bound, units_of(tokens));
-  }
-  tiles *= hkv;
-  work *= hkv;
-  const int64_t all_tiles = a->num_seqs * hkv * plan.row_tiles;
-  const int64_t target = 3 * (int64_t)compute_units();
-  if (tiles == 0 || tiles >= target || bound < 2 || limit == 0) return plan;
-  const int64_t part = std::max<int64_t>(1, (work + target - 1) / target);
-  int64_t parts = std::min<int64_t>((bound + part - 1) / part, mvr::kScoreMaxParts);
-  parts = std::min(parts, kMaxThreads / 256 / (all_tiles + mvr::kScoreXcds * plan.row_tiles));
-  auto bytes_of = [&](int64_t n) {
-    return align_up((size_t)all_tiles * n * plan.tile_rows * a->head_dim * sizeof(float), 256) +
-           align_up((size_t)all_tiles * n * plan.tile_rows * 2 * sizeof(float), 256) +
-           align_up((size_t)all_tiles * sizeof(int32_t), 256);
-  };
-  while (parts > 1 && bytes_of(parts) > limit) parts--;
-  if (parts <= 1) return plan;
-  plan.parts = (int)parts;
-  plan.part_units = (int)std::max(part, (bound + parts - 1) / parts);
-  plan.partial_bytes = bytes_of(parts);
-  return plan;
+  return best;
 }
 
 int copy_floats(const float* dev, size_t count, void* stream, std::vector<float>& host) {

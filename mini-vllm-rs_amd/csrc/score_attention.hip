@@ -20,26 +20,6 @@
 namespace mvr {
 namespace {
 
-constexpr int kWaves = 4; // wavefronts per block
-
-// A block's item: part `part` of row tile rt of (request, KV head) pair.  The parts and
-// row tiles of one pair, which read the same keys, run on one XCD (workgroups are dealt
-// to the 8 XCDs round-robin); the last row tiles, which a causal mask leaves the most
-// keys, start first.
-struct Item {
-  int pair, rt, part;
-};
-
-__device__ __forceinline__ Item block_item(const ScoreAttentionParams& p) {
-  const uint32_t of_xcd = blockIdx.x / kScoreXcds, inner = (uint32_t)(p.row_tiles * p.parts);
-  const uint32_t eight = of_xcd / inner, rest = of_xcd - eight * inner, rt = rest / (uint32_t)p.parts;
-  return {(int)(eight * kScoreXcds + blockIdx.x % kScoreXcds), p.row_tiles - 1 - (int)rt, (int)(rest - rt * p.parts)};
-}
-
-__device__ __forceinline__ int units_of(const KeyRange& k) {
-  return (k.end + kScoreUnitTokens - 1) / kScoreUnitTokens - k.begin / kScoreUnitTokens;
-}
-
 // ---------------------------------------------------------------------------
 // Key streaming: a block of 4 wavefronts per item, 16 rows, each wavefront its share
 // of the part's 16-token chunks straight from the cache; their results merge in LDS.
@@ -51,27 +31,23 @@ constexpr int step_chunks() {
   return sizeof(typename Tr::elem) == 4 ? 1 : 2;
 }
 
-constexpr int stream_blocks_per_cu(bool f16, int head_dim) {
-  return head_dim <= 64 ? 4 : head_dim <= (f16 ? 128 : 96) ? 3 : head_dim <= 160 ? 2 : 1;
-}
-
 // TP: page sizes that are not a multiple of 16, where every token row has a page of its
 // own to look up.
 template <typename Tr, int D, bool TP>
-__global__ __launch_bounds__(kWaveSize* kWaves, (stream_blocks_per_cu(sizeof(typename Tr::elem) == 2, D))) void score_stream_kernel(
+__global__ __launch_bounds__(kWaveSize* kScoreWaves, (score_stream_blocks_per_cu(sizeof(typename Tr::elem) == 2, D))) void score_stream_kernel(
     ScoreAttentionParams p) {
   typedef typename Tr::elem T;
   constexpr int kTileRows = 16, C = step_chunks<Tr>(), kMergeStride = D + 4;
-  constexpr size_t kTileBytes = (size_t)kWaves * C * kChunkTokens * D * sizeof(T);
-  constexpr size_t kMergeBytes = (size_t)kWaves * kTileRows * (kMergeStride + 2) * sizeof(float);
+  constexpr size_t kTileBytes = (size_t)kScoreWaves * C * kChunkTokens * D * sizeof(T);
+  constexpr size_t kMergeBytes = (size_t)kScoreWaves * kTileRows * (kMergeStride + 2) * sizeof(float);
   __shared__ __attribute__((aligned(16))) char lds_raw[kTileBytes > kMergeBytes ? kTileBytes : kMergeBytes];
   float* const merge_o = reinterpret_cast<float*>(lds_raw);
-  float* const merge_ml = merge_o + kWaves * kTileRows * kMergeStride;
+  float* const merge_ml = merge_o + kScoreWaves * kTileRows * kMergeStride;
 
   const int l = lane_id(), g = l >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
   T* const lds = reinterpret_cast<T*>(lds_raw) + (size_t)wave * C * kChunkTokens * D;
-  const Item it = block_item(p);
+  const ScoreItem it = block_item(p);
   const ScoreTables& t = p.t;
   if (it.pair >= t.num_seqs * t.num_kv_heads) return;
   const int b = it.pair / t.num_kv_heads, h = it.pair - b * t.num_kv_heads;
@@ -101,8 +77,8 @@ __global__ __launch_bounds__(kWaveSize* kWaves, (stream_blocks_per_cu(sizeof(typ
   const int n_chunks = (range.end + kChunkTokens - 1) / kChunkTokens;
   const int part0 = kUnitChunks * (unit0 + (int)((int64_t)it.part * units / parts));
   const int part1 = min(kUnitChunks * (unit0 + (int)((int64_t)(it.part + 1) * units / parts)), n_chunks);
-  const int k0 = part0 + (int)((int64_t)(part1 - part0) * wave / kWaves);
-  const int k1 = part0 + (int)((int64_t)(part1 - part0) * (wave + 1) / kWaves);
+  const int k0 = part0 + (int)((int64_t)(part1 - part0) * wave / kScoreWaves);
+  const int k1 = part0 + (int)((int64_t)(part1 - part0) * (wave + 1) / kScoreWaves);
   // What the lane's row sees of them.  (A chunk past k1 is seen by nobody.)
   ScoreRow mine = row;
   mine.lo = max(row.lo, k0 * kChunkTokens);
@@ -271,12 +247,12 @@ __global__ __launch_bounds__(kWaveSize* kWaves, (stream_blocks_per_cu(sizeof(typ
       Tr::stage_v(lds + c * kChunkTokens * D, le, tokens, vbuf[c]);
     }
     load_v(k + C, vbuf);
-    const int first = k * kChunkTokens + 4 * g; // key of element e: first + 16 (e / 4) + e % 4
-    to_scores(p.r, row, 0.f, x, [&](int e) { return first + 16 * (e >> 2) + (e & 3); });
-    if constexpr (kMasked) {
-#pragma unroll
-      for (int e = 0; e < 4 * C; e++) x[e] = sees(mine, first + 16 * (e >> 2) + (e & 3)) ? x[e] : -INFINITY;
-    }
+    const int first = k * kChunkTokens + 4 * g;
+    auto offset = [](int e) { return 16 * (e >> 2) + (e & 3); };
+    if constexpr (kMasked)
+      to_masked_scores(p.r, mine, 0.f, x, first, offset);
+    else
+      to_scores(p.r, mine, 0.f, x, first, offset);
     softmax(x);
     // The V tiles are written by this wavefront's own lanes: wait for the LDS writes
     // before reads of other lanes' rows.
@@ -335,18 +311,18 @@ __global__ __launch_bounds__(kWaveSize* kWaves, (stream_blocks_per_cu(sizeof(typ
   }
   __syncthreads();
   constexpr int kCells = kTileRows * (D / 4); // float4 of the tile
-  for (int c = threadIdx.x; c < kCells; c += kWaves * kWaveSize) {
+  for (int c = threadIdx.x; c < kCells; c += kScoreWaves * kWaveSize) {
     const int rr = c / (D / 4), d = 4 * (c % (D / 4));
     const int at = it.rt * kTileRows + rr;
     if (at >= rows) break; // rows grow with c
     float mmax = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < kWaves; j++) mmax = fmaxf(mmax, merge_ml[(j * kTileRows + rr) * 2]);
+    for (int j = 0; j < kScoreWaves; j++) mmax = fmaxf(mmax, merge_ml[(j * kTileRows + rr) * 2]);
     const float m_use = mmax == -INFINITY ? 0.f : mmax;
     float4v acc = {0.f, 0.f, 0.f, 0.f};
     float sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < kWaves; j++) {
+    for (int j = 0; j < kScoreWaves; j++) {
       const float w = __builtin_amdgcn_exp2f(merge_ml[(j * kTileRows + rr) * 2] - m_use);
       sum += w * merge_ml[(j * kTileRows + rr) * 2 + 1];
       acc += w * *reinterpret_cast<const float4v*>(merge_o + (j * kTileRows + rr) * kMergeStride + d);
@@ -421,25 +397,38 @@ __global__ __launch_bounds__(256) void score_merge_kernel(ScoreAttentionParams p
 }
 
 template <typename Tr, int D>
-hipError_t launch_dim(const ScoreAttentionPlan& plan, const ScoreAttentionParams& p, hipStream_t stream) {
-  const int64_t pairs = (int64_t)p.t.num_seqs * p.t.num_kv_heads;
-  const int64_t eights = (pairs + kScoreXcds - 1) / kScoreXcds;
-  const dim3 grid((unsigned)(eights * kScoreXcds * plan.row_tiles * plan.parts)), block(kWaveSize * kWaves);
+hipError_t launch_stream(const ScoreAttentionPlan& plan, const ScoreAttentionParams& p, hipStream_t stream) {
+  const dim3 grid(score_blocks(plan, p)), block(kWaveSize * kScoreWaves);
   if (p.t.page_size % kChunkTokens == 0)
     hipLaunchKernelGGL((score_stream_kernel<Tr, D, false>), grid, block, 0, stream, p);
   else
     hipLaunchKernelGGL((score_stream_kernel<Tr, D, true>), grid, block, 0, stream, p);
-  const hipError_t err = hipGetLastError();
-  if (err != hipSuccess || plan.parts == 1) return err;
-  constexpr int kTileBlocks = (16 * (D / 4) + 255) / 256;
-  hipLaunchKernelGGL((score_merge_kernel<Tr, D, 16>), dim3((unsigned)(kTileBlocks * pairs * plan.row_tiles)), dim3(256), 0,
-                     stream, p);
   return hipGetLastError();
+}
+
+template <typename Tr, int D, int kTileRows>
+hipError_t launch_merge(const ScoreAttentionPlan& plan, const ScoreAttentionParams& p, hipStream_t stream) {
+  constexpr int kTileBlocks = (kTileRows * (D / 4) + 255) / 256;
+  const dim3 grid((unsigned)((int64_t)kTileBlocks * p.t.num_seqs * p.t.num_kv_heads * plan.row_tiles));
+  hipLaunchKernelGGL((score_merge_kernel<Tr, D, kTileRows>), grid, dim3(256), 0, stream, p);
+  return hipGetLastError();
+}
+
+template <typename Tr, int D>
+hipError_t launch_dim(const ScoreAttentionPlan& plan, const ScoreAttentionParams& p, int dtype, hipStream_t stream) {
+  const hipError_t err =
+      plan.tile_rows == 16 ? launch_stream<Tr, D>(plan, p, stream) : launch_score_tiles(plan, p, dtype, D, stream);
+  if (err != hipSuccess || plan.parts == 1) return err;
+  switch (plan.tile_rows) {
+  case 16: return launch_merge<Tr, D, 16>(plan, p, stream);
+  case 64: return launch_merge<Tr, D, 64>(plan, p, stream);
+  default: return launch_merge<Tr, D, 128>(plan, p, stream);
+  }
 }
 
 template <int D>
 hipError_t launch_type(const ScoreAttentionPlan& plan, const ScoreAttentionParams& p, int dtype, hipStream_t stream) {
-  return dtype == 1 ? launch_dim<F16Traits<D>, D>(plan, p, stream) : launch_dim<F32Traits<D>, D>(plan, p, stream);
+  return dtype == 1 ? launch_dim<F16Traits<D>, D>(plan, p, dtype, stream) : launch_dim<F32Traits<D>, D>(plan, p, dtype, stream);
 }
 
 } // namespace

@@ -29,7 +29,8 @@ struct ScoreTables {
   int32_t page_magic_shift;
 };
 
-// tanh(y) = y * sum_k c_k y^2k for |y| <= kTanhPolynomial.
+// tanh(y) = y * sum_k c_k y^2k for |y| <= kTanhPolynomial but for 4.4e-9 of it (least
+// squares, reweighted towards the largest error); in 32 bits it is within 1.0e-7.
 constexpr float kTanhPolynomial = 0.625f;
 constexpr float kTanhCoefficients[6] = {1.0f,
                                         -0.3333328068256378f,
@@ -41,11 +42,10 @@ constexpr float kTanhCoefficients[6] = {1.0f,
 struct ScoreRules {
   float scale_log2; // scale * log2(e)
   float cap_log2;   // cap * log2(e); 0: none
-  float cap_scale;  // scale / cap
   // Of a dot product s up to cap_poly_limit in size, the capped score in log2 units is
-  // s * sum_k cap_poly[k] s^2k.  (Limit below 0: the coefficients leave the range of 32
-  // bits.)
+  // s * sum_k cap_poly[k] s^2k; of any, cap_log2 * (1 - 2 / (2^(cap_exp_scale * s) + 1)).
   float cap_poly_limit, cap_poly[6];
+  float cap_exp_scale; // 2 * log2(e) * scale / cap
   int32_t window;   // 0: none
   const float* slopes;
   const int32_t* first_keys;
@@ -72,12 +72,44 @@ struct ScoreAttentionParams {
 };
 
 struct ScoreAttentionPlan {
-  int tile_rows;
+  int tile_rows; // 16 (key streaming), 64 or 128 (key tiles in LDS)
   int row_tiles;
   int parts, part_units;
   size_t partial_bytes; // 0: not split
 };
 
+// Row tiles: 16 and 128 rows for every head dimension, 64 up to 128.
+constexpr bool score_tile_supported(int tile_rows, int head_dim) {
+  return tile_rows == 16 || tile_rows == 128 || (tile_rows == 64 && head_dim <= 128);
+}
+
+// Blocks that a CU holds at once, by registers (16 rows, whose wavefronts keep K and V
+// chunks in them) and LDS (64 and 128 rows).
+constexpr int score_stream_blocks_per_cu(bool f16, int head_dim) {
+  return head_dim <= 64 ? 4 : head_dim <= (f16 ? 128 : 96) ? 3 : head_dim <= 160 ? 2 : 1;
+}
+constexpr int score_tile_blocks_per_cu(int tile_rows, bool f16, int head_dim) {
+  if (tile_rows == 64) return f16 || head_dim <= 64 ? 2 : 1;
+  return head_dim <= 128 ? 2 : 1;
+}
+
+constexpr int score_blocks_per_cu(int tile_rows, bool f16, int head_dim) {
+  return tile_rows == 16 ? score_stream_blocks_per_cu(f16, head_dim) : score_tile_blocks_per_cu(tile_rows, f16, head_dim);
+}
+
+// Blocks of one launch: (request, KV head) pairs by eights, so that a pair's blocks run on
+// one XCD.
+inline unsigned score_blocks(const ScoreAttentionPlan& plan, const ScoreAttentionParams& p) {
+  const int64_t eights = ((int64_t)p.t.num_seqs * p.t.num_kv_heads + kScoreXcds - 1) / kScoreXcds;
+  return (unsigned)(eights * kScoreXcds * plan.row_tiles * plan.parts);
+}
+
+// score_tiles.hip: the attention itself, of row tiles of 64 (head_dim up to 128) and 128
+// rows.
+hipError_t launch_score_tiles(const ScoreAttentionPlan& plan, const ScoreAttentionParams& params, int dtype, int head_dim,
+                              hipStream_t stream);
+
+// The attention, then the merge of what was split.
 hipError_t launch_score_attention(const ScoreAttentionPlan& plan, const ScoreAttentionParams& params, int dtype,
                                   int head_dim, hipStream_t stream);
 

@@ -109,33 +109,33 @@ __device__ __forceinline__ KeyRange row_tile_range(const KeyRange& mine) {
   return k;
 }
 
-// tanh(y) / y for |y| <= kTanhPolynomial is a polynomial in y^2 (kTanhCoefficients) but
-// for 4.4e-9 of it (least squares, reweighted towards the largest error); y times it, in
-// 32 bits, is within 1.0e-7.  A form with exponentials takes an e^x and a reciprocal, 16
-// cycles each, and loses the small values to cancellation.
-__device__ __forceinline__ float tanh_over(float u) {
-  float p = kTanhCoefficients[5];
+// Over all lanes' rows.
+__device__ __forceinline__ KeyRange wave_range(const KeyRange& mine) {
+  KeyRange k = mine;
 #pragma unroll
-  for (int k = 4; k >= 0; k--) p = fmaf(p, u, kTanhCoefficients[k]);
-  return p;
-}
-
-// tanh(y), any y: past the polynomial's range 1 - 2 / (e^2|y| + 1), there 0.55 at
-// least, so the difference loses no more than one bit.
-__device__ __forceinline__ float tanh_any(float y) {
-  const float a = fabsf(y);
-  const float e = __builtin_amdgcn_exp2f(a * 2.8853900817779268f);
-  const float big = copysignf(fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f), y);
-  return a <= kTanhPolynomial ? y * tanh_over(y * y) : big; // (a NaN: big, which is one)
+  for (int x = 32; x; x >>= 1) {
+    k.begin = min(k.begin, __shfl_xor(k.begin, x));
+    k.end = max(k.end, __shfl_xor(k.end, x));
+    k.all_begin = max(k.all_begin, __shfl_xor(k.all_begin, x));
+    k.all_end = min(k.all_end, __shfl_xor(k.all_end, x));
+  }
+  auto first = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  k = {first(k.begin), first(k.end), first(k.all_begin), first(k.all_end)};
+  if (k.end == 0) k.begin = 0;
+  return k;
 }
 
 // N dot products q . k of one row to scores in log2 units less `minus`,
-// x = score * log2(e) - minus; key(e): the key of element e.  What the rules lack is left
-// out by branches that all lanes take alike.  A cap costs 7 operations a score while all
-// of them lie in the polynomial's range (those of a model that caps them mostly do): its
-// coefficients hold scale, cap and log2(e).
-template <int N, typename Key>
-__device__ __forceinline__ void to_scores(const ScoreRules& r, const ScoreRow& row, float minus, float (&x)[N], Key key) {
+// x = score * log2(e) - minus; element e is key key0 + offset(e), the offsets constants.
+// What the rules lack is left out by branches that all lanes take alike.
+//
+// A cap costs 7 operations a score while all of them lie in the polynomial's range (those
+// of a model that caps them mostly do): its coefficients hold scale, cap and log2(e).
+// Past it tanh(y) = 1 - 2 / (e^2y + 1), off by 2^-21 at most; that takes an exponential
+// and a reciprocal, 16 cycles each, and loses small values to cancellation.
+template <int N, typename Offset>
+__device__ __forceinline__ void to_scores(const ScoreRules& r, const ScoreRow& row, float minus, float (&x)[N], int key0,
+                                          Offset offset) {
   if (r.cap_log2 > 0.f) {
     float top = 0.f;
 #pragma unroll
@@ -143,7 +143,11 @@ __device__ __forceinline__ void to_scores(const ScoreRules& r, const ScoreRow& r
     // (A NaN among scores in range takes either way as a NaN.)
     if (__any(!(top <= r.cap_poly_limit))) {
 #pragma unroll
-      for (int e = 0; e < N; e++) x[e] = fmaf(r.cap_log2, tanh_any(x[e] * r.cap_scale), -minus);
+      for (int e = 0; e < N; e++) {
+        if (e % 4 == 0) __builtin_amdgcn_sched_barrier(0); // (few at a time: the other way sets the registers)
+        const float ey = __builtin_amdgcn_exp2f(x[e] * r.cap_exp_scale);
+        x[e] = fmaf(r.cap_log2, fmaf(-2.f, __builtin_amdgcn_rcpf(ey + 1.f), 1.f), -minus);
+      }
     } else {
 #pragma unroll
       for (int e = 0; e < N; e++) {
@@ -159,9 +163,50 @@ __device__ __forceinline__ void to_scores(const ScoreRules& r, const ScoreRow& r
     for (int e = 0; e < N; e++) x[e] = fmaf(x[e], r.scale_log2, -minus);
   }
   if (r.slopes) {
+    float away = (float)(key0 - row.pos);
+    asm volatile("" : "+v"(away)); // (or every element's distance is held over the key loop)
 #pragma unroll
-    for (int e = 0; e < N; e++) x[e] = fmaf(-row.slope_log2, fabsf((float)(key(e) - row.pos)), x[e]);
+    for (int e = 0; e < N; e++) x[e] = fmaf(-row.slope_log2, fabsf(away + (float)offset(e)), x[e]);
   }
+}
+
+// `instead` in the place of the scores that the row does not see.
+template <int N, typename Offset>
+__device__ __forceinline__ void mask_scores(const ScoreRow& row, float (&x)[N], int key0, Offset offset, float instead) {
+  int from = key0 - row.lo;
+  asm volatile("" : "+v"(from)); // (as above)
+#pragma unroll
+  for (int e = 0; e < N; e++) x[e] = (uint32_t)(from + offset(e)) < (uint32_t)row.width ? x[e] : instead;
+}
+
+// Both.  What the row does not see is taken out before a cap too, whose way to the tanh
+// depends on the largest score.
+template <int N, typename Offset>
+__device__ __forceinline__ void to_masked_scores(const ScoreRules& r, const ScoreRow& row, float minus, float (&x)[N],
+                                                 int key0, Offset offset) {
+  if (r.cap_log2 > 0.f) mask_scores(row, x, key0, offset, 0.f);
+  to_scores(r, row, minus, x, key0, offset);
+  mask_scores(row, x, key0, offset, -INFINITY);
+}
+
+constexpr int kScoreWaves = 4; // wavefronts per block
+
+// A block's item: part `part` of row tile rt of (request, KV head) pair.  The parts and
+// row tiles of one pair, which read the same keys, run on one XCD (workgroups are dealt
+// to the 8 XCDs round-robin); the last row tiles, which a causal mask leaves the most
+// keys, start first.
+struct ScoreItem {
+  int pair, rt, part;
+};
+
+__device__ __forceinline__ ScoreItem block_item(const ScoreAttentionParams& p) {
+  const uint32_t of_xcd = blockIdx.x / kScoreXcds, inner = (uint32_t)(p.row_tiles * p.parts);
+  const uint32_t eight = of_xcd / inner, rest = of_xcd - eight * inner, rt = rest / (uint32_t)p.parts;
+  return {(int)(eight * kScoreXcds + blockIdx.x % kScoreXcds), p.row_tiles - 1 - (int)rt, (int)(rest - rt * p.parts)};
+}
+
+__device__ __forceinline__ int units_of(const KeyRange& k) {
+  return (k.end + kScoreUnitTokens - 1) / kScoreUnitTokens - k.begin / kScoreUnitTokens;
 }
 
 // log of sum_j e^score_j from the row's maximum (log2 units) and sum; a row without a

@@ -115,12 +115,11 @@ __global__ __launch_bounds__(kWaveSize* kWaves, (weights_waves<typename Tr::elem
 #pragma unroll
       for (int e = 0; e < 4; e++) x[4 * c + e] = sc[e];
     }
-    auto key_of = [&](int e) { return key0 + 4 * g + 16 * (e >> 2) + (e & 3); };
-    to_scores(p.r, r.row, lse_log2, x, key_of);
-    if (masked) {
-#pragma unroll
-      for (int e = 0; e < 4 * kChunks; e++) x[e] = sees(r.row, key_of(e)) ? x[e] : -INFINITY;
-    }
+    auto offset = [](int e) { return 16 * (e >> 2) + (e & 3); };
+    if (masked)
+      to_masked_scores(p.r, r.row, lse_log2, x, key0 + 4 * g, offset);
+    else
+      to_scores(p.r, r.row, lse_log2, x, key0 + 4 * g, offset);
 #pragma unroll
     for (int e = 0; e < 4 * kChunks; e++) acc[e] += __builtin_amdgcn_exp2f(x[e]);
   }

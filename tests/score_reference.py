@@ -61,10 +61,11 @@ class Batch:
         """Scores [G, q, n] of KV head h (-inf where not seen) and how far 32-bit ones may be off (0 there).
 
         A score is off by its D products and sums in 32 bits, the scale's rounding among them (2^-24 each of the sum of
-        |q k|); what the cap makes of it, off by 4 roundings of the tanh and its products (2^-21 of a capped score: past
-        the polynomial's range the tanh is 0.55 at least, and its absolute error 2^-22); the slope, its factor log2(e)
-        and the distance's product (2^-22 of it).  Differences to the row's maximum and the exponential: 2^-20 + 2^-23 of
-        the score."""
+        |q k|); what the cap makes of it: 2^-21 of the capped score by the polynomial, six roundings of a half step, and
+        where a score near it leaves the polynomial's range (0.625 of the cap, 0.09 of caps past 1e4) 2^-21 of the cap by
+        1 - 2 / (e^2y + 1), a reciprocal of 2 at most off by 2^-22 and an exponential off by as much at a slope of 1/2;
+        the slope, its factor log2(e) and the distance's product (2^-22 of it).  Differences to the row's maximum and the
+        exponential: 2^-20 + 2^-23 of the score."""
         group = self.hq // self.hkv
         heads = slice(h * group, (h + 1) * group)
         q, n = int(self.q_lens[b]), int(self.seq_lens[b])
@@ -73,7 +74,9 @@ class Batch:
         s, size = x @ k.T * scale, (x.abs() @ k.abs().T * scale).nan_to_num(0.0, 0.0, 0.0)
         off = 2.0 ** -24 * (self.d + 8) * size
         if self.cap:
+            far = bool((s.abs() > 0.08 * self.cap).any())
             s = self.cap * torch.tanh(s / self.cap)
+            off = off + (2.0 ** -21 * self.cap if far else 0.0)
         off = off + 2.0 ** -21 * s.abs().nan_to_num(0.0, 0.0, 0.0)
         if self.slopes is not None:
             away = (torch.arange(n - q, n)[:, None] - torch.arange(n)).abs().double()
