@@ -7,7 +7,7 @@
 namespace mvr {
 namespace {
 
-constexpr int kTileWaves = 4; // wavefronts per block
+constexpr int kTileWaves = 4; // wavefronts per block, but where a kernel takes more
 
 typedef float float16v __attribute__((ext_vector_type(16)));
 typedef int int4v __attribute__((ext_vector_type(4)));
@@ -41,21 +41,21 @@ __device__ __forceinline__ void stage_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// A block's row tile of 32 * RW rows in 4 / RW groups of wavefronts, which take
+// A block's row tile of 32 * RW rows in W / RW groups of wavefronts, which take
 // alternating key tiles.
-template <int D, typename T, int RW>
+template <int D, typename T, int RW, int W = kTileWaves>
 struct Tile {
   static constexpr bool kF32 = sizeof(T) == 4;
-  static constexpr int kGroups = kTileWaves / RW;
-  static constexpr int kTileTokens = kF32 || kGroups > 1 ? 32 : 64;
+  static constexpr int kGroups = W / RW;
+  static constexpr int kTileTokens = kF32 || (kGroups > 1 && W == kTileWaves) ? 32 : 64;
   static constexpr int kSub = kTileTokens / 32;             // S^T blocks of 32 tokens
   static constexpr int kStageTokens = kTileTokens * kGroups; // one tile per group
   static constexpr int kChunkElems = 16 / (int)sizeof(T);
   static constexpr int kChunksPerRow = D / kChunkElems; // 16-byte chunks per token row
   static constexpr int kElems = kStageTokens * D;       // of K, or V, per stage
-  static constexpr int kLoads = kStageTokens * kChunksPerRow / (kTileWaves * kWaveSize); // per thread and operand
-  static constexpr int kWaveTokens = kStageTokens / kTileWaves; // consecutive tokens that a wavefront stages
-  static_assert(kLoads * kTileWaves * kWaveSize == kStageTokens * kChunksPerRow, "whole loads");
+  static constexpr int kLoads = kStageTokens * kChunksPerRow / (W * kWaveSize); // per thread and operand
+  static constexpr int kWaveTokens = kStageTokens / W; // consecutive tokens that a wavefront stages
+  static_assert(kLoads * W * kWaveSize == kStageTokens * kChunksPerRow, "whole loads");
   // LDS swizzles, so that the lanes of one read fall into different banks: K by
   // 16-byte chunks with the row (inside groups of the row's largest power of
   // two), F16 V by 32-byte pieces (a transposing read takes 4 rows x 2 pieces at

@@ -69,7 +69,7 @@ int check_scored(const mvr_paged_attention_args* a, const mvr_score_rules* r) {
   const int64_t group = a->num_q_heads / a->num_kv_heads;
   const int64_t pairs = (int64_t)a->num_seqs * a->num_kv_heads + mvr::kScoreXcds - 1;
   const int64_t tiles = pairs * ((group * a->max_q_len + 15) / 16);
-  if (group * a->max_q_len > INT32_MAX - 1024 || tiles > kMaxThreads / 256 / 2)
+  if (group * a->max_q_len > INT32_MAX - 1024 || tiles > kMaxThreads / 512 / 2)
     return fail(MVR_E_UNSUPPORTED, "%d requests of %d tokens are more than one call takes", a->num_seqs, a->max_q_len);
   return MVR_OK;
 }
@@ -166,14 +166,18 @@ struct TileWork {
 // What a block of one tile size costs, in us, for head_dim 128: `fixed` beside its keys,
 // `unit` per 64 keys with one to four blocks on its CU.
 struct TileCost {
-  int rows;
+  int rows, waves;
   double fixed, unit[4];
 };
 
-constexpr TileCost kF16Costs[] = {{16, 6.3, {0.57, 1.17, 1.81, 2.48}}, {64, 6.6, {1.02, 1.30, 1.30, 1.30}},
-                                  {128, 8.0, {1.32, 1.62, 1.62, 1.62}}};
-constexpr TileCost kF32Costs[] = {{16, 2.5, {1.97, 4.05, 6.23, 8.55}}, {64, 5.7, {4.73, 9.50, 9.50, 9.50}},
-                                  {128, 6.6, {7.61, 14.8, 14.8, 14.8}}};
+constexpr TileCost kF16Costs[] = {{16, 4, 6.3, {0.57, 1.17, 1.81, 2.48}},
+                                  {64, 4, 6.6, {1.02, 1.30, 1.30, 1.30}},
+                                  {128, 4, 8.0, {1.32, 1.62, 1.62, 1.62}},
+                                  {128, 8, 8.0, {0.95, 0.95, 0.95, 0.95}}};
+constexpr TileCost kF32Costs[] = {{16, 4, 2.5, {1.97, 4.05, 6.23, 8.55}},
+                                  {64, 4, 5.7, {4.73, 9.50, 9.50, 9.50}},
+                                  {128, 4, 6.6, {7.61, 14.8, 14.8, 14.8}},
+                                  {128, 8, 6.6, {7.5, 7.5, 7.5, 7.5}}};
 
 // The tile size and the split of its keys that these costs make fastest: every tile
 // whole, or in parts that give each CU one block, two, up to as many as it holds, or
@@ -188,16 +192,18 @@ mvr::ScoreAttentionPlan plan_scored(const mvr_paged_attention_args* a, const mvr
   const double unit_scale = a->head_dim / 128.0;
   // Overrides, for tests and tuning: a tile size that the head dimension has, and its parts.
   static const int set_rows = env_int("MVR_SCORE_TILE_ROWS", 0);
+  static const int set_waves = env_int("MVR_SCORE_TILE_WAVES", 4);
   static const int set_units = env_int("MVR_SCORE_PART_UNITS", 0);
   bool rows_set = false;
-  for (const TileCost& tile : kF16Costs) rows_set |= tile.rows == set_rows && mvr::score_tile_supported(set_rows, a->head_dim);
+  for (const TileCost& tile : kF16Costs)
+    rows_set |= tile.rows == set_rows && tile.waves == set_waves && mvr::score_tile_supported(set_rows, set_waves, a->head_dim);
   mvr::ScoreAttentionPlan best{};
   double best_cost = INFINITY;
   for (const TileCost& tile : f16 ? kF16Costs : kF32Costs) {
-    if (!mvr::score_tile_supported(tile.rows, a->head_dim)) continue;
+    if (!mvr::score_tile_supported(tile.rows, tile.waves, a->head_dim)) continue;
     // (A tile that no request fills half costs what the smaller one does, or more.)
-    if (rows_set ? tile.rows != set_rows : longest_rows <= tile.rows / 2 && best_cost < INFINITY) continue;
-    const int held = mvr::score_blocks_per_cu(tile.rows, f16, a->head_dim);
+    if (rows_set ? tile.rows != set_rows || tile.waves != set_waves : longest_rows <= tile.rows / 2 && best_cost < INFINITY) continue;
+    const int held = mvr::score_blocks_per_cu(tile.rows, tile.waves, f16, a->head_dim);
     const TileWork w(a, r, tile.rows);
     const int64_t row_tiles = (longest_rows + tile.rows - 1) / tile.rows, all_tiles = pairs * row_tiles;
     // (Row tiles of one KV head read the same keys, which the caches keep.)
@@ -216,6 +222,7 @@ mvr::ScoreAttentionPlan plan_scored(const mvr_paged_attention_args* a, const mvr
       if (!(cost < best_cost)) return;
       best_cost = cost;
       best.tile_rows = tile.rows;
+      best.waves = tile.waves;
       best.row_tiles = (int)row_tiles;
       best.parts = (int)parts;
       best.part_units = (int)std::min<int64_t>(part_units, INT32_MAX / 2); // (units are added to it)
@@ -223,7 +230,7 @@ mvr::ScoreAttentionPlan plan_scored(const mvr_paged_attention_args* a, const mvr
     };
     auto take_split = [&](int64_t part) { // parts of `part` units
       const int64_t parts = std::min<int64_t>((w.longest + part - 1) / part, mvr::kScoreMaxParts);
-      if (parts < 2 || parts > kMaxThreads / 256 / ((pairs + mvr::kScoreXcds) * row_tiles)) return;
+      if (parts < 2 || 2 * parts > kMaxThreads / (64 * tile.waves) / ((pairs + mvr::kScoreXcds) * row_tiles)) return;
       const int64_t rows = all_tiles * parts * tile.rows;
       const size_t bytes = align_up((size_t)rows * a->head_dim * sizeof(float), 256) +
                            align_up((size_t)rows * 2 * sizeof(float), 256) +
@@ -374,6 +381,7 @@ int mvr_paged_attention_scored(const mvr_paged_attention_args* a, const mvr_scor
   p.row_tiles = plan.row_tiles;
   p.parts = plan.parts;
   p.part_units = plan.part_units;
+  p.run = mvr::score_run(plan, (int64_t)a->num_seqs * a->num_kv_heads);
   if (plan.parts > 1) {
     const size_t rows = (size_t)a->num_seqs * a->num_kv_heads * plan.row_tiles * plan.parts * plan.tile_rows;
     char* at = static_cast<char*>(a->workspace);
@@ -497,7 +505,7 @@ static int check_layers(int32_t num_layers, int32_t num_seqs, int32_t num_kv_hea
   if (max_moves < 1) return fail(MVR_E_INVALID_ARGUMENT, "max_moves must be positive");
   if (num_pages > INT32_MAX || num_pages > kMaxSlots / num_kv_heads / page_size)
     return fail(MVR_E_UNSUPPORTED, "pools of over 2^31 pages, or 2^40 tokens and heads");
-  if ((int64_t)num_layers * num_seqs > kMaxThreads / threads_per_row / num_kv_heads)
+  if ((int64_t)num_layers * num_seqs + 7 > kMaxThreads / threads_per_row / num_kv_heads)
     return fail(MVR_E_UNSUPPORTED, "more layers, requests and KV heads than one call takes");
   return MVR_OK;
 }

@@ -65,7 +65,7 @@ __global__ __launch_bounds__(kWaveSize* kScoreWaves, (score_stream_blocks_per_cu
   const ScoreRow row = score_row(t, p.r, s, b, head, i);
   KeyRange range = no_rows();
   if (valid) add_row(range, row);
-  range = row_tile_range(range);
+  range = rows_range<16>(range);
 
   // The part's chunks, and the wavefront's.
   const int units = units_of(range), unit0 = range.begin / kScoreUnitTokens;
@@ -75,8 +75,8 @@ __global__ __launch_bounds__(kWaveSize* kScoreWaves, (score_stream_blocks_per_cu
   if (p.parts > 1 && it.part == 0 && threadIdx.x == 0) p.tile_parts[tile] = parts;
   constexpr int kUnitChunks = kScoreUnitTokens / kChunkTokens;
   const int n_chunks = (range.end + kChunkTokens - 1) / kChunkTokens;
-  const int part0 = kUnitChunks * (unit0 + (int)((int64_t)it.part * units / parts));
-  const int part1 = min(kUnitChunks * (unit0 + (int)((int64_t)(it.part + 1) * units / parts)), n_chunks);
+  const int part0 = kUnitChunks * (unit0 + part_begin(it.part, units, parts));
+  const int part1 = min(kUnitChunks * (unit0 + part_begin(it.part + 1, units, parts)), n_chunks);
   const int k0 = part0 + (int)((int64_t)(part1 - part0) * wave / kScoreWaves);
   const int k1 = part0 + (int)((int64_t)(part1 - part0) * (wave + 1) / kScoreWaves);
   // What the lane's row sees of them.  (A chunk past k1 is seen by nobody.)
@@ -398,7 +398,7 @@ __global__ __launch_bounds__(256) void score_merge_kernel(ScoreAttentionParams p
 
 template <typename Tr, int D>
 hipError_t launch_stream(const ScoreAttentionPlan& plan, const ScoreAttentionParams& p, hipStream_t stream) {
-  const dim3 grid(score_blocks(plan, p)), block(kWaveSize * kScoreWaves);
+  const dim3 grid(score_blocks(p)), block(kWaveSize * kScoreWaves);
   if (p.t.page_size % kChunkTokens == 0)
     hipLaunchKernelGGL((score_stream_kernel<Tr, D, false>), grid, block, 0, stream, p);
   else

@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 namespace mvr {
 
 // Keys are split between parts in units of 64 tokens.
@@ -66,6 +68,7 @@ struct ScoreAttentionParams {
   int64_t out_stride_head, out_stride_token;
   int32_t row_tiles; // of the longest request, per (request, KV head)
   int32_t parts, part_units;
+  int32_t run; // items that follow each other on one XCD
   float* partial_o;    // [pair][row tile][part][tile_rows][head_dim]
   float* partial_ml;   // [pair][row tile][part][tile_rows][2]: maximum (log2 units), sum
   int32_t* tile_parts; // [pair][row tile]: parts that it was split into
@@ -73,14 +76,16 @@ struct ScoreAttentionParams {
 
 struct ScoreAttentionPlan {
   int tile_rows; // 16 (key streaming), 64 or 128 (key tiles in LDS)
+  int waves;     // of a block: 4, or 8 (128 rows)
   int row_tiles;
   int parts, part_units;
   size_t partial_bytes; // 0: not split
 };
 
-// Row tiles: 16 and 128 rows for every head dimension, 64 up to 128.
-constexpr bool score_tile_supported(int tile_rows, int head_dim) {
-  return tile_rows == 16 || tile_rows == 128 || (tile_rows == 64 && head_dim <= 128);
+// Row tiles: 16 and 128 rows for every head dimension, 64, and 128 in 8 wavefronts, up to
+// 128.
+constexpr bool score_tile_supported(int tile_rows, int waves, int head_dim) {
+  return tile_rows == 16 || (tile_rows == 128 && waves == 4) || head_dim <= 128;
 }
 
 // Blocks that a CU holds at once, by registers (16 rows, whose wavefronts keep K and V
@@ -88,20 +93,32 @@ constexpr bool score_tile_supported(int tile_rows, int head_dim) {
 constexpr int score_stream_blocks_per_cu(bool f16, int head_dim) {
   return head_dim <= 64 ? 4 : head_dim <= (f16 ? 128 : 96) ? 3 : head_dim <= 160 ? 2 : 1;
 }
-constexpr int score_tile_blocks_per_cu(int tile_rows, bool f16, int head_dim) {
+constexpr int score_tile_blocks_per_cu(int tile_rows, int waves, bool f16, int head_dim) {
+  if (waves == 8) return 1;
   if (tile_rows == 64) return f16 || head_dim <= 64 ? 2 : 1;
   return head_dim <= 128 ? 2 : 1;
 }
-
-constexpr int score_blocks_per_cu(int tile_rows, bool f16, int head_dim) {
-  return tile_rows == 16 ? score_stream_blocks_per_cu(f16, head_dim) : score_tile_blocks_per_cu(tile_rows, f16, head_dim);
+constexpr int score_tile_waves_per_simd(int tile_rows, int waves, bool f16, int head_dim) {
+  return waves / 4 * score_tile_blocks_per_cu(tile_rows, waves, f16, head_dim);
 }
 
-// Blocks of one launch: (request, KV head) pairs by eights, so that a pair's blocks run on
-// one XCD.
-inline unsigned score_blocks(const ScoreAttentionPlan& plan, const ScoreAttentionParams& p) {
-  const int64_t eights = ((int64_t)p.t.num_seqs * p.t.num_kv_heads + kScoreXcds - 1) / kScoreXcds;
-  return (unsigned)(eights * kScoreXcds * plan.row_tiles * plan.parts);
+constexpr int score_blocks_per_cu(int tile_rows, int waves, bool f16, int head_dim) {
+  return tile_rows == 16 ? score_stream_blocks_per_cu(f16, head_dim)
+                         : score_tile_blocks_per_cu(tile_rows, waves, f16, head_dim);
+}
+
+// Items that follow each other on one XCD: a pair's, where the pairs share out evenly;
+// else fewer, for some eight runs on each.
+inline int score_run(const ScoreAttentionPlan& plan, int64_t pairs) {
+  const int64_t inner = (int64_t)plan.row_tiles * plan.parts;
+  return (int)(pairs % kScoreXcds == 0 ? inner : std::max<int64_t>(1, std::min(inner, pairs * inner / (8 * kScoreXcds))));
+}
+
+// Blocks of one launch.
+inline unsigned score_blocks(const ScoreAttentionParams& p) {
+  const int64_t items = (int64_t)p.t.num_seqs * p.t.num_kv_heads * p.row_tiles * p.parts;
+  const int64_t round = (int64_t)kScoreXcds * p.run; // whole rounds of runs
+  return (unsigned)((items + round - 1) / round * round);
 }
 
 // score_tiles.hip: the attention itself, of row tiles of 64 (head_dim up to 128) and 128

@@ -97,30 +97,18 @@ __device__ __forceinline__ void add_row(KeyRange& k, const ScoreRow& row) {
 
 __device__ __forceinline__ KeyRange no_rows() { return {INT32_MAX, 0, 0, INT32_MAX}; }
 
-// Over the query rows of 16 lanes (the other groups of 16 hold the same ones); nothing
+// Over the query rows of 16 lanes, or of 32 (the other lanes hold the same ones); nothing
 // seen: begin = end = 0.
-__device__ __forceinline__ KeyRange row_tile_range(const KeyRange& mine) {
+template <int kLanes>
+__device__ __forceinline__ KeyRange rows_range(const KeyRange& mine) {
   auto least = [](int a, int b) { return min(a, b); };
   auto most = [](int a, int b) { return max(a, b); };
-  auto first = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-  KeyRange k = {first(row16_reduce(mine.begin, least)), first(row16_reduce(mine.end, most)),
-                first(row16_reduce(mine.all_begin, most)), first(row16_reduce(mine.all_end, least))};
-  if (k.end == 0) k.begin = 0;
-  return k;
-}
-
-// Over all lanes' rows.
-__device__ __forceinline__ KeyRange wave_range(const KeyRange& mine) {
-  KeyRange k = mine;
-#pragma unroll
-  for (int x = 32; x; x >>= 1) {
-    k.begin = min(k.begin, __shfl_xor(k.begin, x));
-    k.end = max(k.end, __shfl_xor(k.end, x));
-    k.all_begin = max(k.all_begin, __shfl_xor(k.all_begin, x));
-    k.all_end = min(k.all_end, __shfl_xor(k.all_end, x));
-  }
-  auto first = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-  k = {first(k.begin), first(k.end), first(k.all_begin), first(k.all_end)};
+  auto over = [](int v, auto op) {
+    v = row16_reduce(v, op);
+    const int first = __builtin_amdgcn_readfirstlane(v);
+    return kLanes == 16 ? first : op(first, __builtin_amdgcn_readlane(v, 16));
+  };
+  KeyRange k = {over(mine.begin, least), over(mine.end, most), over(mine.all_begin, most), over(mine.all_end, least)};
   if (k.end == 0) k.begin = 0;
   return k;
 }
@@ -191,18 +179,27 @@ __device__ __forceinline__ void to_masked_scores(const ScoreRules& r, const Scor
 
 constexpr int kScoreWaves = 4; // wavefronts per block
 
-// A block's item: part `part` of row tile rt of (request, KV head) pair.  The parts and
-// row tiles of one pair, which read the same keys, run on one XCD (workgroups are dealt
-// to the 8 XCDs round-robin); the last row tiles, which a causal mask leaves the most
-// keys, start first.
+// A block's item: part `part` of row tile rt of (request, KV head) pair.  Items are
+// numbered pair by pair, within a pair the last row tiles first, which a causal mask leaves
+// the most keys.  Runs of p.run items go to one XCD (workgroups are dealt to the 8 XCDs
+// round-robin): neighbours read the same keys, through one L2.  Every other round deals
+// them backwards, so that no XCD gets the longer run of each round.
 struct ScoreItem {
   int pair, rt, part;
 };
 
 __device__ __forceinline__ ScoreItem block_item(const ScoreAttentionParams& p) {
-  const uint32_t of_xcd = blockIdx.x / kScoreXcds, inner = (uint32_t)(p.row_tiles * p.parts);
-  const uint32_t eight = of_xcd / inner, rest = of_xcd - eight * inner, rt = rest / (uint32_t)p.parts;
-  return {(int)(eight * kScoreXcds + blockIdx.x % kScoreXcds), p.row_tiles - 1 - (int)rt, (int)(rest - rt * p.parts)};
+  const uint32_t xcd = blockIdx.x % kScoreXcds, of_xcd = blockIdx.x / kScoreXcds, run = (uint32_t)p.run;
+  const uint32_t round = of_xcd / run, turn = round % 2 ? kScoreXcds - 1 - xcd : xcd;
+  const uint32_t item = (round * kScoreXcds + turn) * run + (of_xcd - round * run);
+  const uint32_t inner = (uint32_t)(p.row_tiles * p.parts);
+  const uint32_t pair = item / inner, rest = item - pair * inner, rt = rest / (uint32_t)p.parts;
+  return {(int)pair, p.row_tiles - 1 - (int)rt, (int)(rest - rt * p.parts)};
+}
+
+// First unit of part `part` (of `parts`, 64 at most) of `units`.
+__device__ __forceinline__ int part_begin(int part, int units, int parts) {
+  return (int)((uint32_t)part * (uint32_t)units / (uint32_t)parts);
 }
 
 __device__ __forceinline__ int units_of(const KeyRange& k) {

@@ -47,8 +47,12 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
   __shared__ int found[2]; // digit, keys above it
   __shared__ uint32_t keys[HELD ? kHeldKeys : 1];
   const int tid = threadIdx.x, l = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int row = blockIdx.x;
-  const int table = row / p.num_kv_heads, h = row - table * p.num_kv_heads, b = table % p.num_seqs;
+  // The KV heads of one table follow each other on one XCD (workgroups are dealt to the 8
+  // XCDs round-robin): their weights share cache lines.
+  const unsigned of_xcd = blockIdx.x / 8, eight = of_xcd / (unsigned)p.num_kv_heads;
+  const int table = (int)(eight * 8 + blockIdx.x % 8), h = (int)(of_xcd - eight * p.num_kv_heads);
+  if (table >= p.num_layers * p.num_seqs) return;
+  const int row = table * p.num_kv_heads + h, b = table % p.num_seqs;
   const const_i32* lens = (const const_i32*)p.seq_lens;
   const int n = max(0, min(lens[b], p.max_seq_len));
   const int next = p.next_positions ? ((const const_i32*)p.next_positions)[b] : n;
@@ -141,9 +145,8 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
     if (l == kWave - 1) wave_counts[wave][0] = incl;
     bins[top] = bins[top - 1] = 0; // (for the next digit)
     __syncthreads();
-    int above = incl - c0 - c1;
-#pragma unroll 1
-    for (int w = 0; w < wave; w++) above += wave_counts[w][0];
+    const int before = wave_inclusive_sum(l < kSelectWaves ? wave_counts[l][0] : 0); // lane l: wavefronts 0 .. l's
+    const int above = incl - c0 - c1 + (wave ? __builtin_amdgcn_readlane(before, max(wave - 1, 0)) : 0);
     if (above < missing && above + c0 >= missing) {
       found[0] = top;
       found[1] = above;
@@ -178,29 +181,26 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
     wave_counts[wave][3] = movers;
   }
   __syncthreads();
-  // The runs before it: of a run's tokens at T the first ones stay, which are those below
-  // `keep` first.
-  int before = 0, all = 0, my_hole = 0, my_mover = 0, all_movers = 0, my_before = 0;
-#pragma unroll 1
-  for (int w = 0; w < kSelectWaves; w++) {
-    if (w == wave) {
-      my_hole = all;
-      my_mover = all_movers;
-      my_before = before;
-    }
-    const int at = wave_counts[w][0], low = wave_counts[w][1], stay = max(0, min(missing - before, at));
-    all += wave_counts[w][2] + low - min(low, stay);
-    all_movers += wave_counts[w][3] + max(0, stay - low);
-    before += at;
-  }
+  // The runs before it (lane l: run l): of a run's tokens at T the first ones stay, which
+  // are those below `keep` first.
+  const bool is_run = l < kSelectWaves;
+  const int at = is_run ? wave_counts[l][0] : 0, low = is_run ? wave_counts[l][1] : 0;
+  const int ties_before = wave_inclusive_sum(at) - at, stay = max(0, min(missing - ties_before, at));
+  const int goes_in = is_run ? wave_counts[l][2] + low - min(low, stay) : 0;
+  const int comes_from = is_run ? wave_counts[l][3] + max(0, stay - low) : 0;
+  const int holes_upto = wave_inclusive_sum(goes_in), movers_upto = wave_inclusive_sum(comes_from);
+  int my_before = __builtin_amdgcn_readlane(ties_before, wave);
+  int my_hole = __builtin_amdgcn_readlane(holes_upto - goes_in, wave);
+  int my_mover = __builtin_amdgcn_readlane(movers_upto - comes_from, wave);
+  const int all = __builtin_amdgcn_readlane(holes_upto, kSelectWaves - 1);
   if (tid == 0) *count = all;
   int32_t* const moves = p.moves + (int64_t)row * p.max_moves * 2;
   for (int t = t0; t < t1; t += kWave) {
     const bool in = t + l < t1;
     const uint32_t key = in ? key_of(t + l) : 0;
     const uint64_t tie = __ballot(in && key == prefix);
-    const bool stay = key > prefix || (key == prefix && my_before + (int)__popcll(tie & lower) < missing);
-    const bool hole = in && t + l < keep && !stay, mover = in && t + l >= keep && stay;
+    const bool stays = key > prefix || (key == prefix && my_before + (int)__popcll(tie & lower) < missing);
+    const bool hole = in && t + l < keep && !stays, mover = in && t + l >= keep && stays;
     const uint64_t hole_lanes = __ballot(hole), mover_lanes = __ballot(mover);
     if (hole) moves[2 * (int64_t)(my_hole + (int)__popcll(hole_lanes & lower)) + 1] = t + l;
     if (mover) moves[2 * (int64_t)(my_mover + (int)__popcll(mover_lanes & lower))] = t + l;
@@ -282,8 +282,8 @@ __global__ __launch_bounds__(kMoveThreads) void move_tokens_kernel(MoveTokensPar
 } // namespace
 
 hipError_t launch_select_tokens(const SelectTokensParams& params, hipStream_t stream) {
-  const int64_t rows = (int64_t)params.num_layers * params.num_seqs * params.num_kv_heads;
-  const dim3 grid((unsigned)rows), block(kSelectThreads);
+  const int64_t eights = ((int64_t)params.num_layers * params.num_seqs + 7) / 8;
+  const dim3 grid((unsigned)(eights * 8 * params.num_kv_heads)), block(kSelectThreads);
   if (params.max_seq_len <= kHeldKeys)
     hipLaunchKernelGGL(select_tokens_kernel<true>, grid, block, 0, stream, params);
   else

@@ -24,11 +24,11 @@
 namespace mvr {
 namespace {
 
-// S: LDS stages; S - 1 steps' loads are in flight while a step is computed.
-template <int D, typename T, int RW, int PAGES, int S>
-__global__ __launch_bounds__(kWaveSize* kTileWaves, (score_tile_blocks_per_cu(32 * RW, sizeof(T) == 2, D))) void score_tile_kernel(
+// W: wavefronts.  S: LDS stages; S - 1 steps' loads are in flight while a step is computed.
+template <int D, typename T, int RW, int W, int PAGES, int S>
+__global__ __launch_bounds__(kWaveSize* W, (score_tile_waves_per_simd(32 * RW, W, sizeof(T) == 2, D))) void score_tile_kernel(
     ScoreAttentionParams p) {
-  typedef Tile<D, T, RW> TL;
+  typedef Tile<D, T, RW, W> TL;
   constexpr bool kF32 = TL::kF32;
   constexpr int kTileTokens = TL::kTileTokens, kSub = TL::kSub, G = TL::kGroups;
   constexpr int kTileRows = 32 * RW;
@@ -41,7 +41,7 @@ __global__ __launch_bounds__(kWaveSize* kTileWaves, (score_tile_blocks_per_cu(32
   __shared__ __attribute__((aligned(16))) T v_lds0[TL::kElems], v_lds1[TL::kElems], v_lds2[TL::kElems],
       v_lds3[TL::kElems];
   __shared__ float ml_xfer[RW][2][64]; // hand-off between groups (O goes through the stages)
-  __shared__ __attribute__((aligned(16))) int non_finite[S][kTileWaves]; // by stage: what each wavefront loaded holds any
+  __shared__ __attribute__((aligned(16))) int non_finite[S][W]; // by stage: what each wavefront loaded holds any
   static_assert(S >= 2 && S <= 4, "2, 3 or 4 stages");
   T* const k_st[4] = {k_lds0, k_lds1, k_lds2, k_lds3};
   T* const v_st[4] = {v_lds0, v_lds1, v_lds2, v_lds3};
@@ -69,8 +69,7 @@ __global__ __launch_bounds__(kWaveSize* kTileWaves, (score_tile_blocks_per_cu(32
   ScoreRow row;
   // Q^T as the B operand: lane l holds row l % 32, dims 16 st + 8 hh .. + 8 (F32: 8 st + 4 hh .. + 4).
   qfrag_t q[kQFrags];
-  // What the wavefront's rows see, and the block's.
-  KeyRange mine = no_rows(), range = no_rows();
+  KeyRange mine = no_rows(); // what the wavefront's rows see
   {
     int token, head;
     const bool valid = row_at(rho0 + (l & 31), token, head);
@@ -82,13 +81,23 @@ __global__ __launch_bounds__(kWaveSize* kTileWaves, (score_tile_blocks_per_cu(32
     row = score_row(t, p.r, s, b, head, token);
     if (valid) add_row(mine, row);
   }
-  mine = wave_range(mine);
-#pragma unroll
-  for (int r0 = 0; r0 < kTileRows; r0 += kWaveSize) {
-    int ti, th;
-    if (row_at(it.rt * kTileRows + r0 + l, ti, th)) add_row(range, score_row(t, p.r, s, b, th, ti));
+  mine = rows_range<32>(mine);
+  // And the block's.
+  __shared__ int ranges[RW][4];
+  if (grp == 0 && l == 0) {
+    ranges[rw][0] = mine.end ? mine.begin : INT32_MAX;
+    ranges[rw][1] = mine.end;
+    ranges[rw][2] = mine.all_begin;
+    ranges[rw][3] = mine.all_end;
   }
-  range = wave_range(range);
+  __syncthreads();
+  KeyRange range = no_rows();
+#pragma unroll
+  for (int w = 0; w < RW; w++)
+    range = {min(range.begin, ranges[w][0]), max(range.end, ranges[w][1]), max(range.all_begin, ranges[w][2]),
+             min(range.all_end, ranges[w][3])};
+  auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  range = {uniform(range.end ? range.begin : 0), uniform(range.end), uniform(range.all_begin), uniform(range.all_end)};
 
   // The part's key tiles [j0, j1).
   const int units = units_of(range), unit0 = range.begin / kScoreUnitTokens;
@@ -98,8 +107,8 @@ __global__ __launch_bounds__(kWaveSize* kTileWaves, (score_tile_blocks_per_cu(32
   if (p.parts > 1 && it.part == 0 && threadIdx.x == 0) p.tile_parts[tile] = parts;
   constexpr int kUnitTiles = kScoreUnitTokens / kTileTokens;
   const int n_tiles = (range.end + kTileTokens - 1) / kTileTokens;
-  const int j0 = kUnitTiles * (unit0 + (int)((int64_t)it.part * units / parts));
-  const int j1 = min(kUnitTiles * (unit0 + (int)((int64_t)(it.part + 1) * units / parts)), n_tiles);
+  const int j0 = kUnitTiles * (unit0 + part_begin(it.part, units, parts));
+  const int j1 = min(kUnitTiles * (unit0 + part_begin(it.part + 1, units, parts)), n_tiles);
 
   float16v o[D / 32];
 #pragma unroll
@@ -320,7 +329,7 @@ __global__ __launch_bounds__(kWaveSize* kTileWaves, (score_tile_blocks_per_cu(32
   // rows that see them one by one, and cleared before the product.
   auto clear_non_finite = [&](T* vb) __attribute__((always_inline)) {
 #pragma unroll 1
-    for (int c = wave; c < TL::kElems / TL::kChunkElems / 64; c += kTileWaves) {
+    for (int c = wave; c < TL::kElems / TL::kChunkElems / 64; c += W) {
       qfrag_t* at = reinterpret_cast<qfrag_t*>(vb + (c * 64 + l) * TL::kChunkElems);
       qfrag_t x = *at;
 #pragma unroll
@@ -406,7 +415,8 @@ __global__ __launch_bounds__(kWaveSize* kTileWaves, (score_tile_blocks_per_cu(32
     issue_stage(min(si + S - 1, last_step), next_pages, k_st[into], v_st[into]);
     const int j = j0 + G * si + grp, first = j * kTileTokens;
     const bool works = j < j1 && first < mine.end && first + kTileTokens > mine.begin;
-    const int4v flags = *reinterpret_cast<const int4v*>(non_finite[st]);
+    int4v flags = *reinterpret_cast<const int4v*>(non_finite[st]);
+    if constexpr (W == 8) flags |= *reinterpret_cast<const int4v*>(non_finite[st] + 4);
     const bool bad = __builtin_amdgcn_readfirstlane(flags[0] | flags[1] | flags[2] | flags[3]);
     float16v sc[kSub];
     if (works) {
@@ -525,47 +535,50 @@ __global__ __launch_bounds__(kWaveSize* kTileWaves, (score_tile_blocks_per_cu(32
   }
 }
 
-template <int D, typename T, int RW>
+template <int D, typename T, int RW, int W>
 constexpr int stage_bytes() { // of K and V
-  return 2 * Tile<D, T, RW>::kElems * (int)sizeof(T);
+  return 2 * Tile<D, T, RW, W>::kElems * (int)sizeof(T);
 }
 
-template <int D, typename T, int RW, int S>
+template <int D, typename T, int RW, int W, int S>
 hipError_t launch_stages(const ScoreAttentionPlan& plan, const ScoreAttentionParams& p, hipStream_t stream) {
-  typedef Tile<D, T, RW> TL;
-  const dim3 grid(score_blocks(plan, p)), block(kWaveSize * kTileWaves);
+  typedef Tile<D, T, RW, W> TL;
+  const dim3 grid(score_blocks(p)), block(kWaveSize * W);
   if (p.t.page_size % kChunkTokens == 0) { // a wavefront's 8 or 16 tokens lie in one page
-    hipLaunchKernelGGL((score_tile_kernel<D, T, RW, kRuns, S>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((score_tile_kernel<D, T, RW, W, kRuns, S>), grid, block, 0, stream, p);
     return hipGetLastError();
   }
   if constexpr (D == 64 || D == 128) {
     if (p.t.page_size % (64 / TL::kChunksPerRow) == 0) {
-      hipLaunchKernelGGL((score_tile_kernel<D, T, RW, kWholeLoads, S>), grid, block, 0, stream, p);
+      hipLaunchKernelGGL((score_tile_kernel<D, T, RW, W, kWholeLoads, S>), grid, block, 0, stream, p);
       return hipGetLastError();
     }
   }
   // (Its loads are waited for as a whole: two stages.)
-  hipLaunchKernelGGL((score_tile_kernel<D, T, RW, kAnyPages, 2>), grid, block, 0, stream, p);
+  hipLaunchKernelGGL((score_tile_kernel<D, T, RW, W, kAnyPages, 2>), grid, block, 0, stream, p);
   return hipGetLastError();
 }
 
 // Stages: as many as two blocks per CU leave room for, 4 at most (2 at head_dim 128).
-template <int D, typename T, int RW>
+template <int D, typename T, int RW, int W>
 hipError_t launch_rows(const ScoreAttentionPlan& plan, const ScoreAttentionParams& p, hipStream_t stream) {
-  constexpr int kBytes = stage_bytes<D, T, RW>();
+  constexpr int kBytes = stage_bytes<D, T, RW, W>() * kTileWaves / W;
   constexpr int kStages = 78 * 1024 / kBytes >= 4 ? 4 : 78 * 1024 / kBytes >= 3 ? 3 : 2;
-  return launch_stages<D, T, RW, kStages>(plan, p, stream);
+  return launch_stages<D, T, RW, W, kStages>(plan, p, stream);
+}
+
+template <int D, typename T>
+hipError_t launch_type(const ScoreAttentionPlan& plan, const ScoreAttentionParams& p, hipStream_t stream) {
+  if constexpr (D <= 128) {
+    if (plan.tile_rows == 64) return launch_rows<D, T, 2, 4>(plan, p, stream);
+    if (plan.waves == 8) return launch_rows<D, T, 4, 8>(plan, p, stream);
+  }
+  return launch_rows<D, T, 4, 4>(plan, p, stream);
 }
 
 template <int D>
 hipError_t launch_dim(const ScoreAttentionPlan& plan, const ScoreAttentionParams& p, int dtype, hipStream_t stream) {
-  if (plan.tile_rows == 128)
-    return dtype == 1 ? launch_rows<D, half_t, 4>(plan, p, stream) : launch_rows<D, float, 4>(plan, p, stream);
-  if constexpr (D <= 128) {
-    if (plan.tile_rows == 64)
-      return dtype == 1 ? launch_rows<D, half_t, 2>(plan, p, stream) : launch_rows<D, float, 2>(plan, p, stream);
-  }
-  return hipErrorInvalidValue;
+  return dtype == 1 ? launch_type<D, half_t>(plan, p, stream) : launch_type<D, float>(plan, p, stream);
 }
 
 } // namespace

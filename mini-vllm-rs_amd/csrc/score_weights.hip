@@ -105,7 +105,7 @@ __global__ __launch_bounds__(kWaveSize* kWaves, (weights_waves<typename Tr::elem
     const float lse_log2 = r.lse * 1.4426950408889634f;
     KeyRange range = no_rows();
     add_row(range, r.row);
-    range = row_tile_range(range);
+    range = rows_range<16>(range);
     if (range.end <= key0 || range.begin >= key0 + kUnit) continue;
     const bool masked = range.all_begin > key0 || range.all_end < key0 + kUnit;
     float x[4 * kChunks];
