@@ -486,8 +486,12 @@ int mvr_attention_weights(const mvr_paged_attention_args* a, const mvr_score_rul
   p.weights = w->weights;
   p.decay = w->decay;
   p.fresh_from = w->fresh_from;
+  // Where the keys give the SIMDs less than a wavefront each, a block's wavefronts share
+  // its keys and split the rows (four prompts of 1,500 tokens, 32 rows of ... each).
+  const int64_t unit = mvr::weights_unit_tokens(es_of(a->dtype), a->head_dim);
+  const int64_t units = (int64_t)a->num_seqs * a->num_kv_heads * ((a->max_seq_len + unit - 1) / unit);
   const int64_t rows = (int64_t)(a->num_q_heads / a->num_kv_heads) * a->max_q_len;
-  const bool split = rows > 64;
+  const bool split = rows > 32 && units < 4 * (int64_t)compute_units();
   return launch_status(mvr::launch_score_weights(p, a->dtype, a->head_dim, split, static_cast<hipStream_t>(a->stream)));
 }
 

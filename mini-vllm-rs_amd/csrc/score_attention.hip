@@ -62,7 +62,7 @@ __global__ __launch_bounds__(kWaveSize* kScoreWaves, (score_stream_blocks_per_cu
   typename Tr::qreg_t q[Tr::kQRegs];
   Tr::load_q(static_cast<const T*>(t.q) + (int64_t)head * t.q_stride_head + (int64_t)(s.q_start + i) * t.q_stride_token,
              valid, g, q);
-  const ScoreRow row = score_row(t, p.r, s, b, head, i);
+  const ScoreRow row = score_row(p.r, s, prefix_of(p.r, b), head, i);
   KeyRange range = no_rows();
   if (valid) add_row(range, row);
   range = rows_range<16>(range);

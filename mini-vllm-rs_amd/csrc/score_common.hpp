@@ -41,12 +41,15 @@ struct ScoreRow {
   float slope_log2;
 };
 
-__device__ __forceinline__ ScoreRow score_row(const ScoreTables& t, const ScoreRules& r, const ScoreSeq& s, int b,
-                                              int q_head, int i) {
+// prefix: of the request, 0 for none (prefix_of).
+__device__ __forceinline__ int prefix_of(const ScoreRules& r, int b) {
+  return r.prefix_lens ? ((const const_i32*)r.prefix_lens)[b] : 0;
+}
+
+__device__ __forceinline__ ScoreRow score_row(const ScoreRules& r, const ScoreSeq& s, int prefix, int q_head, int i) {
   ScoreRow row;
   row.pos = s.seq_len - s.q_len + i;
-  int hi = row.pos + 1, lo = 0;
-  if (r.prefix_lens) hi = max(hi, r.prefix_lens[b]);
+  int hi = max(row.pos + 1, prefix), lo = 0;
   if (r.first_keys) lo = max(lo, r.first_keys[s.q_start + i]);
   if (r.window > 0) lo = max(lo, row.pos - (r.window - 1));
   hi = min(hi, s.seq_len);

@@ -26,13 +26,19 @@ constexpr int kWave = 64;
 // order.
 //
 // Bound by the block's own chain of steps, not by the bytes: the weights are read once,
-// and their keys held in LDS for the passes over them.
+// and their keys held in LDS for the passes over them.  A thread takes four slots at a
+// time, one 16-byte access each to weights, positions and keys where pages hold whole
+// fours (VEC).
 // ---------------------------------------------------------------------------
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / kWave;
 constexpr int kDigitBits = 11, kDigits = 3, kBins = 1 << kDigitBits;
+constexpr int kFour = 4; // slots of a thread at a time
 // Keys that LDS holds: two blocks to a CU beside the histograms.  Requests that may be
 // longer read weights and positions anew in each pass.
 constexpr int kHeldKeys = 17408;
+
+typedef int int4v __attribute__((ext_vector_type(4)));
+typedef float float4v __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ uint32_t ascending(float w) {
   const uint32_t x = __float_as_uint(w);
@@ -40,12 +46,12 @@ __device__ __forceinline__ uint32_t ascending(float w) {
   return w == 0.f ? 0x80000000u : x >> 31 ? ~x : x | 0x80000000u;
 }
 
-template <bool HELD>
+template <bool HELD, bool VEC>
 __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(SelectTokensParams p) {
   __shared__ int bins[kBins];
   __shared__ int wave_counts[kSelectWaves][4];
   __shared__ int found[2]; // digit, keys above it
-  __shared__ uint32_t keys[HELD ? kHeldKeys : 1];
+  __shared__ __attribute__((aligned(16))) uint32_t held[HELD ? kHeldKeys : kFour];
   const int tid = threadIdx.x, l = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   // The KV heads of one table follow each other on one XCD (workgroups are dealt to the 8
   // XCDs round-robin): their weights share cache lines.
@@ -61,6 +67,8 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
   if (min(keep, n - keep) > p.max_moves) keep = n; // (its moves might not fit)
   if (table < p.num_seqs && h == 0 && tid == 0 && p.new_seq_lens) p.new_seq_lens[b] = keep;
   const bool cut = keep != n && keep != 0; // (else nothing goes, or nothing stays)
+  int32_t* const count = p.num_moves + row;
+  if (!cut && tid == 0) *count = 0;
 
   const int32_t* bt = p.block_tables + (int64_t)table * p.block_table_stride;
   // Index of slot t in the pools, or -1.
@@ -70,50 +78,67 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
     if (page < 0 || page >= p.num_pages) return -1;
     return (page * p.num_kv_heads + h) * p.page_size + (t - pi * p.page_size);
   };
-  auto key_at = [&](int pos, float w) { return pos < p.first || pos >= (int64_t)next - p.recent ? ~0u : ascending(w); };
-  // (Of slots in pages outside the pool: the lowest key.)
-  auto read_key = [&](int t) -> uint32_t {
-    const int64_t at = index_of(t);
-    return at < 0 ? 0 : key_at(t >= kept ? next - (n - t) : p.positions[at], p.weights[at]);
-  };
-  auto key_of = [&](int t) -> uint32_t {
-    if constexpr (HELD)
-      return keys[t];
-    else
-      return read_key(t);
-  };
-  for (int i = tid; i < kBins; i += kSelectThreads) bins[i] = 0;
-  // Positions of what was appended since the last cut; the keys.  A thread's page entries,
-  // then its weights and positions, are on their way together.
-  constexpr int kAhead = 4;
-  for (int t0 = HELD && cut ? tid : max(kept, 0) + tid; t0 < n; t0 += kAhead * kSelectThreads) {
-    int64_t at[kAhead];
-    float w[kAhead];
-    int pos[kAhead];
+  // Keys of slots t .. t + 3 (0 past the last one, and in pages outside the pool), and
+  // where `writes` is set the positions of those that were appended since the last cut.
+  auto read_four = [&](int t, bool writes, uint32_t (&key)[kFour]) {
+    int64_t at[kFour];
+    float w[kFour];
+    int pos[kFour];
+    if constexpr (VEC) {
+      const int64_t first = index_of(t), some = max(first, (int64_t)0);
+      const float4v w4 = *reinterpret_cast<const float4v*>(p.weights + some);
+      const int4v pos4 = *reinterpret_cast<const int4v*>(p.positions + some);
 #pragma unroll
-    for (int u = 0; u < kAhead; u++) at[u] = index_of(min(t0 + u * kSelectThreads, n - 1));
-    if (HELD && cut) {
+      for (int j = 0; j < kFour; j++) {
+        at[j] = first < 0 ? -1 : first + j;
+        w[j] = w4[j];
+        pos[j] = pos4[j];
+      }
+    } else {
 #pragma unroll
-      for (int u = 0; u < kAhead; u++) {
-        const int64_t some = max(at[u], (int64_t)0);
-        w[u] = p.weights[some];
-        pos[u] = p.positions[some];
+      for (int j = 0; j < kFour; j++) at[j] = index_of(min(t + j, n - 1));
+#pragma unroll
+      for (int j = 0; j < kFour; j++) {
+        const int64_t some = max(at[j], (int64_t)0);
+        w[j] = p.weights[some];
+        pos[j] = p.positions[some];
       }
     }
+    int4v fresh;
+    bool all = at[0] >= 0 && t + kFour <= n;
 #pragma unroll
-    for (int u = 0; u < kAhead; u++) {
-      const int t = t0 + u * kSelectThreads;
-      if (t >= n) break;
-      const int fresh = next - (n - t);
-      if (HELD && cut) keys[t] = at[u] < 0 ? 0 : key_at(t >= kept ? fresh : pos[u], w[u]);
-      if (t >= kept && at[u] >= 0) p.positions[at[u]] = fresh;
+    for (int j = 0; j < kFour; j++) {
+      fresh[j] = next - (n - (t + j));
+      all &= t + j >= kept;
+      if (t + j >= kept) pos[j] = fresh[j];
+      const bool guarded = pos[j] < p.first || pos[j] >= (int64_t)next - p.recent;
+      key[j] = t + j >= n || at[j] < 0 ? 0 : guarded ? ~0u : ascending(w[j]);
     }
+    if (!writes) return;
+    if (VEC && all) {
+      *reinterpret_cast<int4v*>(p.positions + at[0]) = fresh;
+    } else {
+#pragma unroll
+      for (int j = 0; j < kFour; j++)
+        if (t + j < n && t + j >= kept && at[j] >= 0) p.positions[at[j]] = fresh[j];
+    }
+  };
+  auto keys_of = [&](int t, uint32_t (&key)[kFour]) {
+    if constexpr (HELD) {
+      const int4v x = *reinterpret_cast<const int4v*>(held + t);
+#pragma unroll
+      for (int j = 0; j < kFour; j++) key[j] = (uint32_t)x[j];
+    } else {
+      read_four(t, false, key);
+    }
+  };
+  for (int i = tid; i < kBins; i += kSelectThreads) bins[i] = 0;
+  for (int t = HELD && cut ? kFour * tid : max(kept, 0) / kFour * kFour + kFour * tid; t < n; t += kFour * kSelectThreads) {
+    uint32_t key[kFour];
+    read_four(t, true, key);
+    if (HELD && cut) *reinterpret_cast<int4v*>(held + t) = int4v{(int)key[0], (int)key[1], (int)key[2], (int)key[3]};
   }
-  int32_t* const count = p.num_moves + row;
-  if (!cut) {
-    if (tid == 0) *count = 0;
-    return;
-  }
+  if (!cut) return;
   __syncthreads();
 
   // The keep-th largest key.
@@ -121,21 +146,12 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
   int missing = keep;             // of the keys with those digits, the missing-th largest is T
   for (int digit = kDigits - 1; digit >= 0; digit--) {
     const int shift = digit * kDigitBits;
-    for (int t0 = wave * kWave; t0 < n; t0 += kSelectThreads) {
-      const int t = t0 + l;
-      const uint32_t key = t < n ? key_of(t) : 0;
-      const bool in = t < n && (key & known) == prefix;
-      const int bin = (int)((key >> shift) & (kBins - 1));
-      // (Lanes of one bin, as those of equal weights are, add up first: atomics on one
-      // address take their lanes in turn.)
-      const uint64_t lanes = __ballot(in);
-      if (lanes == 0) continue;
-      const int some = __builtin_amdgcn_readlane(bin, __builtin_ctzll(lanes));
-      if (__ballot(in && bin != some) == 0) {
-        if (l == 0) atomicAdd(&bins[some], (int)__popcll(lanes));
-      } else if (in) {
-        atomicAdd(&bins[bin], 1);
-      }
+    for (int t = kFour * tid; t < n; t += kFour * kSelectThreads) {
+      uint32_t key[kFour];
+      keys_of(t, key);
+#pragma unroll
+      for (int j = 0; j < kFour; j++)
+        if (t + j < n && (key[j] & known) == prefix) atomicAdd(&bins[(key[j] >> shift) & (kBins - 1)], 1);
     }
     __syncthreads();
     // Keys above each bin: a scan from the top, two bins per thread.
@@ -145,8 +161,8 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
     if (l == kWave - 1) wave_counts[wave][0] = incl;
     bins[top] = bins[top - 1] = 0; // (for the next digit)
     __syncthreads();
-    const int before = wave_inclusive_sum(l < kSelectWaves ? wave_counts[l][0] : 0); // lane l: wavefronts 0 .. l's
-    const int above = incl - c0 - c1 + (wave ? __builtin_amdgcn_readlane(before, max(wave - 1, 0)) : 0);
+    const int waves_upto = wave_inclusive_sum(l < kSelectWaves ? wave_counts[l][0] : 0); // lane l: wavefronts 0 .. l
+    const int above = incl - c0 - c1 + (wave ? __builtin_amdgcn_readlane(waves_upto, max(wave - 1, 0)) : 0);
     if (above < missing && above + c0 >= missing) {
       found[0] = top;
       found[1] = above;
@@ -162,19 +178,27 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
   // Tokens above T stay, and the first `missing` at T.  Each wavefront looks at a run of
   // slots of its own.  What its run holds: tokens at T, those of them below slot `keep`,
   // tokens below T in slots below `keep`, tokens above T in the others.
-  const int run = (n + kSelectThreads - 1) / kSelectThreads * kWave;
+  constexpr int kWaveSlots = kFour * kWave;
+  const int run = (n + kSelectWaves * kWaveSlots - 1) / (kSelectWaves * kWaveSlots) * kWaveSlots;
   const int t0 = min(wave * run, n), t1 = min(t0 + run, n);
-  const uint64_t lower = (1ull << l) - 1;
   int ties = 0, low_ties = 0, holes = 0, movers = 0;
-  for (int t = t0; t < t1; t += kWave) {
-    const bool in = t + l < t1, low = t + l < keep;
-    const uint32_t key = in ? key_of(t + l) : 0;
-    ties += (int)__popcll(__ballot(in && key == prefix));
-    low_ties += (int)__popcll(__ballot(in && key == prefix && low));
-    holes += (int)__popcll(__ballot(in && key < prefix && low));
-    movers += (int)__popcll(__ballot(in && key > prefix && !low));
+  for (int t = t0 + kFour * l; t < t1; t += kWaveSlots) {
+    uint32_t key[kFour];
+    keys_of(t, key);
+#pragma unroll
+    for (int j = 0; j < kFour; j++) {
+      const bool in = t + j < t1, low = t + j < keep, tie = in && key[j] == prefix;
+      ties += tie;
+      low_ties += tie && low;
+      holes += in && key[j] < prefix && low;
+      movers += in && key[j] > prefix && !low;
+    }
   }
-  if (l == 0) {
+  ties = wave_inclusive_sum(ties);
+  low_ties = wave_inclusive_sum(low_ties);
+  holes = wave_inclusive_sum(holes);
+  movers = wave_inclusive_sum(movers);
+  if (l == kWave - 1) {
     wave_counts[wave][0] = ties;
     wave_counts[wave][1] = low_ties;
     wave_counts[wave][2] = holes;
@@ -184,29 +208,50 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
   // The runs before it (lane l: run l): of a run's tokens at T the first ones stay, which
   // are those below `keep` first.
   const bool is_run = l < kSelectWaves;
-  const int at = is_run ? wave_counts[l][0] : 0, low = is_run ? wave_counts[l][1] : 0;
-  const int ties_before = wave_inclusive_sum(at) - at, stay = max(0, min(missing - ties_before, at));
+  const int at_t = is_run ? wave_counts[l][0] : 0, low = is_run ? wave_counts[l][1] : 0;
+  const int ties_before = wave_inclusive_sum(at_t) - at_t, stay = max(0, min(missing - ties_before, at_t));
   const int goes_in = is_run ? wave_counts[l][2] + low - min(low, stay) : 0;
   const int comes_from = is_run ? wave_counts[l][3] + max(0, stay - low) : 0;
   const int holes_upto = wave_inclusive_sum(goes_in), movers_upto = wave_inclusive_sum(comes_from);
-  int my_before = __builtin_amdgcn_readlane(ties_before, wave);
+  int my_ties = __builtin_amdgcn_readlane(ties_before, wave);
   int my_hole = __builtin_amdgcn_readlane(holes_upto - goes_in, wave);
   int my_mover = __builtin_amdgcn_readlane(movers_upto - comes_from, wave);
   const int all = __builtin_amdgcn_readlane(holes_upto, kSelectWaves - 1);
   if (tid == 0) *count = all;
   int32_t* const moves = p.moves + (int64_t)row * p.max_moves * 2;
-  for (int t = t0; t < t1; t += kWave) {
-    const bool in = t + l < t1;
-    const uint32_t key = in ? key_of(t + l) : 0;
-    const uint64_t tie = __ballot(in && key == prefix);
-    const bool stays = key > prefix || (key == prefix && my_before + (int)__popcll(tie & lower) < missing);
-    const bool hole = in && t + l < keep && !stays, mover = in && t + l >= keep && stays;
-    const uint64_t hole_lanes = __ballot(hole), mover_lanes = __ballot(mover);
-    if (hole) moves[2 * (int64_t)(my_hole + (int)__popcll(hole_lanes & lower)) + 1] = t + l;
-    if (mover) moves[2 * (int64_t)(my_mover + (int)__popcll(mover_lanes & lower))] = t + l;
-    my_hole += (int)__popcll(hole_lanes);
-    my_mover += (int)__popcll(mover_lanes);
-    my_before += (int)__popcll(tie);
+  for (int base = t0; base < t1; base += kWaveSlots) {
+    const int t = base + kFour * l;
+    uint32_t key[kFour] = {0, 0, 0, 0};
+    if (t < t1) keys_of(t, key);
+    int lane_ties = 0;
+#pragma unroll
+    for (int j = 0; j < kFour; j++) lane_ties += t + j < t1 && key[j] == prefix;
+    int before = 0; // tokens at T in the lanes before it
+    if (__any(lane_ties)) before = wave_inclusive_sum(lane_ties) - lane_ties;
+    int rank = my_ties + before, lane_holes = 0, lane_movers = 0;
+    bool hole[kFour], mover[kFour];
+#pragma unroll
+    for (int j = 0; j < kFour; j++) {
+      const bool in = t + j < t1, tie = key[j] == prefix;
+      const bool stays = key[j] > prefix || (tie && rank < missing);
+      rank += in && tie;
+      hole[j] = in && t + j < keep && !stays;
+      mover[j] = in && t + j >= keep && stays;
+      lane_holes += hole[j];
+      lane_movers += mover[j];
+    }
+    // (Both counts, 256 at most, in one scan.)
+    const int both = wave_inclusive_sum(lane_holes + (lane_movers << 16));
+    int to = my_hole + (both & 0xffff) - lane_holes, from = my_mover + (both >> 16) - lane_movers;
+#pragma unroll
+    for (int j = 0; j < kFour; j++) {
+      if (hole[j]) moves[2 * (int64_t)to++ + 1] = t + j;
+      if (mover[j]) moves[2 * (int64_t)from++] = t + j;
+    }
+    const int total = __builtin_amdgcn_readlane(both, kWave - 1);
+    my_hole += total & 0xffff;
+    my_mover += total >> 16;
+    my_ties += __builtin_amdgcn_readlane(before + lane_ties, kWave - 1);
   }
 }
 
@@ -284,10 +329,12 @@ __global__ __launch_bounds__(kMoveThreads) void move_tokens_kernel(MoveTokensPar
 hipError_t launch_select_tokens(const SelectTokensParams& params, hipStream_t stream) {
   const int64_t eights = ((int64_t)params.num_layers * params.num_seqs + 7) / 8;
   const dim3 grid((unsigned)(eights * 8 * params.num_kv_heads)), block(kSelectThreads);
+  const bool vec = params.page_size % kFour == 0 && ((uintptr_t)params.weights | (uintptr_t)params.positions) % 16 == 0;
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, params); };
   if (params.max_seq_len <= kHeldKeys)
-    hipLaunchKernelGGL(select_tokens_kernel<true>, grid, block, 0, stream, params);
+    vec ? launch(select_tokens_kernel<true, true>) : launch(select_tokens_kernel<true, false>);
   else
-    hipLaunchKernelGGL(select_tokens_kernel<false>, grid, block, 0, stream, params);
+    vec ? launch(select_tokens_kernel<false, true>) : launch(select_tokens_kernel<false, false>);
   return hipGetLastError();
 }
 

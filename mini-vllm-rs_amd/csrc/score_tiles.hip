@@ -78,7 +78,7 @@ __global__ __launch_bounds__(kWaveSize* W, (score_tile_waves_per_simd(32 * RW, W
 #pragma unroll
     for (int st = 0; st < kQFrags; st++)
       q[st] = valid ? *reinterpret_cast<const qfrag_t*>(qrow + kFragDims * st + (kFragDims / 2) * hh) : qfrag_t{};
-    row = score_row(t, p.r, s, b, head, token);
+    row = score_row(p.r, s, prefix_of(p.r, b), head, token);
     if (valid) add_row(mine, row);
   }
   mine = rows_range<32>(mine);

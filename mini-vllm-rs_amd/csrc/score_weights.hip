@@ -42,7 +42,7 @@ __global__ __launch_bounds__(kWaveSize* kWaves, (weights_waves<typename Tr::elem
   const int b = pair / t.num_kv_heads, h = pair - b * t.num_kv_heads;
   const ScoreSeq s = load_score_seq(t, b);
   if (key0 >= s.seq_len) return; // (SPLIT: the whole block)
-  const int rows = t.group_size * s.q_len;
+  const int rows = t.group_size * s.q_len, prefix = prefix_of(p.r, b);
 
   // Lane l holds the page entry of key key0 + l (lanes past the last key that key's).
   const int my_key = min(key0 + l % kUnit, s.seq_len - 1);
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(kWaveSize* kWaves, (weights_waves<typename Tr::elem
       token++;
     }
     r.lse = p.r.lse[(int64_t)head * p.r.lse_stride_head + s.q_start + i];
-    r.row = score_row(t, p.r, s, b, head, i);
+    r.row = score_row(p.r, s, prefix, head, i);
     Tr::load_q(static_cast<const T*>(t.q) + (int64_t)head * t.q_stride_head + (int64_t)(s.q_start + i) * t.q_stride_token,
                r.valid, g, r.q);
   };
@@ -103,11 +103,9 @@ __global__ __launch_bounds__(kWaveSize* kWaves, (weights_waves<typename Tr::elem
     if (rho0 + kRowStep < rows) load_rows(next);
     if (!r.valid || r.lse == -INFINITY) r.row.width = 0;
     const float lse_log2 = r.lse * 1.4426950408889634f;
-    KeyRange range = no_rows();
-    add_row(range, r.row);
-    range = rows_range<16>(range);
-    if (range.end <= key0 || range.begin >= key0 + kUnit) continue;
-    const bool masked = range.all_begin > key0 || range.all_end < key0 + kUnit;
+    const int end = r.row.lo + r.row.width;
+    if (!__any(r.row.width && end > key0 && r.row.lo < key0 + kUnit)) continue;
+    const bool masked = __any(end < key0 + kUnit || r.row.lo > key0); // some row does not see all the keys
     float x[4 * kChunks];
 #pragma unroll
     for (int c = 0; c < kChunks; c++) {
