@@ -134,62 +134,90 @@ int64_t units_of(int64_t tokens) { return (tokens + mvr::kScoreUnitTokens - 1) /
 
 // Row tiles of one size, as the planner sees them: by the host tables, or as if all
 // requests were alike.
-struct TileWork {
-  int64_t tiles = 0, units = 0; // row tiles; units of 64 keys over all of them
-  int64_t longest = 0;          // units of one
-
-  TileWork(const mvr_paged_attention_args* a, const mvr_score_rules* r, int tile_rows) {
-    const int64_t group = a->num_q_heads / a->num_kv_heads;
-    int64_t bound = INT64_MAX; // units that a window leaves a row tile
-    if (r->window > 0 && !r->prefix_lens) bound = units_of((int64_t)r->window + (tile_rows + group - 1) / group) + 1;
-    const int32_t *cu = a->cu_q_lens_host, *sl = a->seq_lens_host;
-    auto add = [&](int64_t q, int64_t keys, int64_t requests) {
-      const int64_t n = (group * q + tile_rows - 1) / tile_rows;
-      tiles += requests * n;
-      // (A causal mask leaves the request's queries half of its new tokens on average.)
-      units += requests * n * std::min(bound, units_of(std::max<int64_t>(keys - q / 2, 1)));
-      if (n) longest = std::max(longest, std::min(bound, units_of(keys)));
-    };
-    if (cu && sl) {
-      for (int s = 0; s < a->num_seqs; s++)
-        add(std::min<int64_t>(std::max<int64_t>(0, (int64_t)cu[s + 1] - cu[s]), a->max_q_len),
-            std::min(std::max(sl[s], 0), a->max_seq_len), 1);
-    } else {
-      add(a->max_q_len, a->sum_seq_lens > 0 ? (a->sum_seq_lens + a->num_seqs - 1) / a->num_seqs : a->max_seq_len,
-          a->num_seqs);
-    }
+class TileWork {
+ public:
+  TileWork(const mvr_paged_attention_args* a, const mvr_score_rules* r, int tile_rows)
+      : a_(a), group_(a->num_q_heads / a->num_kv_heads), rows_(tile_rows) {
+    if (r->window > 0 && !r->prefix_lens) bound_ = units_of((int64_t)r->window + (tile_rows + group_ - 1) / group_) + 1;
+    for_each([&](int64_t n, int64_t least, int64_t most) {
+      tiles += n;
+      units += n * (least + most) / 2;
+      if (n) longest = std::max(longest, most);
+    });
     tiles *= a->num_kv_heads;
     units *= a->num_kv_heads;
   }
+
+  // Blocks of a call that is split into parts of `part` units.
+  int64_t blocks(int64_t part) const {
+    // Parts of tiles of 1, 2, ... x units, together.
+    auto upto = [part](int64_t x) {
+      const int64_t k = x / part;
+      return part * k * (k + 1) / 2 + (x - k * part) * (k + 1);
+    };
+    int64_t count = 0;
+    for_each([&](int64_t n, int64_t least, int64_t most) {
+      count += (n * (upto(most) - upto(least - 1)) + most - least) / (most - least + 1);
+    });
+    return count * a_->num_kv_heads;
+  }
+
+  int64_t tiles = 0, units = 0; // row tiles; units of 64 keys over all of them
+  int64_t longest = 0;          // units of one
+
+ private:
+  // f(row tiles of a KV head, units that the first one's keys take, the last one's) for
+  // every request: a causal mask leaves the first token its past alone.
+  template <typename F>
+  void for_each(F f) const {
+    const int32_t *cu = a_->cu_q_lens_host, *sl = a_->seq_lens_host;
+    auto request = [&](int64_t q, int64_t keys, int64_t requests) {
+      f(requests * ((group_ * q + rows_ - 1) / rows_), std::min(bound_, units_of(std::max<int64_t>(keys - q + 1, 1))),
+        std::min(bound_, units_of(std::max<int64_t>(keys, 1))));
+    };
+    if (cu && sl) {
+      for (int s = 0; s < a_->num_seqs; s++)
+        request(std::min<int64_t>(std::max<int64_t>(0, (int64_t)cu[s + 1] - cu[s]), a_->max_q_len),
+                std::min(std::max(sl[s], 0), a_->max_seq_len), 1);
+    } else {
+      request(a_->max_q_len, a_->sum_seq_lens > 0 ? (a_->sum_seq_lens + a_->num_seqs - 1) / a_->num_seqs : a_->max_seq_len,
+              a_->num_seqs);
+    }
+  }
+
+  const mvr_paged_attention_args* a_;
+  int64_t group_, rows_, bound_ = INT64_MAX; // units that a window leaves a row tile
 };
 
 // What a block of one tile size costs, in us, for head_dim 128: `fixed` beside its keys,
-// `unit` per 64 keys with one to four blocks on its CU.
+// `unit` per 64 keys with one to four blocks on its CU, of which the share `own` does not
+// go by the head dimension; `capped` times that under a cap.  Fitted to 185 timed plans
+// (tile sizes and splits of 13 calls: 1 to 32 requests on 100 to 16,000 tokens, 1 to 2,000
+// new ones, head_dim 64 and 128), which they meet within 13 to 25% (root mean square).
 struct TileCost {
   int rows, waves;
-  double fixed, unit[4];
+  double fixed, unit[4], own, capped;
 };
 
-constexpr TileCost kF16Costs[] = {{16, 4, 6.3, {0.57, 1.17, 1.81, 2.48}},
-                                  {64, 4, 6.6, {1.02, 1.30, 1.30, 1.30}},
-                                  {128, 4, 8.0, {1.32, 1.62, 1.62, 1.62}},
-                                  {128, 8, 8.0, {0.95, 0.95, 0.95, 0.95}}};
-constexpr TileCost kF32Costs[] = {{16, 4, 2.5, {1.97, 4.05, 6.23, 8.55}},
-                                  {64, 4, 5.7, {4.73, 9.50, 9.50, 9.50}},
-                                  {128, 4, 6.6, {7.61, 14.8, 14.8, 14.8}},
-                                  {128, 8, 6.6, {7.5, 7.5, 7.5, 7.5}}};
+constexpr TileCost kF16Costs[] = {{16, 4, 3.0, {0.70, 1.45, 2.20, 3.00}, 0.85, 1.1},
+                                  {64, 4, 7.2, {0.97, 1.57, 1.57, 1.57}, 0.7, 1.3},
+                                  {128, 4, 6.5, {1.50, 1.53, 1.53, 1.53}, 0.5, 1.4},
+                                  {128, 8, 7.0, {0.97, 0.97, 0.97, 0.97}, 0.5, 1.45}};
+constexpr TileCost kF32Costs[] = {{16, 4, 3.3, {2.00, 4.20, 5.80, 6.90}, 0.0, 1.0},
+                                  {64, 4, 10.0, {5.50, 8.50, 8.50, 8.50}, 0.0, 1.0},
+                                  {128, 4, 12.0, {7.20, 14.3, 14.3, 14.3}, 0.0, 1.0},
+                                  {128, 8, 12.0, {7.50, 7.50, 7.50, 7.50}, 0.0, 1.0}};
 
 // The tile size and the split of its keys that these costs make fastest: every tile
 // whole, or in parts that give each CU one block, two, up to as many as it holds, or
 // two, three or four times that.  A call takes its blocks' time (all of them in one
 // round; in more rounds the average load and most of a last block), joined with the time
-// that its keys take from HBM (as a 3-norm).  A split call merges: a launch, and its
-// partial results written and read at 4.3 TB/s.
+// that its keys take from HBM (as a 3-norm).  A split call merges: a launch, a chain of
+// loads over a row's parts, and its partial results written and read at 4.3 TB/s.
 mvr::ScoreAttentionPlan plan_scored(const mvr_paged_attention_args* a, const mvr_score_rules* r, size_t limit) {
   const bool f16 = a->dtype == MVR_DTYPE_F16;
   const int64_t group = a->num_q_heads / a->num_kv_heads, longest_rows = group * a->max_q_len;
   const int64_t cus = compute_units(), pairs = (int64_t)a->num_seqs * a->num_kv_heads;
-  const double unit_scale = a->head_dim / 128.0;
   // Overrides, for tests and tuning: a tile size that the head dimension has, and its parts.
   static const int set_rows = env_int("MVR_SCORE_TILE_ROWS", 0);
   static const int set_waves = env_int("MVR_SCORE_TILE_WAVES", 4);
@@ -205,6 +233,7 @@ mvr::ScoreAttentionPlan plan_scored(const mvr_paged_attention_args* a, const mvr
     if (rows_set ? tile.rows != set_rows || tile.waves != set_waves : longest_rows <= tile.rows / 2 && best_cost < INFINITY) continue;
     const int held = mvr::score_blocks_per_cu(tile.rows, tile.waves, f16, a->head_dim);
     const TileWork w(a, r, tile.rows);
+    const double unit_scale = (tile.own + (1 - tile.own) * a->head_dim / 128.0) * (r->cap > 0.f ? tile.capped : 1.0);
     const int64_t row_tiles = (longest_rows + tile.rows - 1) / tile.rows, all_tiles = pairs * row_tiles;
     // (Row tiles of one KV head read the same keys, which the caches keep.)
     const double hbm = (double)w.units / std::max<int64_t>(1, row_tiles) *
@@ -237,10 +266,10 @@ mvr::ScoreAttentionPlan plan_scored(const mvr_paged_attention_args* a, const mvr
                            align_up((size_t)all_tiles * sizeof(int32_t), 256);
       if (bytes > limit) return;
       part = std::max(part, (w.longest + parts - 1) / parts);
-      const int64_t blocks = std::max(w.tiles, w.units / part + w.tiles / 2);
+      const int64_t blocks = w.blocks(part);
       // (The partials that are written: the others' slots are left alone.)
       const double moved = 2.0 * blocks * tile.rows * (a->head_dim + 2) * sizeof(float) / 4.3e6;
-      take(cost_of(blocks, part) + 4.5 + moved, parts, part, bytes);
+      take(cost_of(blocks, part) + 3.5 + 0.17 * parts + moved, parts, part, bytes);
     };
     take(cost_of(w.tiles, w.longest), 1, INT32_MAX, 0);
     if (w.tiles == 0 || w.longest < 2 || limit == 0) continue;

@@ -31,7 +31,7 @@ constexpr int kWave = 64;
 // fours (VEC).
 // ---------------------------------------------------------------------------
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / kWave;
-constexpr int kDigitBits = 11, kDigits = 3, kBins = 1 << kDigitBits;
+constexpr int kDigitBits = 11, kDigits = 3, kBins = 1 << kDigitBits, kThreadBins = kBins / kSelectThreads;
 constexpr int kFour = 4; // slots of a thread at a time
 // Keys that LDS holds: two blocks to a CU beside the histograms.  Requests that may be
 // longer read weights and positions anew in each pass.
@@ -154,21 +154,26 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
         if (t + j < n && (key[j] & known) == prefix) atomicAdd(&bins[(key[j] >> shift) & (kBins - 1)], 1);
     }
     __syncthreads();
-    // Keys above each bin: a scan from the top, two bins per thread.
-    const int top = kBins - 1 - 2 * tid;
-    const int c0 = bins[top], c1 = bins[top - 1];
-    const int incl = wave_inclusive_sum(c0 + c1);
+    // Keys above each bin: a scan from the top, kThreadBins bins per thread.
+    const int top = kBins - 1 - kThreadBins * tid;
+    int in_bin[kThreadBins], mine = 0;
+#pragma unroll
+    for (int i = 0; i < kThreadBins; i++) {
+      mine += in_bin[i] = bins[top - i];
+      bins[top - i] = 0; // (for the next digit)
+    }
+    const int incl = wave_inclusive_sum(mine);
     if (l == kWave - 1) wave_counts[wave][0] = incl;
-    bins[top] = bins[top - 1] = 0; // (for the next digit)
     __syncthreads();
     const int waves_upto = wave_inclusive_sum(l < kSelectWaves ? wave_counts[l][0] : 0); // lane l: wavefronts 0 .. l
-    const int above = incl - c0 - c1 + (wave ? __builtin_amdgcn_readlane(waves_upto, max(wave - 1, 0)) : 0);
-    if (above < missing && above + c0 >= missing) {
-      found[0] = top;
-      found[1] = above;
-    } else if (above + c0 < missing && above + c0 + c1 >= missing) {
-      found[0] = top - 1;
-      found[1] = above + c0;
+    int above = incl - mine + (wave ? __builtin_amdgcn_readlane(waves_upto, max(wave - 1, 0)) : 0);
+#pragma unroll
+    for (int i = 0; i < kThreadBins; i++) {
+      if (above < missing && above + in_bin[i] >= missing) {
+        found[0] = top - i;
+        found[1] = above;
+      }
+      above += in_bin[i];
     }
     __syncthreads();
     prefix |= (uint32_t)found[0] << shift;
