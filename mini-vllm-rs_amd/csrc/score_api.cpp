@@ -228,7 +228,7 @@ constexpr TileCost kF32Costs[] = {{16, 4, 3.3, {2.00, 4.20, 5.80, 6.90}, 0.0, 1.
 mvr::ScoreAttentionPlan plan_scored(const mvr_paged_attention_args* a, const mvr_score_rules* r, size_t limit) {
   const bool f16 = a->dtype == MVR_DTYPE_F16;
   const int64_t group = a->num_q_heads / a->num_kv_heads, longest_rows = group * a->max_q_len;
-  const int64_t cus = compute_units(), pairs = (int64_t)a->num_seqs * a->num_kv_heads;
+  const int64_t cus = compute_units();
   // Overrides, for tests and tuning: a tile size that the head dimension has, and its parts.
   static const int set_rows = env_int("MVR_SCORE_TILE_ROWS", 0);
   static const int set_waves = env_int("MVR_SCORE_TILE_WAVES", 4);
@@ -244,10 +244,19 @@ mvr::ScoreAttentionPlan plan_scored(const mvr_paged_attention_args* a, const mvr
     if (rows_set ? tile.rows != set_rows || tile.waves != set_waves : longest_rows <= tile.rows / 2 && best_cost < INFINITY) continue;
     const int held = mvr::score_blocks_per_cu(tile.rows, tile.waves, f16, a->head_dim);
     const TileWork w(a, r, tile.rows);
+    // Places for the longest request's row tiles of every request; packed, for as many as
+    // the packed tokens have and one more of each request, whose owner a block finds by a
+    // search of cu_q_lens: where that leaves half of the places out.  (63 single tokens and
+    // 2,000 new ones on 2,000 keys each, F16: 112 us packed and 151 padded for 28/4 heads,
+    // 43 and 125 for 7/1; ten batches whose lengths vary less, 0.82 to 1.07 times.)
+    const int64_t padded = (longest_rows + tile.rows - 1) / tile.rows;
+    const int64_t in_all = group * (a->total_q > 0 ? a->total_q : (int64_t)a->num_seqs * a->max_q_len) / tile.rows + a->num_seqs;
+    const bool packed = a->cu_q_lens && 2 * in_all <= padded * a->num_seqs;
+    const int64_t row_tiles = packed ? in_all : padded;
+    const int64_t groups = mvr::score_groups(packed, a->num_seqs, a->num_kv_heads), all_tiles = groups * row_tiles;
     const double unit_scale = (tile.own + (1 - tile.own) * a->head_dim / 128.0) * (r->cap > 0.f ? tile.capped : 1.0);
-    const int64_t row_tiles = (longest_rows + tile.rows - 1) / tile.rows, all_tiles = pairs * row_tiles;
     // (Row tiles of one KV head read the same keys, which the caches keep.)
-    const double hbm = (double)w.units / std::max<int64_t>(1, row_tiles) *
+    const double hbm = (double)w.units / std::max<int64_t>(1, padded) *
                        (2.0 * mvr::kScoreUnitTokens * a->head_dim * es_of(a->dtype) / 5.9e6);
     auto cost_of = [&](int64_t blocks, double longest) { // of `longest` units at most
       double body;
@@ -264,13 +273,15 @@ mvr::ScoreAttentionPlan plan_scored(const mvr_paged_attention_args* a, const mvr
       best.tile_rows = tile.rows;
       best.waves = tile.waves;
       best.row_tiles = (int)row_tiles;
+      best.packed = packed;
       best.parts = (int)parts;
       best.part_units = (int)std::min<int64_t>(part_units, INT32_MAX / 2); // (units are added to it)
       best.partial_bytes = bytes;
     };
     auto take_split = [&](int64_t part) { // parts of `part` units
       const int64_t parts = std::min<int64_t>((w.longest + part - 1) / part, mvr::kScoreMaxParts);
-      if (parts < 2 || 2 * parts > kMaxThreads / (64 * tile.waves) / ((pairs + mvr::kScoreXcds) * row_tiles)) return;
+      if (parts < 2 || 2 * parts > kMaxThreads / (64 * tile.waves) / ((groups + mvr::kScoreXcds) * row_tiles)) return;
+      if (all_tiles > kMaxThreads / (tile.rows * a->head_dim / 4 + 256)) return; // (the merge's)
       const int64_t rows = all_tiles * parts * tile.rows;
       const size_t bytes = align_up((size_t)rows * a->head_dim * sizeof(float), 256) +
                            align_up((size_t)rows * 2 * sizeof(float), 256) +
@@ -342,12 +353,12 @@ int validate_scored(const mvr_paged_attention_args* a, const int32_t* block_tabl
   for (int h = 0; slopes_host && h < a->num_q_heads; h++)
     if (!isfinite(slopes_host[h])) return fail(MVR_E_INVALID_ARGUMENT, "slope of head %d is not finite", h);
   for (int s = 0; s < a->num_seqs; s++) {
-    int64_t q_len = a->num_seqs == 1 ? a->max_q_len : -1, at = 0;
+    int64_t q_len = a->cu_q_lens ? -1 : a->max_q_len, at = 0; // (-1: not known here)
     if (cu_q_lens_host) {
       at = cu_q_lens_host[s];
       q_len = (int64_t)cu_q_lens_host[s + 1] - at;
     }
-    const int64_t seq_len = seq_lens_host ? seq_lens_host[s] : a->num_seqs == 1 ? a->max_seq_len : -1;
+    const int64_t seq_len = seq_lens_host ? seq_lens_host[s] : a->seq_lens ? -1 : a->max_seq_len;
     if (seq_lens_host) {
       if (seq_len < 0 || seq_len > a->max_seq_len)
         return fail(MVR_E_INVALID_ARGUMENT, "request %d has seq_len %lld outside [0, max_seq_len %d]", s,
@@ -419,11 +430,13 @@ int mvr_paged_attention_scored(const mvr_paged_attention_args* a, const mvr_scor
   p.out_stride_head = a->out_stride_head;
   p.out_stride_token = a->out_stride_token;
   p.row_tiles = plan.row_tiles;
+  p.packed = plan.packed;
   p.parts = plan.parts;
   p.part_units = plan.part_units;
-  p.run = mvr::score_run(plan, (int64_t)a->num_seqs * a->num_kv_heads);
+  const int64_t groups = mvr::score_groups(plan.packed, a->num_seqs, a->num_kv_heads);
+  p.run = mvr::score_run(plan, groups);
   if (plan.parts > 1) {
-    const size_t rows = (size_t)a->num_seqs * a->num_kv_heads * plan.row_tiles * plan.parts * plan.tile_rows;
+    const size_t rows = (size_t)groups * plan.row_tiles * plan.parts * plan.tile_rows;
     char* at = static_cast<char*>(a->workspace);
     p.partial_o = reinterpret_cast<float*>(at);
     at += align_up(rows * a->head_dim * sizeof(float), 256);
@@ -477,7 +490,7 @@ static int validate_weights(const mvr_paged_attention_args* a, const int32_t* bl
   if (rc != MVR_OK) return rc;
   for (int s = 0; fresh_from_host && s < a->num_seqs; s++)
     if (fresh_from_host[s] < 0) return fail(MVR_E_INVALID_ARGUMENT, "request %d has fresh_from %d", s, fresh_from_host[s]);
-  if (!block_tables_host || (a->num_seqs > 1 && (!seq_lens_host || !cu_q_lens_host))) return MVR_OK;
+  if (!block_tables_host || (a->seq_lens && !seq_lens_host) || (a->cu_q_lens && !cu_q_lens_host)) return MVR_OK;
   std::unique_ptr<uint8_t[]> written(new (std::nothrow) uint8_t[(size_t)a->num_pages]());
   if (!written) return fail(MVR_E_INVALID_ARGUMENT, "out of host memory");
   for (int s = 0; s < a->num_seqs; s++) {

@@ -49,14 +49,15 @@ __global__ __launch_bounds__(kWaveSize* kScoreWaves, (score_stream_blocks_per_cu
   T* const lds = reinterpret_cast<T*>(lds_raw) + (size_t)wave * C * kChunkTokens * D;
   const ScoreItem it = block_item(p);
   const ScoreTables& t = p.t;
-  if (it.pair >= t.num_seqs * t.num_kv_heads) return;
-  const int b = it.pair / t.num_kv_heads, h = it.pair - b * t.num_kv_heads;
+  if (it.group >= groups_of(p)) return;
+  const ScoreTile tile = tile_at<kTileRows>(p, it.group, it.at);
+  const int b = tile.b, h = tile.h;
   const ScoreSeq s = load_score_seq(t, b);
   const int rows = t.group_size * s.q_len;
-  if (it.rt * kTileRows >= rows) return;
+  if (!has_rows<kTileRows>(tile, rows)) return;
 
   // The lane's row.
-  const int rho = it.rt * kTileRows + (l & 15);
+  const int rho = tile.rt * kTileRows + (l & 15);
   const bool valid = rho < rows;
   const int i = valid ? rho / t.group_size : 0, head = h * t.group_size + (valid ? rho - i * t.group_size : 0);
   typename Tr::qreg_t q[Tr::kQRegs];
@@ -71,8 +72,7 @@ __global__ __launch_bounds__(kWaveSize* kScoreWaves, (score_stream_blocks_per_cu
   const int units = units_of(range), unit0 = range.begin / kScoreUnitTokens;
   const int parts = max(1, min(p.parts, (units + p.part_units - 1) / p.part_units));
   if (it.part >= parts) return;
-  const int64_t tile = (int64_t)it.pair * p.row_tiles + it.rt;
-  if (p.parts > 1 && it.part == 0 && threadIdx.x == 0) p.tile_parts[tile] = parts;
+  if (p.parts > 1 && it.part == 0 && threadIdx.x == 0) p.tile_parts[tile.place] = parts;
   constexpr int kUnitChunks = kScoreUnitTokens / kChunkTokens;
   const int n_chunks = (range.end + kChunkTokens - 1) / kChunkTokens;
   const int part0 = kUnitChunks * (unit0 + part_begin(it.part, units, parts));
@@ -153,15 +153,15 @@ __global__ __launch_bounds__(kWaveSize* kScoreWaves, (score_stream_blocks_per_cu
   };
 
   // Scores to probabilities.  The running maximum moves, and what the row holds is
-  // rescaled, only where a score exceeds it by more than 2^8.
+  // rescaled, only where a score exceeds it by enough.
   auto softmax = [&](float (&x)[4 * C]) {
     float mx = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 4 * C; e++) mx = fmaxf(mx, x[e]);
     mx = row_max(mx);
-    const bool grow = mx > m + kRescaleThreshold || (m == -INFINITY && mx != -INFINITY);
+    const bool grow = mx > m + kTopLimit || (m == -INFINITY && mx != -INFINITY);
     if (__any(grow)) {
-      const float m_new = grow ? mx : m;
+      const float m_new = grow ? mx - kTopStart : m;
       const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
 #pragma unroll
       for (int n = 0; n < D / 16; n++) o[n] *= alpha;
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(kWaveSize* kScoreWaves, (score_stream_blocks_per_cu
   };
   // O^T += V^T P^T of the chunks.  F16: two chunks in one product of 32 keys, lane group
   // g with tokens 4 g .. + 4 of each.  P enters as hi + lo, two F16 numbers whose sum is
-  // p but for 2^-20 of it (2^-24 where that is more): both are cut towards 0, p - hi is
+  // p but for 2^-20 of it (or 2^-24): both are cut towards 0, p - hi is
   // exact in 32 bits.  (With hi alone outputs are up to 1.8 times as far from the formula
   // as those of a form that holds 32 bits; the second product costs nothing where HBM is
   // the bound.)
@@ -313,7 +313,7 @@ __global__ __launch_bounds__(kWaveSize* kScoreWaves, (score_stream_blocks_per_cu
   constexpr int kCells = kTileRows * (D / 4); // float4 of the tile
   for (int c = threadIdx.x; c < kCells; c += kScoreWaves * kWaveSize) {
     const int rr = c / (D / 4), d = 4 * (c % (D / 4));
-    const int at = it.rt * kTileRows + rr;
+    const int at = tile.rt * kTileRows + rr;
     if (at >= rows) break; // rows grow with c
     float mmax = -INFINITY;
 #pragma unroll
@@ -328,7 +328,7 @@ __global__ __launch_bounds__(kWaveSize* kScoreWaves, (score_stream_blocks_per_cu
       acc += w * *reinterpret_cast<const float4v*>(merge_o + (j * kTileRows + rr) * kMergeStride + d);
     }
     if (parts > 1) {
-      const int64_t prow = (tile * p.parts + it.part) * kTileRows + rr;
+      const int64_t prow = (tile.place * p.parts + it.part) * kTileRows + rr;
       *reinterpret_cast<float4v*>(p.partial_o + prow * D + d) = acc;
       if (d == 0) {
         p.partial_ml[prow * 2 + 0] = mmax;
@@ -354,15 +354,15 @@ __global__ __launch_bounds__(256) void score_merge_kernel(ScoreAttentionParams p
   constexpr int kTileBlocks = (kTileRows * (D / 4) + 255) / 256;
   const int c = (int)(blockIdx.x % kTileBlocks) * 256 + threadIdx.x;
   const int rr = c / (D / 4), d = 4 * (c % (D / 4));
-  const int64_t tile = blockIdx.x / kTileBlocks;
-  const int pair = (int)(tile / p.row_tiles), rt = (int)(tile - (int64_t)pair * p.row_tiles);
-  const int b = pair / p.t.num_kv_heads, h = pair - b * p.t.num_kv_heads;
+  const int place = (int)(blockIdx.x / kTileBlocks), group = place / p.row_tiles;
+  const ScoreTile tile = tile_at<kTileRows>(p, group, place - group * p.row_tiles);
+  const int b = tile.b, h = tile.h;
   const ScoreSeq s = load_score_seq(p.t, b);
-  const int rho = rt * kTileRows + rr;
-  if (rt * kTileRows >= p.t.group_size * s.q_len) return; // (its parts were not counted)
-  const int parts = ((const const_i32*)p.tile_parts)[tile];
+  if (!has_rows<kTileRows>(tile, p.t.group_size * s.q_len)) return; // (its parts were not counted)
+  const int rho = tile.rt * kTileRows + rr;
+  const int parts = ((const const_i32*)p.tile_parts)[place];
   if (parts <= 1 || rr >= kTileRows || rho >= p.t.group_size * s.q_len) return;
-  const int64_t row0 = tile * p.parts * kTileRows + rr;
+  const int64_t row0 = tile.place * p.parts * kTileRows + rr;
   float4v acc = {0.f, 0.f, 0.f, 0.f};
   float sum = 0.f, m = -INFINITY;
   for (int j0 = 0; j0 < parts; j0 += kAhead) {
@@ -409,7 +409,7 @@ hipError_t launch_stream(const ScoreAttentionPlan& plan, const ScoreAttentionPar
 template <typename Tr, int D, int kTileRows>
 hipError_t launch_merge(const ScoreAttentionPlan& plan, const ScoreAttentionParams& p, hipStream_t stream) {
   constexpr int kTileBlocks = (kTileRows * (D / 4) + 255) / 256;
-  const dim3 grid((unsigned)((int64_t)kTileBlocks * p.t.num_seqs * p.t.num_kv_heads * plan.row_tiles));
+  const dim3 grid((unsigned)(kTileBlocks * score_groups(p.packed, p.t.num_seqs, p.t.num_kv_heads) * p.row_tiles));
   hipLaunchKernelGGL((score_merge_kernel<Tr, D, kTileRows>), grid, dim3(256), 0, stream, p);
   return hipGetLastError();
 }

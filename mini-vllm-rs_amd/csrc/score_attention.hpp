@@ -66,18 +66,24 @@ struct ScoreAttentionParams {
   const void* value_pool;
   void* out;
   int64_t out_stride_head, out_stride_token;
-  int32_t row_tiles; // of the longest request, per (request, KV head)
+  // Places for row tiles.  Padded: `row_tiles` of each (request, KV head), as many as the
+  // longest request has.  Packed: `row_tiles` of each KV head, request b's from
+  // cu_q_lens[b] * group_size / tile_rows + b on (rounded down: a request's tiles fit
+  // before the next one's).
+  int32_t row_tiles;
+  bool packed;
   int32_t parts, part_units;
   int32_t run; // items that follow each other on one XCD
-  float* partial_o;    // [pair][row tile][part][tile_rows][head_dim]
-  float* partial_ml;   // [pair][row tile][part][tile_rows][2]: maximum (log2 units), sum
-  int32_t* tile_parts; // [pair][row tile]: parts that it was split into
+  float* partial_o;    // [place][part][tile_rows][head_dim]
+  float* partial_ml;   // [place][part][tile_rows][2]: maximum (log2 units), sum
+  int32_t* tile_parts; // [place]: parts that its tile was split into
 };
 
 struct ScoreAttentionPlan {
   int tile_rows; // 16 (key streaming), 64 or 128 (key tiles in LDS)
   int waves;     // of a block: 4, or 8 (128 rows)
   int row_tiles;
+  bool packed;
   int parts, part_units;
   size_t partial_bytes; // 0: not split
 };
@@ -107,16 +113,21 @@ constexpr int score_blocks_per_cu(int tile_rows, int waves, bool f16, int head_d
                          : score_tile_blocks_per_cu(tile_rows, waves, f16, head_dim);
 }
 
-// Items that follow each other on one XCD: a pair's, where the pairs share out evenly;
+// Row tiles' places: so many times row_tiles.
+inline int64_t score_groups(bool packed, int64_t num_seqs, int64_t num_kv_heads) {
+  return packed ? num_kv_heads : num_seqs * num_kv_heads;
+}
+
+// Items that follow each other on one XCD: a group's, where the groups share out evenly;
 // else fewer, for some eight runs on each.
-inline int score_run(const ScoreAttentionPlan& plan, int64_t pairs) {
+inline int score_run(const ScoreAttentionPlan& plan, int64_t groups) {
   const int64_t inner = (int64_t)plan.row_tiles * plan.parts;
-  return (int)(pairs % kScoreXcds == 0 ? inner : std::max<int64_t>(1, std::min(inner, pairs * inner / (8 * kScoreXcds))));
+  return (int)(groups % kScoreXcds == 0 ? inner : std::max<int64_t>(1, std::min(inner, groups * inner / (8 * kScoreXcds))));
 }
 
 // Blocks of one launch.
 inline unsigned score_blocks(const ScoreAttentionParams& p) {
-  const int64_t items = (int64_t)p.t.num_seqs * p.t.num_kv_heads * p.row_tiles * p.parts;
+  const int64_t items = score_groups(p.packed, p.t.num_seqs, p.t.num_kv_heads) * p.row_tiles * p.parts;
   const int64_t round = (int64_t)kScoreXcds * p.run; // whole rounds of runs
   return (unsigned)((items + round - 1) / round * round);
 }

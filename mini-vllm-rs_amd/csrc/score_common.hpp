@@ -180,15 +180,69 @@ __device__ __forceinline__ void to_masked_scores(const ScoreRules& r, const Scor
   mask_scores(row, x, key0, offset, -INFINITY);
 }
 
+// The running maximum of a row is where its largest probability is 2^kTopStart, and moves
+// once one would exceed 2^kTopLimit: those that enter a product in F16, whose least step
+// is 2^-24, are then counted down to some 2^-31 of the largest, which a long cache may
+// hold millions of.  (F16 ends at 2^16.)
+constexpr float kTopStart = 7.f, kTopLimit = 15.f;
+
 constexpr int kScoreWaves = 4; // wavefronts per block
 
-// A block's item: part `part` of row tile rt of (request, KV head) pair.  Items are
-// numbered pair by pair, within a pair the last row tiles first, which a causal mask leaves
+// Row tile `rt` of request b and KV head h, in place `place`.
+struct ScoreTile {
+  int b, h, rt;
+  int64_t place;
+};
+
+// Packed: the last request whose places begin at or before place `at` of its head, by 64
+// requests at a time.
+template <int kTileRows>
+__device__ __forceinline__ int packed_request(const ScoreTables& t, int at, int& begin) {
+  auto begin_of = [&](int b) { return (int)((int64_t)t.cu_q_lens[b] * t.group_size / kTileRows) + b; };
+  int b = 0;
+  for (int n = t.num_seqs; n > 1;) {
+    const int step = (n + kWaveSize - 1) / kWaveSize, mine = b + lane_id() * step;
+    const int upto = __popcll(__ballot(mine < b + n && begin_of(min(mine, t.num_seqs - 1)) <= at));
+    const int skip = max(upto - 1, 0) * step;
+    b += skip;
+    n = min(step, n - skip);
+  }
+  b = __builtin_amdgcn_readfirstlane(b);
+  begin = __builtin_amdgcn_readfirstlane(begin_of(b));
+  return b;
+}
+
+// The tile of place `at` of group `group`.  (Its rt may lie behind the request's last tile,
+// or before its first where cu_q_lens does not begin at 0.)
+template <int kTileRows>
+__device__ __forceinline__ ScoreTile tile_at(const ScoreAttentionParams& p, int group, int at) {
+  ScoreTile x;
+  x.place = (int64_t)group * p.row_tiles + at;
+  if (p.packed) {
+    int begin;
+    x.b = packed_request<kTileRows>(p.t, at, begin);
+    x.h = group;
+    x.rt = at - begin;
+  } else {
+    x.b = group / p.t.num_kv_heads;
+    x.h = group - x.b * p.t.num_kv_heads;
+    x.rt = at;
+  }
+  return x;
+}
+
+template <int kTileRows>
+__device__ __forceinline__ bool has_rows(const ScoreTile& x, int rows) {
+  return x.rt >= 0 && (int64_t)x.rt * kTileRows < rows;
+}
+
+// A block's item: part `part` of the tile of a place.  Items are numbered group by group,
+// within one from the last place: the last row tiles first, which a causal mask leaves
 // the most keys.  Runs of p.run items go to one XCD (workgroups are dealt to the 8 XCDs
 // round-robin): neighbours read the same keys, through one L2.  Every other round deals
 // them backwards, so that no XCD gets the longer run of each round.
 struct ScoreItem {
-  int pair, rt, part;
+  int group, at, part;
 };
 
 __device__ __forceinline__ ScoreItem block_item(const ScoreAttentionParams& p) {
@@ -196,8 +250,12 @@ __device__ __forceinline__ ScoreItem block_item(const ScoreAttentionParams& p) {
   const uint32_t round = of_xcd / run, turn = round % 2 ? kScoreXcds - 1 - xcd : xcd;
   const uint32_t item = (round * kScoreXcds + turn) * run + (of_xcd - round * run);
   const uint32_t inner = (uint32_t)(p.row_tiles * p.parts);
-  const uint32_t pair = item / inner, rest = item - pair * inner, rt = rest / (uint32_t)p.parts;
-  return {(int)pair, p.row_tiles - 1 - (int)rt, (int)(rest - rt * p.parts)};
+  const uint32_t group = item / inner, rest = item - group * inner, at = rest / (uint32_t)p.parts;
+  return {(int)group, p.row_tiles - 1 - (int)at, (int)(rest - at * p.parts)};
+}
+
+__device__ __forceinline__ int groups_of(const ScoreAttentionParams& p) {
+  return p.packed ? p.t.num_kv_heads : p.t.num_seqs * p.t.num_kv_heads;
 }
 
 // First unit of part `part` (of `parts`, 64 at most) of `units`.

@@ -51,11 +51,12 @@ __global__ __launch_bounds__(kWaveSize* W, (score_tile_waves_per_simd(32 * RW, W
   const int rw = wave % RW, grp = wave / RW, hh = l >> 5;
   const ScoreItem it = block_item(p);
   const ScoreTables& t = p.t;
-  if (it.pair >= t.num_seqs * t.num_kv_heads) return;
-  const int b = it.pair / t.num_kv_heads, h = it.pair - b * t.num_kv_heads;
+  if (it.group >= groups_of(p)) return;
+  const ScoreTile tile = tile_at<kTileRows>(p, it.group, it.at);
+  const int b = tile.b, h = tile.h;
   const ScoreSeq s = load_score_seq(t, b);
   const int rows = t.group_size * s.q_len;
-  if (it.rt * kTileRows >= rows) return;
+  if (!has_rows<kTileRows>(tile, rows)) return;
 
   // The lane's row: query token i, query head of the KV head's group.
   auto row_at = [&](int rho, int& i, int& head) {
@@ -64,7 +65,7 @@ __global__ __launch_bounds__(kWaveSize* W, (score_tile_waves_per_simd(32 * RW, W
     head = h * t.group_size + (valid ? rho - i * t.group_size : 0);
     return valid;
   };
-  const int rho0 = it.rt * kTileRows + rw * 32; // the wavefront's first row
+  const int rho0 = tile.rt * kTileRows + rw * 32; // the wavefront's first row
   const bool live = rho0 < rows;                // it has rows
   ScoreRow row;
   // Q^T as the B operand: lane l holds row l % 32, dims 16 st + 8 hh .. + 8 (F32: 8 st + 4 hh .. + 4).
@@ -103,8 +104,7 @@ __global__ __launch_bounds__(kWaveSize* W, (score_tile_waves_per_simd(32 * RW, W
   const int units = units_of(range), unit0 = range.begin / kScoreUnitTokens;
   const int parts = max(1, min(p.parts, (units + p.part_units - 1) / p.part_units));
   if (it.part >= parts) return;
-  const int64_t tile = (int64_t)it.pair * p.row_tiles + it.rt;
-  if (p.parts > 1 && it.part == 0 && threadIdx.x == 0) p.tile_parts[tile] = parts;
+  if (p.parts > 1 && it.part == 0 && threadIdx.x == 0) p.tile_parts[tile.place] = parts;
   constexpr int kUnitTiles = kScoreUnitTokens / kTileTokens;
   const int n_tiles = (range.end + kTileTokens - 1) / kTileTokens;
   const int j0 = kUnitTiles * (unit0 + part_begin(it.part, units, parts));
@@ -165,8 +165,8 @@ __global__ __launch_bounds__(kWaveSize* W, (score_tile_waves_per_simd(32 * RW, W
     const char* vpool = static_cast<const char*>(p.value_pool);
     if constexpr (PAGES == kAnyPages) {
       // A load's tokens may lie in several pages, which take their lanes in turn.
-      // Lanes of tokens past
-      // the last key go with the last page, whose bound reads them as zeros.
+      // Lanes of tokens past the last key go with the last page, whose bound reads them
+      // as zeros.
       const int last_page_index = page_div(last_key);
 #pragma unroll
       for (int u = 0; u < TL::kLoads; u++) {
@@ -251,7 +251,7 @@ __global__ __launch_bounds__(kWaveSize* W, (score_tile_waves_per_simd(32 * RW, W
   };
   // In block c the lane holds tokens 32 c + 8 (e / 4) + 4 hh + e % 4 of its row.
   // Scores less the running maximum (log2 units), which moves, and O and the sum with it,
-  // only where a score exceeds it by more than 2^8; then P = 2^x in place, and its sum.
+  // only where a score exceeds it by enough; then P = 2^x in place, and its sum.
   // F16: the product with V takes P rounded to F16 (half a step, 2^-11 of p; a second
   // product for what the rounding leaves would cost a quarter), the sum holds 32 bits.
   auto softmax = [&](float16v (&sc)[kSub], int first, bool masked) __attribute__((always_inline)) { // first: the tile's first key
@@ -268,14 +268,14 @@ __global__ __launch_bounds__(kWaveSize* W, (score_tile_waves_per_simd(32 * RW, W
     for (int e = 0; e < 16 * kSub; e += 4) mx = fmaxf(mx, fmaxf(fmaxf(x[e], x[e + 1]), fmaxf(x[e + 2], x[e + 3])));
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
     mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-    const bool grow = mx > kRescaleThreshold || (m == -INFINITY && mx != -INFINITY);
+    const bool grow = mx > kTopLimit || (m == -INFINITY && mx != -INFINITY);
     if (__any(grow)) {
-      const float up = grow ? mx : 0.f;
+      const float up = grow ? mx - kTopStart : 0.f;
       const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-up);
 #pragma unroll
       for (int n = 0; n < D / 32; n++) o[n] *= alpha;
       lsum *= alpha;
-      m = grow ? (m == -INFINITY ? mx : m + mx) : m;
+      m = grow ? (m == -INFINITY ? up : m + up) : m;
 #pragma unroll
       for (int e = 0; e < 16 * kSub; e++) x[e] -= up;
     }
@@ -522,7 +522,7 @@ __global__ __launch_bounds__(kWaveSize* W, (score_tile_waves_per_simd(32 * RW, W
       }
   };
   if (parts > 1) {
-    const int64_t prow = (tile * p.parts + it.part) * kTileRows + rw * 32 + le;
+    const int64_t prow = (tile.place * p.parts + it.part) * kTileRows + rw * 32 + le;
     put(p.partial_o + prow * D, 1.f);
     if (hh == 0) {
       p.partial_ml[prow * 2 + 0] = m;

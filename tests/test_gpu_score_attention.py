@@ -237,6 +237,80 @@ def test_many_requests():
         check(b)
 
 
+@pytest.mark.parametrize("q", [[1] * 70 + [200], [200] + [1] * 70, [1, 0, 1, 90, 0, 1, 1, 0, 1, 1], [1] * 30 + [33, 0, 0] + [2] * 40 + [64],
+                               [0] * 63 + [128], [0] * 64 + [129], [5] + [0] * 200 + [64]])
+@pytest.mark.parametrize("group", [1, 3, 8])
+def test_mixed_batches(group, q):
+    """Prompts among single tokens and empty requests, where row tiles' places are packed by the tokens there are."""
+    for dtype in (F16, F32):
+        rng = np.random.default_rng(len(q) + group)
+        b = Batch(31, dtype, 2 * group, 2, 64, 16, rng.integers(0, 300, len(q)), q, cap=20.0, tail=2)
+        t = b.device()
+        out, lse = torch.full_like(t["q"], 7.0), torch.full(t["q"].shape[:2], 7.0, device="cuda")
+        check_attention(*run(b, dict(t, out=out, lse=lse)), b)
+        assert bool((out[:, int(b.cu[-1]):] == 7).all()) and bool((lse[:, int(b.cu[-1]):] == 7).all())
+
+
+def test_mixed_batch_of_thousands():
+    rng = np.random.default_rng(8)
+    for n in (4095, 4200):
+        q = np.ones(n, np.int64)
+        q[rng.integers(0, n, 3)] = 150
+        q[rng.integers(0, n, 500)] = 0
+        check(Batch(32, F16, 4, 1, 32, 4, rng.integers(0, 6, n), q))
+
+
+def test_mixed_graph_replays():
+    """A captured call whose prompt is another request's at each replay."""
+    batches = [Batch(33, F16, 8, 2, 128, 16, [700] * 20, [1] * k + [150] + [1] * (19 - k), cap=30.0) for k in (3, 0, 19, 11)]
+    t = batches[0].device()
+    out, lse = torch.empty_like(t["q"]), torch.empty(t["q"].shape[:2], device="cuda")
+    call = S.make_scored_call(*t.values(), out, lse, **batches[0].rules())
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    pages = t["block_tables"].shape[1]
+    for b in batches + batches[::-1]:
+        for name, x in b.device().items():
+            if name == "block_tables":
+                t[name][:, :min(pages, x.shape[1])] = x[:, :pages]
+            else:
+                t[name].copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        check_attention(out, lse, b)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_many_keys_far_below_one(dtype, new):
+    """One key at e^18.75 of 200,000 others, which hold 0.14% of a row together and all of its output.
+
+    F16 probabilities are off by 2^-25 at most where they are that small, the largest being 2^7 or more: 2^-32 of the sum
+    for each key (2^-31, where both halves of one are cut); 2^-24 of the sum for each in 32 bits, of which the large key's
+    own adds 2^-24 of the sum; then half a step of the output."""
+    n, page, d = 200_000, 16, 32
+    pages = n // page
+    q = torch.zeros((2, new, d), dtype=dtype, device="cuda")
+    q[..., 0] = 8.0
+    keys = torch.zeros((pages, 1, 1, page, d), dtype=dtype, device="cuda")
+    values = torch.ones_like(keys)
+    keys[0, 0, 0, 0, 0], values[0, 0, 0, 0] = 18.75 / 8, 0.0
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    out, lse = S.paged_attention_scored(q, keys, values, table, ints(n), ints(0, new), max_q_len=new, max_seq_len=n, scale=1.0)
+    torch.cuda.synchronize()
+    others = torch.arange(n - new, n, dtype=torch.float64) * np.exp(-18.75)
+    want = (others / (1 + others))[None, :, None]
+    u = 2.0 ** -11 if dtype == F16 else 2.0 ** -24
+    tol = n * (2.0 ** -31 if dtype == F16 else 0) + want * (u + 2.0 ** -16) + 2.0 ** -24
+    assert bool(((out.double().cpu() - want).abs() <= tol).all()), float(((out.double().cpu() - want).abs() / tol).max())
+    within = (lse.double().cpu() - (18.75 + torch.log1p(others))).abs()
+    assert float(within.max()) <= 2.0 ** -18
+
+
 def test_graph_replays():
     """Captured calls, split and not, replayed with changed lengths and values between, with eager work in between."""
     for cached, q, rules in (([3000], [1], dict(cap=30.0)), ([200, 90], [70, 4], dict(slopes=True, window=50))):

@@ -43,7 +43,9 @@ def cases():
         yield f"window {window}", lambda a=(window, 90): A.test_windows(*a)
     for cap in (1e-3, 5.0, 1e6):
         yield f"cap {cap}", lambda a=cap: A.test_caps(a)
-    for f in (A.test_scale_and_far_keys, A.test_rows_that_see_nothing, A.test_empty_requests_and_padded_rows,
+    for q in ([1] * 70 + [200], [1, 0, 1, 90, 0, 1, 1, 0, 1, 1], [0] * 64 + [129]):
+        yield f"mixed {len(q)}", lambda a=(4, q): A.test_mixed_batches(*a)
+    for f in (A.test_mixed_batch_of_thousands, A.test_mixed_graph_replays, A.test_scale_and_far_keys, A.test_rows_that_see_nothing, A.test_empty_requests_and_padded_rows,
               A.test_lse_is_not_wanted, A.test_strides, A.test_split_keys_and_workspaces, A.test_stale_hints,
               A.test_lengths_above_their_bounds_are_clamped, A.test_one_request_without_tables, A.test_pools_past_32_bits,
               A.test_many_requests, A.test_graph_replays, A.test_streams_and_repeats):

@@ -193,6 +193,31 @@ def test_attention_validate():
         assert e.value.code == code and text in e.value.message, e.value.message
 
 
+def test_validate_leaves_out_what_only_the_device_knows():
+    """One request whose tables are on the device alone: its bounds are not taken for its lengths."""
+    bt = np.array([[5, 1 << 20]], np.int32)  # (one page is used, the other entry never written)
+    sizes = dict(num_seqs=1, total_q=20, max_seq_len=32, max_pages_per_seq=2, max_q_len=20)
+    one = dict(seq_lens_host=np.array([3]))
+    for validate, args in ((S.validate_scored, scored_args(**sizes)), (S.validate_weights, weights_args(**sizes))):
+        validate(*args, block_tables_host=bt)
+        validate(*args, block_tables_host=bt, **one)
+        validate(*args, block_tables_host=bt, **one, cu_q_lens_host=np.array([0, 1]))
+        with pytest.raises(M.MvrError) as e:
+            validate(*args, block_tables_host=bt, seq_lens_host=np.array([20]))
+        assert e.value.code == M.MVR_E_PAGE_ID
+    with pytest.raises(M.MvrError) as e:  # without tables the bounds are the lengths
+        S.validate_weights(*weights_args(**sizes, seq_lens=None, cu_q_lens=None), block_tables_host=bt)
+    assert e.value.code == M.MVR_E_PAGE_ID
+
+
+def test_workspace_of_mixed_batches():
+    """By the tokens that are there, not by the longest request in every place."""
+    lens, cu = np.full(64, 2000, np.int32), np.concatenate([[0], np.cumsum([1] * 63 + [2000])]).astype(np.int32)
+    a, r = scored_args(num_seqs=64, num_q_heads=7, num_kv_heads=1, max_q_len=2000, max_seq_len=2000, max_pages_per_seq=125,
+                       total_q=int(cu[-1]), seq_lens_host=lens.ctypes.data, cu_q_lens_host=cu.ctypes.data, q_stride_head=1 << 20)
+    assert S.load_library().mvr_paged_attention_scored_workspace_size(ctypes.byref(a), ctypes.byref(r)) < 256 << 20
+
+
 def test_workspace_follows_the_hints():
     """Bounded by the splits, none for batches that fill the device, and no table makes the plan fail."""
     lib = S.load_library()
