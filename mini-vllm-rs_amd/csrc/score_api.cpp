@@ -699,7 +699,7 @@ int mvr_select_tokens(const mvr_select_tokens_args* a) {
   p.recent = a->recent;
   p.first = a->first;
   mvr::page_divider(a->page_size, p.page_magic, p.page_magic_shift);
-  return launch_status(mvr::launch_select_tokens(p, static_cast<hipStream_t>(a->stream)));
+  return launch_status(mvr::launch_select_tokens(p, compute_units(), static_cast<hipStream_t>(a->stream)));
 }
 
 // ---------------------------------------------------------------------------

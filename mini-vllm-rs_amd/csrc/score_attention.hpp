@@ -177,7 +177,7 @@ struct SelectTokensParams {
   int32_t page_magic_shift;
 };
 
-hipError_t launch_select_tokens(const SelectTokensParams& params, hipStream_t stream);
+hipError_t launch_select_tokens(const SelectTokensParams& params, int compute_units, hipStream_t stream);
 
 // Moves.
 struct MoveTokensParams {

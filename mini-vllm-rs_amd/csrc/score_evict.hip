@@ -4,6 +4,8 @@
 
 #include <limits.h>
 
+#include <type_traits>
+
 #include "cache_rows.hpp"
 #include "wave_scan.hpp"
 
@@ -25,33 +27,40 @@ constexpr int kWave = 64;
 // stays past slot `keep` and what goes below it are as many, and are paired in ascending
 // order.
 //
-// Bound by the block's own chain of steps, not by the bytes: the weights are read once,
-// and their keys held in LDS for the passes over them.  A thread takes four slots at a
-// time, one 16-byte access each to weights, positions and keys where pages hold whole
-// fours (VEC).
+// The weights are read once, and their keys held in LDS for the passes over them; a
+// thread takes four slots at a time, one 16-byte access each to weights, positions and
+// keys where pages hold whole fours (VEC).  Not bound by the bytes: by a block's own chain
+// of steps where blocks are few (2 heads of 1,040 tokens in 24 layers: 6.7 us), by the
+// vector unit, some 100 instructions per four slots and pass, where they are many (8 heads
+// of 16 requests of 1,500 to 8,000 tokens in 8 layers: 30.5 us, the bytes' 8.3).
 // ---------------------------------------------------------------------------
-constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / kWave;
-constexpr int kDigitBits = 11, kDigits = 3, kBins = 1 << kDigitBits, kThreadBins = kBins / kSelectThreads;
+constexpr int kDigitBits = 11, kDigits = 3, kBins = 1 << kDigitBits;
 constexpr int kFour = 4; // slots of a thread at a time
-// Keys that LDS holds: two blocks to a CU beside the histograms.  Requests that may be
-// longer read weights and positions anew in each pass.
-constexpr int kHeldKeys = 17408;
+// Keys that LDS holds beside the histogram: of four blocks to a CU, or of two.  Requests
+// that may be longer read weights and positions anew in each pass.
+constexpr int kFewKeys = 8128, kManyKeys = 17408;
 
 typedef int int4v __attribute__((ext_vector_type(4)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ uint32_t ascending(float w) {
-  const uint32_t x = __float_as_uint(w);
-  if (w != w || x == 0xff800000u) return 0; // NaN, -infinity
-  return w == 0.f ? 0x80000000u : x >> 31 ? ~x : x | 0x80000000u;
+  const int x = __float_as_int(w != w ? -INFINITY : w + 0.f); // (-0 is 0)
+  return (uint32_t)(x ^ (x >> 31 | INT_MIN));
 }
 
-template <bool HELD, bool VEC>
+// Lanes below this one that are in `lanes`, and `more`.
+__device__ __forceinline__ int lanes_before(uint64_t lanes, int more) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, more));
+}
+
+template <int kSelectThreads, int kHeldKeys, bool VEC>
 __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(SelectTokensParams p) {
+  constexpr bool HELD = kHeldKeys > 0;
+  constexpr int kSelectWaves = kSelectThreads / kWave, kThreadBins = kBins / kSelectThreads;
   __shared__ int bins[kBins];
   __shared__ int wave_counts[kSelectWaves][4];
   __shared__ int found[2]; // digit, keys above it
-  __shared__ __attribute__((aligned(16))) uint32_t held[HELD ? kHeldKeys : kFour];
+  __shared__ __attribute__((aligned(16))) uint32_t held[kHeldKeys + kFour];
   const int tid = threadIdx.x, l = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   // The KV heads of one table follow each other on one XCD (workgroups are dealt to the 8
   // XCDs round-robin): their weights share cache lines.
@@ -67,6 +76,7 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
   if (min(keep, n - keep) > p.max_moves) keep = n; // (its moves might not fit)
   if (table < p.num_seqs && h == 0 && tid == 0 && p.new_seq_lens) p.new_seq_lens[b] = keep;
   const bool cut = keep != n && keep != 0; // (else nothing goes, or nothing stays)
+  const int last_from = (int)max((int64_t)next - p.recent, (int64_t)INT_MIN); // positions of the last `recent`
   int32_t* const count = p.num_moves + row;
   if (!cut && tid == 0) *count = 0;
 
@@ -87,7 +97,8 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
     if constexpr (VEC) {
       const int64_t first = index_of(t), some = max(first, (int64_t)0);
       const float4v w4 = *reinterpret_cast<const float4v*>(p.weights + some);
-      const int4v pos4 = *reinterpret_cast<const int4v*>(p.positions + some);
+      int4v pos4 = {0, 0, 0, 0};
+      if (t < kept) pos4 = *reinterpret_cast<const int4v*>(p.positions + some);
 #pragma unroll
       for (int j = 0; j < kFour; j++) {
         at[j] = first < 0 ? -1 : first + j;
@@ -111,7 +122,7 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
       fresh[j] = next - (n - (t + j));
       all &= t + j >= kept;
       if (t + j >= kept) pos[j] = fresh[j];
-      const bool guarded = pos[j] < p.first || pos[j] >= (int64_t)next - p.recent;
+      const bool guarded = pos[j] < p.first || pos[j] >= last_from;
       key[j] = t + j >= n || at[j] < 0 ? 0 : guarded ? ~0u : ascending(w[j]);
     }
     if (!writes) return;
@@ -187,23 +198,30 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
   const int run = (n + kSelectWaves * kWaveSlots - 1) / (kSelectWaves * kWaveSlots) * kWaveSlots;
   const int t0 = min(wave * run, n), t1 = min(t0 + run, n);
   int ties = 0, low_ties = 0, holes = 0, movers = 0;
-  for (int t = t0 + kFour * l; t < t1; t += kWaveSlots) {
-    uint32_t key[kFour];
-    keys_of(t, key);
+  for (int base = t0; base < t1; base += kWaveSlots) {
+    const int t = base + kFour * l;
+    uint32_t key[kFour] = {0, 0, 0, 0};
+    if (t < t1) keys_of(t, key);
+    if (base + kWaveSlots <= min(t1, keep)) { // whole, in slots below `keep`
 #pragma unroll
-    for (int j = 0; j < kFour; j++) {
-      const bool in = t + j < t1, low = t + j < keep, tie = in && key[j] == prefix;
-      ties += tie;
-      low_ties += tie && low;
-      holes += in && key[j] < prefix && low;
-      movers += in && key[j] > prefix && !low;
+      for (int j = 0; j < kFour; j++) {
+        const int at_t = __popcll(__ballot(key[j] == prefix));
+        ties += at_t;
+        low_ties += at_t;
+        holes += __popcll(__ballot(key[j] < prefix));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kFour; j++) {
+        const bool in = t + j < t1, low = t + j < keep, tie = in && key[j] == prefix;
+        ties += __popcll(__ballot(tie));
+        low_ties += __popcll(__ballot(tie && low));
+        holes += __popcll(__ballot(in && key[j] < prefix && low));
+        movers += __popcll(__ballot(in && key[j] > prefix && !low));
+      }
     }
   }
-  ties = wave_inclusive_sum(ties);
-  low_ties = wave_inclusive_sum(low_ties);
-  holes = wave_inclusive_sum(holes);
-  movers = wave_inclusive_sum(movers);
-  if (l == kWave - 1) {
+  if (l == 0) {
     wave_counts[wave][0] = ties;
     wave_counts[wave][1] = low_ties;
     wave_counts[wave][2] = holes;
@@ -228,35 +246,40 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
     const int t = base + kFour * l;
     uint32_t key[kFour] = {0, 0, 0, 0};
     if (t < t1) keys_of(t, key);
-    int lane_ties = 0;
+    uint64_t tie[kFour], any_ties = 0;
 #pragma unroll
-    for (int j = 0; j < kFour; j++) lane_ties += t + j < t1 && key[j] == prefix;
-    int before = 0; // tokens at T in the lanes before it
-    if (__any(lane_ties)) before = wave_inclusive_sum(lane_ties) - lane_ties;
-    int rank = my_ties + before, lane_holes = 0, lane_movers = 0;
+    for (int j = 0; j < kFour; j++) any_ties |= tie[j] = __ballot(t + j < t1 && key[j] == prefix);
     bool hole[kFour], mover[kFour];
+    uint64_t holes_at[kFour], movers_at[kFour];
+    int rank = my_ties; // of the lane's next token at T
+    if (any_ties) {
+#pragma unroll
+      for (int j = 0; j < kFour; j++) {
+        rank = lanes_before(tie[j], rank);
+        my_ties += __popcll(tie[j]);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < kFour; j++) {
-      const bool in = t + j < t1, tie = key[j] == prefix;
-      const bool stays = key[j] > prefix || (tie && rank < missing);
-      rank += in && tie;
-      hole[j] = in && t + j < keep && !stays;
-      mover[j] = in && t + j >= keep && stays;
-      lane_holes += hole[j];
-      lane_movers += mover[j];
+      const bool in = t + j < t1, at_t = in && key[j] == prefix;
+      const bool stays = key[j] > prefix || (at_t && rank < missing);
+      rank += at_t;
+      holes_at[j] = __ballot(hole[j] = in && t + j < keep && !stays);
+      movers_at[j] = __ballot(mover[j] = in && t + j >= keep && stays);
     }
-    // (Both counts, 256 at most, in one scan.)
-    const int both = wave_inclusive_sum(lane_holes + (lane_movers << 16));
-    int to = my_hole + (both & 0xffff) - lane_holes, from = my_mover + (both >> 16) - lane_movers;
+    int to = my_hole, from = my_mover;
+#pragma unroll
+    for (int j = 0; j < kFour; j++) {
+      to = lanes_before(holes_at[j], to);
+      from = lanes_before(movers_at[j], from);
+      my_hole += __popcll(holes_at[j]);
+      my_mover += __popcll(movers_at[j]);
+    }
 #pragma unroll
     for (int j = 0; j < kFour; j++) {
       if (hole[j]) moves[2 * (int64_t)to++ + 1] = t + j;
       if (mover[j]) moves[2 * (int64_t)from++] = t + j;
     }
-    const int total = __builtin_amdgcn_readlane(both, kWave - 1);
-    my_hole += total & 0xffff;
-    my_mover += total >> 16;
-    my_ties += __builtin_amdgcn_readlane(before + lane_ties, kWave - 1);
   }
 }
 
@@ -331,15 +354,27 @@ __global__ __launch_bounds__(kMoveThreads) void move_tokens_kernel(MoveTokensPar
 
 } // namespace
 
-hipError_t launch_select_tokens(const SelectTokensParams& params, hipStream_t stream) {
+hipError_t launch_select_tokens(const SelectTokensParams& params, int compute_units, hipStream_t stream) {
   const int64_t eights = ((int64_t)params.num_layers * params.num_seqs + 7) / 8;
-  const dim3 grid((unsigned)(eights * 8 * params.num_kv_heads)), block(kSelectThreads);
+  const int64_t blocks = eights * 8 * params.num_kv_heads;
+  const dim3 grid((unsigned)blocks);
   const bool vec = params.page_size % kFour == 0 && ((uintptr_t)params.weights | (uintptr_t)params.positions) % 16 == 0;
-  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, params); };
-  if (params.max_seq_len <= kHeldKeys)
-    vec ? launch(select_tokens_kernel<true, true>) : launch(select_tokens_kernel<true, false>);
+  auto launch = [&](auto threads, auto held) {
+    constexpr int kThreads = decltype(threads)::value, kHeld = decltype(held)::value;
+    if (vec)
+      hipLaunchKernelGGL((select_tokens_kernel<kThreads, kHeld, true>), grid, dim3(kThreads), 0, stream, params);
+    else
+      hipLaunchKernelGGL((select_tokens_kernel<kThreads, kHeld, false>), grid, dim3(kThreads), 0, stream, params);
+  };
+  // More blocks than CUs hold of the large ones at once: small ones, whose passes then
+  // overlap.  (128 heads of 1,500 to 8,000 tokens in 8 layers, 1,024 blocks: 30.5 us in
+  // small blocks and 32.7 in large ones; 16 heads of 8,000, 128 blocks: 14.6 and 12.7.)
+  if (params.max_seq_len <= kFewKeys && blocks > 2 * compute_units)
+    launch(std::integral_constant<int, 512>(), std::integral_constant<int, kFewKeys>());
+  else if (params.max_seq_len <= kManyKeys)
+    launch(std::integral_constant<int, 1024>(), std::integral_constant<int, kManyKeys>());
   else
-    vec ? launch(select_tokens_kernel<false, true>) : launch(select_tokens_kernel<false, false>);
+    launch(std::integral_constant<int, 1024>(), std::integral_constant<int, 0>());
   return hipGetLastError();
 }
 
