@@ -221,7 +221,7 @@ constexpr TileCost kF32Costs[] = {{16, 4, 3.3, {2.00, 4.20, 5.80, 6.90}, 0.0, 1.
 
 // The tile size and the split of its keys that these costs make fastest: every tile
 // whole, or in parts that give each CU one block, two, up to as many as it holds, or
-// two, three or four times that.  A call takes its blocks' time (all of them in one
+// two, three or four times that, or in fewer parts where tiles are few.  A call takes its blocks' time (all of them in one
 // round; in more rounds the average load and most of a last block), joined with the time
 // that its keys take from HBM (as a 3-norm).  A split call merges: a launch, a chain of
 // loads over a row's parts, and its partial results written and read at 4.3 TB/s.
@@ -307,6 +307,11 @@ mvr::ScoreAttentionPlan plan_scored(const mvr_paged_attention_args* a, const mvr
       if (part < w.longest && part != last) take_split(part);
       last = part;
     }
+    // And where tiles of 16 rows are few, fewer parts than that, which are merged sooner.
+    // (One token on 3,000, 14/2 heads of 64 F16: 9.7 us in 12 parts, 15.7 in 47.)
+    for (int64_t parts = 2; tile.rows == 16 && parts * w.tiles < cus && parts < std::min<int64_t>(w.longest, mvr::kScoreMaxParts);
+         parts += (parts + 1) / 2)
+      take_split((w.longest + parts - 1) / parts);
     // Where a workspace is too small for all of these, the fewest parts that fit.
     if (limit != SIZE_MAX && best.parts <= 1)
       for (int64_t parts = 2; parts <= 8; parts++) take_split((w.longest + parts - 1) / parts);
