@@ -568,6 +568,7 @@ static int check_layers(int32_t num_layers, int32_t num_seqs, int32_t num_kv_hea
   if (max_moves < 1) return fail(MVR_E_INVALID_ARGUMENT, "max_moves must be positive");
   if (num_pages > INT32_MAX || num_pages > kMaxSlots / num_kv_heads / page_size)
     return fail(MVR_E_UNSUPPORTED, "pools of over 2^31 pages, or 2^40 tokens and heads");
+  if ((int64_t)num_kv_heads * page_size > INT32_MAX) return fail(MVR_E_UNSUPPORTED, "pages of over 2^31 rows");
   if ((int64_t)num_layers * num_seqs + 7 > kMaxThreads / threads_per_row / num_kv_heads)
     return fail(MVR_E_UNSUPPORTED, "more layers, requests and KV heads than one call takes");
   return MVR_OK;

@@ -23,6 +23,14 @@ namespace {
 // ---------------------------------------------------------------------------
 // Key streaming: a block of 4 wavefronts per item, 16 rows, each wavefront its share
 // of the part's 16-token chunks straight from the cache; their results merge in LDS.
+//
+// For rows that are few: bound by HBM where there are blocks enough (32/8 heads of 128 F16:
+// 64 single tokens on 300 to 8,192 201 us, 5.2 TB/s; 32 of them with a window of 4,096
+// 94 us, 5.7 TB/s), else by the chunks that follow each other in a wavefront, some 1 us
+// each (one token on 512, 2 KV heads of 64 F32: 12.2 us whole, 8.8 in 8 parts with their
+// merge).  8 and 16 wavefronts to a block: 11.1 and 12.1, whole.  For more rows key tiles
+// win: 4 requests of 8 tokens on 2,000 14.1 us here and 19.1 in tiles of 64 rows, of 16
+// tokens 20.7 and 20.3, of 32 23.8 and 21.5 (32/8 heads of 128 F16).
 // ---------------------------------------------------------------------------
 // Chunks of one step: two of F16, whose softmax and products are then one of 32 keys;
 // F32 rows hold twice the registers.
@@ -346,7 +354,8 @@ __global__ __launch_bounds__(kWaveSize* kScoreWaves, (score_stream_blocks_per_cu
 
 // out = sum_j 2^(m_j - M) o_j / sum_j 2^(m_j - M) l_j over the parts of each row tile
 // that was split; one thread per 4 elements, 4 parts' loads in flight, one pass with a
-// running maximum.
+// running maximum.  Bound by its launch and a chain of loads: 3.3 us for a row of 8 parts,
+// 5.5 for 512 tiles of 16 rows, 8.5 for 144 of 128 rows in 4 parts.
 template <typename Tr, int D, int kTileRows>
 __global__ __launch_bounds__(256) void score_merge_kernel(ScoreAttentionParams p) {
   typedef typename Tr::elem T;

@@ -28,8 +28,9 @@ constexpr int kWave = 64;
 // order.
 //
 // The weights are read once, and their keys held in LDS for the passes over them; a
-// thread takes four slots at a time, one 16-byte access each to weights, positions and
-// keys where pages hold whole fours (VEC).  Not bound by the bytes: by a block's own chain
+// thread takes four slots at a time, with one 16-byte access each to weights, positions
+// and keys where pages hold whole fours (VEC; 8 heads of 32 requests of 8,000 tokens, 4
+// layers: 38 us, in 6-token pages 44).  Not bound by the bytes: by a block's own chain
 // of steps where blocks are few (2 heads of 1,040 tokens in 24 layers: 6.7 us), by the
 // vector unit, some 100 instructions per four slots and pass, where they are many (8 heads
 // of 16 requests of 1,500 to 8,000 tokens in 8 layers: 30.5 us, the bytes' 8.3).
@@ -37,7 +38,8 @@ constexpr int kWave = 64;
 constexpr int kDigitBits = 11, kDigits = 3, kBins = 1 << kDigitBits;
 constexpr int kFour = 4; // slots of a thread at a time
 // Keys that LDS holds beside the histogram: of four blocks to a CU, or of two.  Requests
-// that may be longer read weights and positions anew in each pass.
+// that may be longer read weights and positions anew in each pass (the same 8,000 tokens,
+// where max_seq_len lets them be longer: 50 us).
 constexpr int kFewKeys = 8128, kManyKeys = 17408;
 
 typedef int int4v __attribute__((ext_vector_type(4)));
@@ -81,16 +83,18 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
   if (!cut && tid == 0) *count = 0;
 
   const int32_t* bt = p.block_tables + (int64_t)table * p.block_table_stride;
+  const uint32_t page_rows = (uint32_t)(p.num_kv_heads * p.page_size);
+  const int head_rows = h * p.page_size;
   // Index of slot t in the pools, or -1.
   auto index_of = [&](int t) -> int64_t {
-    const int pi = (int)(((uint64_t)(uint32_t)t * p.page_magic) >> p.page_magic_shift);
-    const int64_t page = bt[pi];
+    const int pi = (int)(((uint64_t)(uint32_t)t * p.page_magic) >> p.page_magic_shift), page = bt[pi];
     if (page < 0 || page >= p.num_pages) return -1;
-    return (page * p.num_kv_heads + h) * p.page_size + (t - pi * p.page_size);
+    return (int64_t)((uint64_t)(uint32_t)page * page_rows + (uint32_t)(head_rows + (t - pi * p.page_size)));
   };
-  // Keys of slots t .. t + 3 (0 past the last one, and in pages outside the pool), and
-  // where `writes` is set the positions of those that were appended since the last cut.
-  auto read_four = [&](int t, bool writes, uint32_t (&key)[kFour]) {
+  // Keys of slots t, t + stride, ... (VEC: stride 1; 0 past the last one, and in pages
+  // outside the pool), and where `writes` is set the positions of those that were appended
+  // since the last cut.
+  auto read_four = [&](int t, int stride, bool writes, uint32_t (&key)[kFour]) __attribute__((always_inline)) {
     int64_t at[kFour];
     float w[kFour];
     int pos[kFour];
@@ -107,23 +111,25 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < kFour; j++) at[j] = index_of(min(t + j, n - 1));
+      for (int j = 0; j < kFour; j++) at[j] = index_of(min(t + stride * j, n - 1));
 #pragma unroll
       for (int j = 0; j < kFour; j++) {
         const int64_t some = max(at[j], (int64_t)0);
         w[j] = p.weights[some];
-        pos[j] = p.positions[some];
+        pos[j] = 0;
+        if (t + stride * j < kept) pos[j] = p.positions[some];
       }
     }
     int4v fresh;
     bool all = at[0] >= 0 && t + kFour <= n;
 #pragma unroll
     for (int j = 0; j < kFour; j++) {
-      fresh[j] = next - (n - (t + j));
-      all &= t + j >= kept;
-      if (t + j >= kept) pos[j] = fresh[j];
+      const int slot = t + stride * j;
+      fresh[j] = next - (n - slot);
+      all &= slot >= kept;
+      if (slot >= kept) pos[j] = fresh[j];
       const bool guarded = pos[j] < p.first || pos[j] >= last_from;
-      key[j] = t + j >= n || at[j] < 0 ? 0 : guarded ? ~0u : ascending(w[j]);
+      key[j] = slot >= n || at[j] < 0 ? 0 : guarded ? ~0u : ascending(w[j]);
     }
     if (!writes) return;
     if (VEC && all) {
@@ -131,7 +137,7 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
     } else {
 #pragma unroll
       for (int j = 0; j < kFour; j++)
-        if (t + j < n && t + j >= kept && at[j] >= 0) p.positions[at[j]] = fresh[j];
+        if (t + stride * j < n && t + stride * j >= kept && at[j] >= 0) p.positions[at[j]] = fresh[j];
     }
   };
   auto keys_of = [&](int t, uint32_t (&key)[kFour]) {
@@ -140,14 +146,25 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
 #pragma unroll
       for (int j = 0; j < kFour; j++) key[j] = (uint32_t)x[j];
     } else {
-      read_four(t, false, key);
+      read_four(t, 1, false, key);
     }
   };
   for (int i = tid; i < kBins; i += kSelectThreads) bins[i] = 0;
-  for (int t = HELD && cut ? kFour * tid : max(kept, 0) / kFour * kFour + kFour * tid; t < n; t += kFour * kSelectThreads) {
-    uint32_t key[kFour];
-    read_four(t, true, key);
-    if (HELD && cut) *reinterpret_cast<int4v*>(held + t) = int4v{(int)key[0], (int)key[1], (int)key[2], (int)key[3]};
+  const int t_begin = HELD && cut ? 0 : max(kept, 0) / kFour * kFour;
+  if constexpr (VEC || !HELD) {
+    for (int t = t_begin + kFour * tid; t < n; t += kFour * kSelectThreads) {
+      uint32_t key[kFour];
+      read_four(t, 1, true, key);
+      if (HELD && cut) *reinterpret_cast<int4v*>(held + t) = int4v{(int)key[0], (int)key[1], (int)key[2], (int)key[3]};
+    }
+  } else { // (a slot's neighbours to the lanes beside)
+    for (int t = t_begin + tid; t < n; t += kFour * kSelectThreads) {
+      uint32_t key[kFour];
+      read_four(t, kSelectThreads, true, key);
+#pragma unroll
+      for (int j = 0; j < kFour; j++)
+        if (cut && t + kSelectThreads * j < n) held[t + kSelectThreads * j] = key[j];
+    }
   }
   if (!cut) return;
   __syncthreads();
@@ -287,7 +304,9 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
 // Moves: a wavefront takes 32 moves of a (layer, request, KV head) at a time.  Its lanes
 // look up the pages of all their slots at once, then share the rows' vectors out among
 // them, a batch of K and V in flight together.  No slot is both a source and a target,
-// so rows move in any order.  Bound by HBM where there are many.
+// so rows move in any order.  Bound by HBM where there are many: 180,000 rows of 256
+// bytes of K and V in random pages 47.4 us, 3.9 TB/s read and written (a large copy: 5.1);
+// 8 vectors to a batch 49.5, 16 moves to a wavefront 48.6.
 // ---------------------------------------------------------------------------
 constexpr int kMoveThreads = 256, kMoveWaves = kMoveThreads / kWave;
 constexpr int kWaveMoves = kWave / 2;

@@ -13,9 +13,18 @@
 // those that any of them sees, tests masks in the steps at the ends only, and a wavefront
 // whose rows see nothing of a step leaves it out.
 //
-// Bound by the vector unit: a score takes its scale, exponential, sum and rounding, and a
-// cap as many operations again, while the two products of its 32 x 32 block take the
-// matrix pipe half that time.
+// Bound by the vector unit and the matrix pipe in turn: a score takes its scale,
+// exponential, sum and rounding, and a cap as many operations again, while the two
+// products of its 32 x 32 block take the matrix pipe half that time.  28/4 heads of 128
+// F16: a prompt of 8,192 549 us, 0.88 PFLOP/s; four of 256 on 2,048 with a cap 57.6 us,
+// 0.56.  F32 by the matrix pipe: three of 217 on up to 1,218 130 us, 75% busy in the CUs
+// that have a block.
+//
+// 64 rows (two groups) where rows are few, 128 where a key's bytes should serve more of
+// them, in 4 wavefronts, two blocks to a CU, or in 8, one, where blocks are fewer than
+// CUs.  32/8 heads of 128 F16, unsplit, 64 rows, 128, 128 in 8 wavefronts: 32 requests of
+// 16 tokens on 4,000 102, 107 and 100 us (16 rows streamed: 179); a prompt of 2,000 57, 59
+// and 57 (170); documents of 1,500 in a prompt of 6,000 178, 163 and 183.
 #include "key_tiles.hpp"
 #include "score_common.hpp"
 
