@@ -65,8 +65,9 @@ typedef struct mvr_score_rules {
 /* mvr_paged_attention under the rules above.  Same arguments, layouts, dtypes, head
    dimensions (multiples of 32 up to 256), page sizes (any; nothing is repacked) and
    hints.  Scores, softmax state and sums are held in 32 bits.  F16 probabilities
-   enter the product with V with 20 bits; calls of many rows round them to F16 for it,
-   not for the sum that divides them.  Differences to mvr_paged_attention:
+   enter the product with V with 20 bits, and calls of many rows round them to F16 for
+   it (in steps of 2^-31 of a row's largest, where they are that small), not for the
+   sum that divides them.  Differences to mvr_paged_attention:
      - a request may have q_len 0: nothing is computed for it, so total_q, where
        given, lies in [0, num_seqs * max_q_len];
      - rows of q, out and lse from cu_q_lens[num_seqs] on are neither read nor
