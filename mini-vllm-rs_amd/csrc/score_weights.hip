@@ -10,8 +10,9 @@
 // row tile are summed once, at the end.
 //
 // Bound by HBM where rows are few (every key is read once, all of a wavefront's loads in
-// flight together: 64 single tokens on 8,192, 28/4 heads of 128 F16, 217 us, 4.95 TB/s), by
-// the exponentials and the cap where they are many (4 of 32 on 6,000, capped: 24.5 us).  Each weight has one
+// flight together: 64 single tokens on 8,192, 28/4 heads of 128 F16, 112 us, 4.8 TB/s), by
+// the exponentials and the cap where they are many (4 of 32 on 6,000, capped: 24.5 us, with
+// 32 keys to a wavefront 28.1).  Each weight has one
 // writer and one order of its sum.
 #include "score_common.hpp"
 
