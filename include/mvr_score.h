@@ -155,7 +155,7 @@ typedef struct mvr_select_tokens_args {
   const int32_t* seq_lens;       /* device [num_seqs] */
   const int32_t* next_positions; /* device [num_seqs]: position of the next token to come; NULL: seq_lens (no token
                                     was dropped before) */
-  const int32_t* kept_lens;      /* device [num_seqs]: slots whose positions are known; NULL: 0 */
+  const int32_t* kept_lens;      /* device [num_seqs]: slots whose positions are known (above seq_len: all); NULL: 0 */
   const int32_t* keep_lens;      /* device [num_seqs]: tokens to keep; not below seq_len: all stay */
   int32_t* moves;                /* device [num_layers][num_seqs][num_kv_heads][max_moves][2]: from slot, to slot */
   int32_t* num_moves;            /* device [num_layers][num_seqs][num_kv_heads], written */

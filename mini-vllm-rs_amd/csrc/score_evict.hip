@@ -73,7 +73,7 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
   const const_i32* lens = (const const_i32*)p.seq_lens;
   const int n = max(0, min(lens[b], p.max_seq_len));
   const int next = p.next_positions ? ((const const_i32*)p.next_positions)[b] : n;
-  const int kept = p.kept_lens ? ((const const_i32*)p.kept_lens)[b] : 0;
+  const int kept = p.kept_lens ? min(((const const_i32*)p.kept_lens)[b], n) : 0;
   int keep = max(0, min(((const const_i32*)p.keep_lens)[b], n));
   if (min(keep, n - keep) > p.max_moves) keep = n; // (its moves might not fit)
   if (table < p.num_seqs && h == 0 && tid == 0 && p.new_seq_lens) p.new_seq_lens[b] = keep;
