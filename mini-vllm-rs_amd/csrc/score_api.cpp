@@ -589,7 +589,7 @@ static int check_select(const mvr_select_tokens_args* a) {
   rc = check_layers(a->num_layers, a->num_seqs, a->num_kv_heads, a->page_size, a->num_pages, 1024, a->max_moves);
   if (rc != MVR_OK) return rc;
   if (a->max_seq_len < 1) return fail(MVR_E_INVALID_ARGUMENT, "max_seq_len must be positive");
-  if (a->max_seq_len > INT32_MAX - 2048)
+  if (a->max_seq_len > INT32_MAX - mvr::kSelectStep)
     return fail(MVR_E_UNSUPPORTED, "max_seq_len %d is too close to 2^31", a->max_seq_len);
   if (a->recent < 0 || a->first < 0) return fail(MVR_E_INVALID_ARGUMENT, "recent and first must not be negative");
   const int64_t pages_needed = (a->max_seq_len + (int64_t)a->page_size - 1) / a->page_size;

@@ -158,7 +158,10 @@ constexpr int weights_unit_tokens(int elem_bytes, int head_dim) {
 // split: the rows are shared out among a block's wavefronts, not the keys.
 hipError_t launch_score_weights(const ScoreWeightsParams& params, int dtype, int head_dim, bool split, hipStream_t stream);
 
-// Which tokens stay.
+// Which tokens stay.  Slots that a block steps over at a time, at most: the kernel's slot
+// numbers pass a request's length by less than that.
+constexpr int kSelectStep = 4096;
+
 struct SelectTokensParams {
   const float* weights;
   int32_t* positions;

@@ -59,6 +59,7 @@ template <int kSelectThreads, int kHeldKeys, bool VEC>
 __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(SelectTokensParams p) {
   constexpr bool HELD = kHeldKeys > 0;
   constexpr int kSelectWaves = kSelectThreads / kWave, kThreadBins = kBins / kSelectThreads;
+  static_assert(kFour * kSelectThreads <= kSelectStep, "slots are counted in 32 bits");
   __shared__ int bins[kBins];
   __shared__ int wave_counts[kSelectWaves][4];
   __shared__ int found[2]; // digit, keys above it
