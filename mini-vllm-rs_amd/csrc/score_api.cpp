@@ -718,6 +718,8 @@ static int check_move(const mvr_move_tokens_args* a) {
   if (rc != MVR_OK) return rc;
   rc = check_layers(a->num_layers, a->num_seqs, a->num_kv_heads, a->page_size, a->num_pages, 256, a->max_moves);
   if (rc != MVR_OK) return rc;
+  if (a->max_moves > INT32_MAX - mvr::kMoveStep)
+    return fail(MVR_E_UNSUPPORTED, "max_moves %d is too close to 2^31", a->max_moves);
   if (a->max_pages_per_seq < 1) return fail(MVR_E_INVALID_ARGUMENT, "max_pages_per_seq must be positive");
   if (!a->block_tables || !a->moves || !a->num_moves) return fail(MVR_E_INVALID_ARGUMENT, "null table pointer");
   if ((uintptr_t)a->moves % 8) return fail(MVR_E_INVALID_ARGUMENT, "moves must be 8-byte aligned");

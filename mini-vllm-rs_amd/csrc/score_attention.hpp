@@ -182,7 +182,10 @@ struct SelectTokensParams {
 
 hipError_t launch_select_tokens(const SelectTokensParams& params, int compute_units, hipStream_t stream);
 
-// Moves.
+// Moves.  Those of one row that its blocks step over at a time, at most: the kernel's
+// numbers of moves pass max_moves by less than that.
+constexpr int kMoveStep = 1 << 23;
+
 struct MoveTokensParams {
   void* key_pool;
   void* value_pool;

@@ -403,7 +403,8 @@ hipError_t launch_move_tokens(const MoveTokensParams& params, int64_t row_bytes,
   // Blocks for all of a row's moves at once, but no more than some tens of rounds of them.
   constexpr int kBlockMoves = kMoveWaves * kWaveMoves;
   const int64_t pieces = ((int64_t)params.max_moves + kBlockMoves - 1) / kBlockMoves;
-  const int blocks_per_row = (int)std::max<int64_t>(1, std::min<int64_t>(pieces, 65536 / rows));
+  constexpr int kMostBlocks = kMoveStep / kBlockMoves;
+  const int blocks_per_row = (int)std::max<int64_t>(1, std::min<int64_t>(pieces, kMostBlocks / rows));
   return with_vector(row_bytes, params.key_pool, params.value_pool, [&](auto v, int row_vecs) {
     hipLaunchKernelGGL(move_tokens_kernel<decltype(v)>, dim3((unsigned)(rows * blocks_per_row)), dim3(kMoveThreads), 0,
                        stream, params, row_vecs, blocks_per_row);

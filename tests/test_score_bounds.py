@@ -3,7 +3,7 @@ import pytest
 
 import mvr_attn as M
 import mvr_score as S
-from test_score_api import select_args
+from test_score_api import move_args, select_args
 
 
 def refused(validate, *args, text, code=M.MVR_E_UNSUPPORTED):
@@ -21,3 +21,10 @@ def test_longest_request_of_a_selection():
     S.validate_select(select_args(**sizes, max_seq_len=2 ** 31 - 1 - 4096))
     for n in (2 ** 31 - 4096, 2 ** 31 - 2049, 2 ** 31 - 1):
         refused(S.validate_select, select_args(**sizes, max_seq_len=n), text="too close to 2^31")
+
+
+def test_most_moves_of_a_row():
+    """A row's blocks step over up to 2^23 moves at a time, and count them in 32 bits."""
+    S.validate_move(move_args(max_moves=2 ** 31 - 1 - 2 ** 23))
+    for n in (2 ** 31 - 2 ** 23, 2 ** 31 - 1):
+        refused(S.validate_move, move_args(max_moves=n), text="too close to 2^31")
