@@ -49,9 +49,11 @@ __device__ __forceinline__ int prefix_of(const ScoreRules& r, int b) {
 __device__ __forceinline__ ScoreRow score_row(const ScoreRules& r, const ScoreSeq& s, int prefix, int q_head, int i) {
   ScoreRow row;
   row.pos = s.seq_len - s.q_len + i;
-  int hi = max(row.pos + 1, prefix), lo = 0;
+  // (Slots below 0, of a request shorter than its query, and negative table entries count as
+  // 0 here: no difference leaves 32 bits.)
+  int hi = max(max(row.pos + 1, prefix), 0), lo = 0;
   if (r.first_keys) lo = max(lo, r.first_keys[s.q_start + i]);
-  if (r.window > 0) lo = max(lo, row.pos - (r.window - 1));
+  if (r.window > 0) lo = max(lo, max(row.pos, 0) - (r.window - 1));
   hi = min(hi, s.seq_len);
   row.width = max(hi - lo, 0);
   row.lo = row.width ? lo : 0;

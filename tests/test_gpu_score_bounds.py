@@ -5,7 +5,10 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import mvr_score as S  # noqa: E402
+from score_reference import Batch, check_attention  # noqa: E402
+from test_gpu_score_attention import run  # noqa: E402
 from test_gpu_score_evict import Cache, check as check_selection  # noqa: E402
+from test_gpu_score_weights import check as check_weights  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -25,3 +28,23 @@ def test_kept_lengths_above_the_request(kept, lens, keep, page):
     t = c.device()
     t["kept_lens"].fill_(kept)
     check_selection(c, t)
+
+
+def broken(dtype, cached, q, **rules):
+    """Requests shorter than their queries among whole ones, first keys and prefixes at the ends of their type."""
+    ends = dict(first_keys=[2 ** 31 - 1, 0, -2 ** 31, 1, 2 ** 31 - 1, -5], prefix=[-2 ** 31, 2 ** 31 - 1, 1, -1, 0])
+    return Batch(22, dtype, 16, 2, 64, 16, cached, q, **{**ends, **rules})
+
+
+@pytest.mark.parametrize("window", [0, 1, 2 ** 31 - 1])
+@pytest.mark.parametrize("q", [[5, 3, 5, 7, 2], [45, 40, 5, 70, 60]])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_row_ranges_at_the_ends_of_32_bits(dtype, q, window):
+    """Slots below 0 see no key, or a prefix; no difference of a slot and a table's number wraps."""
+    for cached in ([-3, 60, -4, 90, -1], [-1, 200, 3, 0, 20]):
+        b = broken(dtype, cached, q, window=window)
+        check_attention(*run(b, hints=False), b, note=str(cached))
+        check_weights(b, 0.5, note=str(cached))
+        no_prefix = broken(dtype, cached, q, window=window, prefix=None)
+        check_attention(*run(no_prefix, hints=False), no_prefix, note=str(cached))
+        check_weights(no_prefix, 0.5, note=str(cached))
