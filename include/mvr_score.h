@@ -49,7 +49,8 @@ extern "C" {
      s = scale * q . k_j,   s = cap * tanh(s / cap),   s - slopes[h] * |p - j|.
    Distances and windows count cache slots: after a cut, whose moves change the
    order, only the cap and masks that end before the moved slots mean what they say.
-   A query that sees no key has output 0 and log-sum-exp -infinity. */
+   A query that sees no key, as those of a request of length 0, has output 0 and
+   log-sum-exp -infinity. */
 typedef struct mvr_score_rules {
   float cap;                  /* > 0; 0: scores are not capped */
   int32_t window;             /* keys that a query sees at most, up to itself; 0: any number */

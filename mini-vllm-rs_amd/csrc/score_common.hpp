@@ -28,7 +28,8 @@ __device__ __forceinline__ ScoreSeq load_score_seq(const ScoreTables& t, int b) 
   s.seq_len = t.seq_lens ? min(seq_len, t.max_seq_len) : t.max_seq_len;
   s.q_start = t.cu_q_lens ? q_start : 0;
   s.q_len = t.cu_q_lens ? min(q_end - q_start, t.max_q_len) : t.max_q_len;
-  if (s.seq_len <= 0 || s.q_len <= 0) s.seq_len = s.q_len = 0;
+  s.seq_len = max(s.seq_len, 0); // (its rows see nothing, but they are rows)
+  if (s.q_len <= 0) s.seq_len = s.q_len = 0;
   return s;
 }
 

@@ -48,3 +48,20 @@ def test_row_ranges_at_the_ends_of_32_bits(dtype, q, window):
         no_prefix = broken(dtype, cached, q, window=window, prefix=None)
         check_attention(*run(no_prefix, hints=False), no_prefix, note=str(cached))
         check_weights(no_prefix, 0.5, note=str(cached))
+
+
+@pytest.mark.parametrize("seq_len", [0, -7, -2 ** 31])
+@pytest.mark.parametrize("q", [[1, 1, 1], [3, 2, 70], [60, 90, 1]])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_requests_of_length_0_with_query_tokens(dtype, q, seq_len):
+    """A padded slot of a batch: its rows see nothing, which is an output of 0 and a log-sum-exp of -infinity; nobody's
+    weights change for it."""
+    for rules in (dict(cap=20.0), dict(prefix=[9, 2000, 5]), dict(slopes=True, window=40)):
+        b = Batch(23, dtype, 16, 2, 64, 16, [100, -q[1], 2000], q, **rules)
+        t = b.device()
+        t["seq_lens"][1] = seq_len
+        out, lse = torch.full_like(t["q"], 7.0), torch.full(t["q"].shape[:2], 7.0, device="cuda")
+        check_attention(*run(b, dict(t, out=out, lse=lse), hints=False), b, note=str(rules))
+        rows = slice(q[0], q[0] + q[1])
+        assert not out[:, rows].any() and bool((lse[:, rows] == -float("inf")).all())
+        check_weights(b, 0.5, note=str(rules))
