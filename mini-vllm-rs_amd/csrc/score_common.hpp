@@ -24,12 +24,11 @@ __device__ __forceinline__ ScoreSeq load_score_seq(const ScoreTables& t, int b) 
   const int q_start = *(t.cu_q_lens ? (const word*)t.cu_q_lens + b : any);
   const int q_end = *(t.cu_q_lens ? (const word*)t.cu_q_lens + b + 1 : any);
   ScoreSeq s;
-  // Clamped to the bounds that the host has checked tables for.
-  s.seq_len = t.seq_lens ? min(seq_len, t.max_seq_len) : t.max_seq_len;
+  // Clamped to the bounds that the host has checked tables for.  (Rows of a request of
+  // length 0 see nothing, but they are rows.)
+  s.seq_len = max(t.seq_lens ? min(seq_len, t.max_seq_len) : t.max_seq_len, 0);
   s.q_start = t.cu_q_lens ? q_start : 0;
-  s.q_len = t.cu_q_lens ? min(q_end - q_start, t.max_q_len) : t.max_q_len;
-  s.seq_len = max(s.seq_len, 0); // (its rows see nothing, but they are rows)
-  if (s.q_len <= 0) s.seq_len = s.q_len = 0;
+  s.q_len = max(t.cu_q_lens ? min(q_end - q_start, t.max_q_len) : t.max_q_len, 0);
   return s;
 }
 

@@ -43,7 +43,7 @@ __global__ __launch_bounds__(kWaveSize* kWaves, (weights_waves<typename Tr::elem
   const int key0 = (SPLIT ? block : block * kWaves + wave) * kUnit;
   const int b = pair / t.num_kv_heads, h = pair - b * t.num_kv_heads;
   const ScoreSeq s = load_score_seq(t, b);
-  if (key0 >= s.seq_len) return; // (SPLIT: the whole block)
+  if (key0 >= s.seq_len || s.q_len == 0) return; // (SPLIT: the whole block)
   const int rows = t.group_size * s.q_len, prefix = prefix_of(p.r, b);
 
   // Lane l holds the page entry of key key0 + l (lanes past the last key that key's).
