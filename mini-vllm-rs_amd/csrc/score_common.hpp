@@ -46,19 +46,26 @@ __device__ __forceinline__ int prefix_of(const ScoreRules& r, int b) {
   return r.prefix_lens ? ((const const_i32*)r.prefix_lens)[b] : 0;
 }
 
-__device__ __forceinline__ ScoreRow score_row(const ScoreRules& r, const ScoreSeq& s, int prefix, int q_head, int i) {
+__device__ __forceinline__ int first_key_of(const ScoreRules& r, int token) { return r.first_keys ? r.first_keys[token] : 0; }
+__device__ __forceinline__ float slope_of(const ScoreRules& r, int q_head) { return r.slopes ? r.slopes[q_head] : 0.f; }
+
+__device__ __forceinline__ ScoreRow score_row(const ScoreRules& r, const ScoreSeq& s, int prefix, int i, int first_key,
+                                              float slope) {
   ScoreRow row;
   row.pos = s.seq_len - s.q_len + i;
   // (Slots below 0, of a request shorter than its query, and negative table entries count as
   // 0 here: no difference leaves 32 bits.)
-  int hi = max(max(row.pos + 1, prefix), 0), lo = 0;
-  if (r.first_keys) lo = max(lo, r.first_keys[s.q_start + i]);
+  int hi = max(max(row.pos + 1, prefix), 0), lo = max(first_key, 0);
   if (r.window > 0) lo = max(lo, max(row.pos, 0) - (r.window - 1));
   hi = min(hi, s.seq_len);
   row.width = max(hi - lo, 0);
   row.lo = row.width ? lo : 0;
-  row.slope_log2 = r.slopes ? r.slopes[q_head] * 1.4426950408889634f : 0.f;
+  row.slope_log2 = slope * 1.4426950408889634f;
   return row;
+}
+
+__device__ __forceinline__ ScoreRow score_row(const ScoreRules& r, const ScoreSeq& s, int prefix, int q_head, int i) {
+  return score_row(r, s, prefix, i, first_key_of(r, s.q_start + i), slope_of(r, q_head));
 }
 
 __device__ __forceinline__ bool sees(const ScoreRow& row, int key) {
@@ -125,7 +132,9 @@ __device__ __forceinline__ KeyRange rows_range(const KeyRange& mine) {
 // A cap costs 7 operations a score while all of them lie in the polynomial's range (those
 // of a model that caps them mostly do): its coefficients hold scale, cap and log2(e).
 // Past it tanh(y) = 1 - 2 / (e^2y + 1), off by 2^-21 at most; that takes an exponential
-// and a reciprocal, 16 cycles each, and loses small values to cancellation.
+// and a reciprocal, 16 cycles each, and loses small values to cancellation, so the scores
+// in range take the polynomial also where others are past it: a score is the same number
+// whatever the others are.
 template <int N, typename Offset>
 __device__ __forceinline__ void to_scores(const ScoreRules& r, const ScoreRow& row, float minus, float (&x)[N], int key0,
                                           Offset offset) {
@@ -134,22 +143,27 @@ __device__ __forceinline__ void to_scores(const ScoreRules& r, const ScoreRow& r
 #pragma unroll
     for (int e = 0; e < N; e++) top = fmaxf(top, fabsf(x[e]));
     // (A NaN among scores in range takes either way as a NaN.)
+    auto in_range = [&](float s, float p) {
+      const float u = s * s;
+#pragma unroll
+      for (int k = 4; k >= 0; k--) p = fmaf(p, u, r.cap_poly[k]);
+      return fmaf(s, p, -minus);
+    };
     if (__any(!(top <= r.cap_poly_limit))) {
 #pragma unroll
       for (int e = 0; e < N; e++) {
-        if (e % 4 == 0) __builtin_amdgcn_sched_barrier(0); // (few at a time: the other way sets the registers)
-        const float ey = __builtin_amdgcn_exp2f(x[e] * r.cap_exp_scale);
-        x[e] = fmaf(r.cap_log2, fmaf(-2.f, __builtin_amdgcn_rcpf(ey + 1.f), 1.f), -minus);
+        // (One at a time, and nothing that both ways compute, or all scores, worked out
+        // before: the other way sets the registers.)
+        __builtin_amdgcn_sched_barrier(0);
+        float s = x[e], p;
+        asm volatile("v_mov_b32 %0, %2" : "=v"(p), "+v"(s) : "s"(r.cap_poly[5]));
+        const float ey = __builtin_amdgcn_exp2f(s * r.cap_exp_scale);
+        const float past = fmaf(r.cap_log2, fmaf(-2.f, __builtin_amdgcn_rcpf(ey + 1.f), 1.f), -minus);
+        x[e] = fabsf(s) <= r.cap_poly_limit ? in_range(s, p) : past;
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < N; e++) {
-        const float u = x[e] * x[e];
-        float p = r.cap_poly[5];
-#pragma unroll
-        for (int k = 4; k >= 0; k--) p = fmaf(p, u, r.cap_poly[k]);
-        x[e] = fmaf(x[e], p, -minus);
-      }
+      for (int e = 0; e < N; e++) x[e] = in_range(x[e], r.cap_poly[5]);
     }
   } else {
 #pragma unroll

@@ -54,8 +54,8 @@ __global__ __launch_bounds__(kWaveSize* kWaves, (weights_waves<typename Tr::elem
   // The next row tile's queries and rows are on their way while one is computed.
   struct Rows {
     typename Tr::qreg_t q[Tr::kQRegs];
-    ScoreRow row;
-    float lse;
+    int i, first_key;
+    float slope, lse;
     bool valid;
   };
   int token = (16 * (SPLIT ? wave : 0) + (l & 15)) / t.group_size; // the lane's row of the next tile: token and head
@@ -71,7 +71,9 @@ __global__ __launch_bounds__(kWaveSize* kWaves, (weights_waves<typename Tr::elem
       token++;
     }
     r.lse = p.r.lse[(int64_t)head * p.r.lse_stride_head + s.q_start + i];
-    r.row = score_row(p.r, s, prefix, head, i);
+    r.i = i;
+    r.first_key = first_key_of(p.r, s.q_start + i);
+    r.slope = slope_of(p.r, head);
     Tr::load_q(static_cast<const T*>(t.q) + (int64_t)head * t.q_stride_head + (int64_t)(s.q_start + i) * t.q_stride_token,
                r.valid, g, r.q);
   };
@@ -95,6 +97,8 @@ __global__ __launch_bounds__(kWaveSize* kWaves, (weights_waves<typename Tr::elem
   const int fresh = p.fresh_from ? ((const const_i32*)p.fresh_from)[b] : s.seq_len - s.q_len;
   const bool keeps = writes && my_key < fresh && p.decay != 0.f;
   const float had = keeps ? p.weights[slot] : 0.f;
+  __shared__ uint64_t slots[kWaves][kWaveSize]; // (each lane's own: no register holds it over the rows)
+  slots[wave][l] = slot;
 
   float acc[4 * kChunks];
 #pragma unroll
@@ -103,11 +107,12 @@ __global__ __launch_bounds__(kWaveSize* kWaves, (weights_waves<typename Tr::elem
   for (; rho0 < rows; rho0 += kRowStep) {
     Rows r = next;
     if (rho0 + kRowStep < rows) load_rows(next);
-    if (!r.valid || r.lse == -INFINITY) r.row.width = 0;
+    ScoreRow row = score_row(p.r, s, prefix, r.i, r.first_key, r.slope);
+    if (!r.valid || r.lse == -INFINITY) row.width = 0;
     const float lse_log2 = r.lse * 1.4426950408889634f;
-    const int end = r.row.lo + r.row.width;
-    if (!__any(r.row.width && end > key0 && r.row.lo < key0 + kUnit)) continue;
-    const bool masked = __any(end < key0 + kUnit || r.row.lo > key0); // some row does not see all the keys
+    const int end = row.lo + row.width;
+    if (!__any(row.width && end > key0 && row.lo < key0 + kUnit)) continue;
+    const bool masked = __any(end < key0 + kUnit || row.lo > key0); // some row does not see all the keys
     float x[4 * kChunks];
 #pragma unroll
     for (int c = 0; c < kChunks; c++) {
@@ -117,9 +122,9 @@ __global__ __launch_bounds__(kWaveSize* kWaves, (weights_waves<typename Tr::elem
     }
     auto offset = [](int e) { return 16 * (e >> 2) + (e & 3); };
     if (masked)
-      to_masked_scores(p.r, r.row, lse_log2, x, key0 + 4 * g, offset);
+      to_masked_scores(p.r, row, lse_log2, x, key0 + 4 * g, offset);
     else
-      to_scores(p.r, r.row, lse_log2, x, key0 + 4 * g, offset);
+      to_scores(p.r, row, lse_log2, x, key0 + 4 * g, offset);
 #pragma unroll
     for (int e = 0; e < 4 * kChunks; e++) acc[e] += __builtin_amdgcn_exp2f(x[e]);
   }
@@ -140,7 +145,7 @@ __global__ __launch_bounds__(kWaveSize* kWaves, (weights_waves<typename Tr::elem
     __syncthreads();
     got = ((sums[0][l] + sums[1][l]) + sums[2][l]) + sums[3][l];
   }
-  if (writes) p.weights[slot] = (keeps ? p.decay * had : 0.f) + got;
+  if (writes) p.weights[slots[wave][l]] = (keeps ? p.decay * had : 0.f) + got;
 }
 
 template <typename Tr, int D>
