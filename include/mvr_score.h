@@ -80,7 +80,7 @@ typedef struct mvr_score_rules {
    launch; rows are computed from the device tables whatever they hold. */
 int mvr_paged_attention_scored(const mvr_paged_attention_args* args, const mvr_score_rules* rules);
 
-/* Bytes of workspace that the call needs (0: none; contents need no
+/* Bytes of workspace that the call needs (0: none; 96 MiB at most; contents need no
    initialisation and are dead after the call).  Depends on the scalars and the
    hints.  With less workspace, or none, the call still runs: it splits the keys as
    far as its workspace allows, down to not at all.  Calls that share a workspace

@@ -219,6 +219,12 @@ constexpr TileCost kF32Costs[] = {{16, 4, 3.3, {2.00, 4.20, 5.80, 6.90}, 0.0, 1.
                                   {128, 4, 12.0, {7.20, 14.3, 14.3, 14.3}, 0.0, 1.0},
                                   {128, 8, 12.0, {7.50, 7.50, 7.50, 7.50}, 0.0, 1.0}};
 
+// Bytes of partial results that a split may take, at most; they hold a slot for every part
+// of every place, also where few tiles have so many.  (11 calls of F32 prompts and long
+// contexts whose fastest plans by cost take 37 to 238 MiB: none is over 5% slower within
+// 96 MiB, four are faster; within 48, 36%, 41% and 20% slower are three.)
+constexpr size_t kSplitBudget = (size_t)96 << 20;
+
 // The tile size and the split of its keys that these costs make fastest: every tile
 // whole, or in parts that give each CU one block, two, up to as many as it holds, or
 // two, three or four times that, or in fewer parts where tiles are few.  A call takes its blocks' time (all of them in one
@@ -226,6 +232,7 @@ constexpr TileCost kF32Costs[] = {{16, 4, 3.3, {2.00, 4.20, 5.80, 6.90}, 0.0, 1.
 // that its keys take from HBM (as a 3-norm).  A split call merges: a launch, a chain of
 // loads over a row's parts, and its partial results written and read at 4.3 TB/s.
 mvr::ScoreAttentionPlan plan_scored(const mvr_paged_attention_args* a, const mvr_score_rules* r, size_t limit) {
+  limit = std::min(limit, kSplitBudget);
   const bool f16 = a->dtype == MVR_DTYPE_F16;
   const int64_t group = a->num_q_heads / a->num_kv_heads, longest_rows = group * a->max_q_len;
   const int64_t cus = compute_units();
@@ -278,6 +285,7 @@ mvr::ScoreAttentionPlan plan_scored(const mvr_paged_attention_args* a, const mvr
       best.part_units = (int)std::min<int64_t>(part_units, INT32_MAX / 2); // (units are added to it)
       best.partial_bytes = bytes;
     };
+    bool too_large = false;
     auto take_split = [&](int64_t part) { // parts of `part` units
       const int64_t parts = std::min<int64_t>((w.longest + part - 1) / part, mvr::kScoreMaxParts);
       if (parts < 2 || 2 * parts > kMaxThreads / (64 * tile.waves) / ((groups + mvr::kScoreXcds) * row_tiles)) return;
@@ -286,7 +294,10 @@ mvr::ScoreAttentionPlan plan_scored(const mvr_paged_attention_args* a, const mvr
       const size_t bytes = align_up((size_t)rows * a->head_dim * sizeof(float), 256) +
                            align_up((size_t)rows * 2 * sizeof(float), 256) +
                            align_up((size_t)all_tiles * sizeof(int32_t), 256);
-      if (bytes > limit) return;
+      if (bytes > limit) {
+        too_large = true;
+        return;
+      }
       part = std::max(part, (w.longest + parts - 1) / parts);
       const int64_t blocks = w.blocks(part);
       // (The partials that are written: the others' slots are left alone.)
@@ -312,8 +323,8 @@ mvr::ScoreAttentionPlan plan_scored(const mvr_paged_attention_args* a, const mvr
     for (int64_t parts = 2; tile.rows == 16 && parts * w.tiles < cus && parts < std::min<int64_t>(w.longest, mvr::kScoreMaxParts);
          parts += (parts + 1) / 2)
       take_split((w.longest + parts - 1) / parts);
-    // Where a workspace is too small for all of these, the fewest parts that fit.
-    if (limit != SIZE_MAX && best.parts <= 1)
+    // Where a workspace is too small for these, the fewest parts that fit.
+    if (too_large && best.parts <= 1)
       for (int64_t parts = 2; parts <= 8; parts++) take_split((w.longest + parts - 1) / parts);
   }
   return best;

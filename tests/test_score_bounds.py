@@ -1,9 +1,12 @@
 """Sizes at which the calls on scores are accepted or refused, on the CPU: nothing is launched."""
+import ctypes
+
+import numpy as np
 import pytest
 
 import mvr_attn as M
 import mvr_score as S
-from test_score_api import move_args, select_args
+from test_score_api import move_args, scored_args, select_args
 
 
 def refused(validate, *args, text, code=M.MVR_E_UNSUPPORTED):
@@ -28,3 +31,33 @@ def test_most_moves_of_a_row():
     S.validate_move(move_args(max_moves=2 ** 31 - 1 - 2 ** 23))
     for n in (2 ** 31 - 2 ** 23, 2 ** 31 - 1):
         refused(S.validate_move, move_args(max_moves=n), text="too close to 2^31")
+
+
+def workspace(q, keys, total=True, **kw):
+    """Bytes that a call asks for whose requests have these new tokens and keys, its host tables given."""
+    seq, cu = np.array(keys, np.int32), np.concatenate([[0], np.cumsum(q)]).astype(np.int32)
+    sizes = dict(num_seqs=len(q), max_q_len=int(max(q)), max_seq_len=int(max(keys)), max_pages_per_seq=1 << 14,
+                 total_q=int(cu[-1]) if total else 0, lse_stride_head=int(cu[-1]), q_stride_head=1 << 28,
+                 seq_lens_host=seq.ctypes.data, cu_q_lens_host=cu.ctypes.data, num_q_heads=28, num_kv_heads=4)
+    refs = [ctypes.byref(x) for x in scored_args(**{**sizes, **kw})]
+    return S.load_library().mvr_paged_attention_scored_workspace_size(*refs)
+
+
+def test_a_split_never_asks_for_more_than_its_budget():
+    """Partial results hold a slot for every part of every place, also where few row tiles have so many parts."""
+    budget = 96 << 20
+    for dtype in (M.DTYPE_F16, M.DTYPE_F32):
+        for total in (True, False):
+            prompt = [2509] + [1] * 190
+            assert workspace(prompt, [2518] * 191, total, dtype=dtype) <= budget
+            for q, keys in (([2131, 1], [34602] * 2), ([1024, 1024], [34602] * 2), ([1] * 63 + [2000], [2000] * 64)):
+                assert workspace(q, keys, total, dtype=dtype) <= budget, (q, total)
+            rng = np.random.default_rng(5)
+            for _ in range(300):
+                q = rng.integers(0, int(2 ** rng.uniform(1, 12)), rng.integers(1, 200)) + (rng.random() < 0.5)
+                keys = q + rng.integers(0, int(2 ** rng.uniform(1, 16)), len(q))
+                q[0] += not q.any()
+                heads = rng.choice([1, 2, 8])
+                assert workspace(q, np.maximum(keys, q), total, dtype=dtype, num_kv_heads=heads, num_q_heads=heads * rng.integers(1, 9),
+                                 head_dim=int(rng.choice([32, 64, 128, 256]))) <= budget
+    assert workspace([1] * 4, [30000] * 4) > 0  # (and calls are split)
