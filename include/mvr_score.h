@@ -74,6 +74,9 @@ typedef struct mvr_score_rules {
      - rows of q, out and lse from cu_q_lens[num_seqs] on are neither read nor
        written;
      - a device q_len above max_q_len is clamped to it;
+     - a launch holds 2^24 tiles of 16 rows (a row: a query token and a query head of
+       its KV head's group), or up to an eighth less: calls of more are refused, counted by
+       total_q where it and cu_q_lens are given, else by max_q_len for every request;
      - a NaN or an infinity in the K or V row of a key reaches only the rows that
        see the key.
    Host tables (seq_lens_host, cu_q_lens_host) and sum_seq_lens only shape the

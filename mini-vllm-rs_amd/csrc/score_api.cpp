@@ -66,11 +66,45 @@ int check_scored(const mvr_paged_attention_args* a, const mvr_score_rules* r) {
   // The kernels count a page's rows, a head's rows and work items in 32 bits.
   if (a->num_pages > INT32_MAX || (int64_t)a->num_kv_heads * a->page_size > INT32_MAX)
     return fail(MVR_E_UNSUPPORTED, "pools of over 2^31 pages, or pages of over 2^31 rows");
+  if ((int64_t)(a->num_q_heads / a->num_kv_heads) * a->max_q_len > INT32_MAX - 1024)
+    return fail(MVR_E_UNSUPPORTED, "requests of %d tokens are more than one call takes", a->max_q_len);
+  return MVR_OK;
+}
+
+// Places for row tiles: those of the longest request for every request; packed, as many as
+// the packed tokens have and one more of each request, whose owner a block finds by a
+// search of cu_q_lens: where that leaves half of the places out, or a launch could not
+// hold them.  (63 single tokens and 2,000 new ones on 2,000 keys each, F16: 112 us packed
+// and 151 padded for 28/4 heads, 43 and 125 for 7/1; ten batches whose lengths vary less,
+// 0.82 to 1.07 times.)
+struct Places {
+  int64_t groups, row_tiles, padded; // (padded: row tiles of the longest request)
+  bool packed;
+};
+
+bool one_launch(int64_t groups, int64_t inner, int waves) {
+  const int64_t blocks = kMaxThreads / (64 * waves);
+  return inner <= blocks / groups && mvr::score_grid(groups, inner) <= blocks;
+}
+
+Places places_of(const mvr_paged_attention_args* a, int tile_rows, int waves) {
   const int64_t group = a->num_q_heads / a->num_kv_heads;
-  const int64_t pairs = (int64_t)a->num_seqs * a->num_kv_heads + mvr::kScoreXcds - 1;
-  const int64_t tiles = pairs * ((group * a->max_q_len + 15) / 16);
-  if (group * a->max_q_len > INT32_MAX - 1024 || tiles > kMaxThreads / 512 / 2)
-    return fail(MVR_E_UNSUPPORTED, "%d requests of %d tokens are more than one call takes", a->num_seqs, a->max_q_len);
+  const int64_t padded = (group * a->max_q_len + tile_rows - 1) / tile_rows, all = mvr::score_groups(false, a->num_seqs, a->num_kv_heads);
+  const int64_t tokens = a->total_q > 0 ? a->total_q : (int64_t)a->num_seqs * a->max_q_len;
+  const int64_t in_all = group * tokens / tile_rows + a->num_seqs;
+  if (a->cu_q_lens && (2 * in_all <= padded * a->num_seqs || !one_launch(all, padded, waves)))
+    return {mvr::score_groups(true, a->num_seqs, a->num_kv_heads), in_all, padded, true};
+  return {all, padded, padded, false};
+}
+
+// The checks of the attention call.
+int check_attention(const mvr_paged_attention_args* a, const mvr_score_rules* r) {
+  const int rc = check_scored(a, r);
+  if (rc != MVR_OK) return rc;
+  const Places x = places_of(a, 16, 4);
+  if (!one_launch(x.groups, x.row_tiles, 4))
+    return fail(MVR_E_UNSUPPORTED, "%d requests of up to %d tokens (%d in all; 0: not given) are more than one call takes",
+                a->num_seqs, a->max_q_len, a->total_q);
   return MVR_OK;
 }
 
@@ -241,29 +275,24 @@ mvr::ScoreAttentionPlan plan_scored(const mvr_paged_attention_args* a, const mvr
   static const int set_waves = env_int("MVR_SCORE_TILE_WAVES", 4);
   static const int set_units = env_int("MVR_SCORE_PART_UNITS", 0);
   bool rows_set = false;
+  auto runs = [&](const TileCost& tile, const Places& x) {
+    return mvr::score_tile_supported(tile.rows, tile.waves, a->head_dim) && one_launch(x.groups, x.row_tiles, tile.waves);
+  };
   for (const TileCost& tile : kF16Costs)
-    rows_set |= tile.rows == set_rows && tile.waves == set_waves && mvr::score_tile_supported(set_rows, set_waves, a->head_dim);
+    rows_set |= tile.rows == set_rows && tile.waves == set_waves && runs(tile, places_of(a, tile.rows, tile.waves));
   mvr::ScoreAttentionPlan best{};
   double best_cost = INFINITY;
   for (const TileCost& tile : f16 ? kF16Costs : kF32Costs) {
-    if (!mvr::score_tile_supported(tile.rows, tile.waves, a->head_dim)) continue;
+    const Places x = places_of(a, tile.rows, tile.waves);
+    if (!runs(tile, x)) continue; // (16 rows do: check_attention)
     // (A tile that no request fills half costs what the smaller one does, or more.)
     if (rows_set ? tile.rows != set_rows || tile.waves != set_waves : longest_rows <= tile.rows / 2 && best_cost < INFINITY) continue;
     const int held = mvr::score_blocks_per_cu(tile.rows, tile.waves, f16, a->head_dim);
     const TileWork w(a, r, tile.rows);
-    // Places for the longest request's row tiles of every request; packed, for as many as
-    // the packed tokens have and one more of each request, whose owner a block finds by a
-    // search of cu_q_lens: where that leaves half of the places out.  (63 single tokens and
-    // 2,000 new ones on 2,000 keys each, F16: 112 us packed and 151 padded for 28/4 heads,
-    // 43 and 125 for 7/1; ten batches whose lengths vary less, 0.82 to 1.07 times.)
-    const int64_t padded = (longest_rows + tile.rows - 1) / tile.rows;
-    const int64_t in_all = group * (a->total_q > 0 ? a->total_q : (int64_t)a->num_seqs * a->max_q_len) / tile.rows + a->num_seqs;
-    const bool packed = a->cu_q_lens && 2 * in_all <= padded * a->num_seqs;
-    const int64_t row_tiles = packed ? in_all : padded;
-    const int64_t groups = mvr::score_groups(packed, a->num_seqs, a->num_kv_heads), all_tiles = groups * row_tiles;
+    const int64_t groups = x.groups, row_tiles = x.row_tiles, all_tiles = groups * row_tiles;
     const double unit_scale = (tile.own + (1 - tile.own) * a->head_dim / 128.0) * (r->cap > 0.f ? tile.capped : 1.0);
     // (Row tiles of one KV head read the same keys, which the caches keep.)
-    const double hbm = (double)w.units / std::max<int64_t>(1, padded) *
+    const double hbm = (double)w.units / std::max<int64_t>(1, x.padded) *
                        (2.0 * mvr::kScoreUnitTokens * a->head_dim * es_of(a->dtype) / 5.9e6);
     auto cost_of = [&](int64_t blocks, double longest) { // of `longest` units at most
       double body;
@@ -280,7 +309,7 @@ mvr::ScoreAttentionPlan plan_scored(const mvr_paged_attention_args* a, const mvr
       best.tile_rows = tile.rows;
       best.waves = tile.waves;
       best.row_tiles = (int)row_tiles;
-      best.packed = packed;
+      best.packed = x.packed;
       best.parts = (int)parts;
       best.part_units = (int)std::min<int64_t>(part_units, INT32_MAX / 2); // (units are added to it)
       best.partial_bytes = bytes;
@@ -288,7 +317,7 @@ mvr::ScoreAttentionPlan plan_scored(const mvr_paged_attention_args* a, const mvr
     bool too_large = false;
     auto take_split = [&](int64_t part) { // parts of `part` units
       const int64_t parts = std::min<int64_t>((w.longest + part - 1) / part, mvr::kScoreMaxParts);
-      if (parts < 2 || 2 * parts > kMaxThreads / (64 * tile.waves) / ((groups + mvr::kScoreXcds) * row_tiles)) return;
+      if (parts < 2 || !one_launch(groups, row_tiles * parts, tile.waves)) return;
       if (all_tiles > kMaxThreads / (tile.rows * a->head_dim / 4 + 256)) return; // (the merge's)
       const int64_t rows = all_tiles * parts * tile.rows;
       const size_t bytes = align_up((size_t)rows * a->head_dim * sizeof(float), 256) +
@@ -405,7 +434,7 @@ int validate_scored(const mvr_paged_attention_args* a, const int32_t* block_tabl
 extern "C" {
 
 size_t mvr_paged_attention_scored_workspace_size(const mvr_paged_attention_args* a, const mvr_score_rules* r) {
-  if (check_scored(a, r) != MVR_OK) return 0;
+  if (check_attention(a, r) != MVR_OK) return 0;
   return plan_scored(a, r, SIZE_MAX).partial_bytes;
 }
 
@@ -414,7 +443,7 @@ int mvr_paged_attention_scored_validate(const mvr_paged_attention_args* a, const
                                         const int32_t* cu_q_lens_host, const int32_t* first_keys_host,
                                         const int32_t* prefix_lens_host, const float* slopes_host) {
   clear_error();
-  const int rc = check_scored(a, r);
+  const int rc = check_attention(a, r);
   if (rc != MVR_OK) return rc;
   return validate_scored(a, block_tables_host, seq_lens_host, cu_q_lens_host, first_keys_host, prefix_lens_host,
                          slopes_host);
@@ -423,7 +452,7 @@ int mvr_paged_attention_scored_validate(const mvr_paged_attention_args* a, const
 int mvr_paged_attention_scored(const mvr_paged_attention_args* a, const mvr_score_rules* r) {
   Range range("attn"); // trace.rs:64
   clear_error();
-  int rc = check_scored(a, r);
+  int rc = check_attention(a, r);
   if (rc != MVR_OK) return rc;
   if (checked()) {
     rc = run_checked([&] {
@@ -450,7 +479,7 @@ int mvr_paged_attention_scored(const mvr_paged_attention_args* a, const mvr_scor
   p.parts = plan.parts;
   p.part_units = plan.part_units;
   const int64_t groups = mvr::score_groups(plan.packed, a->num_seqs, a->num_kv_heads);
-  p.run = mvr::score_run(plan, groups);
+  p.run = (int)mvr::score_run(groups, (int64_t)plan.row_tiles * plan.parts);
   if (plan.parts > 1) {
     const size_t rows = (size_t)groups * plan.row_tiles * plan.parts * plan.tile_rows;
     char* at = static_cast<char*>(a->workspace);

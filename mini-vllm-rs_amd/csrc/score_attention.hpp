@@ -118,18 +118,20 @@ inline int64_t score_groups(bool packed, int64_t num_seqs, int64_t num_kv_heads)
   return packed ? num_kv_heads : num_seqs * num_kv_heads;
 }
 
-// Items that follow each other on one XCD: a group's, where the groups share out evenly;
-// else fewer, for some eight runs on each.
-inline int score_run(const ScoreAttentionPlan& plan, int64_t groups) {
-  const int64_t inner = (int64_t)plan.row_tiles * plan.parts;
-  return (int)(groups % kScoreXcds == 0 ? inner : std::max<int64_t>(1, std::min(inner, groups * inner / (8 * kScoreXcds))));
+// Items that follow each other on one XCD: a group's `inner` ones, where the groups share
+// out evenly; else fewer, for some eight runs on each.
+inline int64_t score_run(int64_t groups, int64_t inner) {
+  return groups % kScoreXcds == 0 ? inner : std::max<int64_t>(1, std::min(inner, groups * inner / (8 * kScoreXcds)));
 }
 
-// Blocks of one launch.
+// Blocks of one launch: whole rounds of runs.
+inline int64_t score_grid(int64_t groups, int64_t inner) {
+  const int64_t round = kScoreXcds * score_run(groups, inner);
+  return (groups * inner + round - 1) / round * round;
+}
+
 inline unsigned score_blocks(const ScoreAttentionParams& p) {
-  const int64_t items = score_groups(p.packed, p.t.num_seqs, p.t.num_kv_heads) * p.row_tiles * p.parts;
-  const int64_t round = (int64_t)kScoreXcds * p.run; // whole rounds of runs
-  return (unsigned)((items + round - 1) / round * round);
+  return (unsigned)score_grid(score_groups(p.packed, p.t.num_seqs, p.t.num_kv_heads), (int64_t)p.row_tiles * p.parts);
 }
 
 // score_tiles.hip: the attention itself, of row tiles of 64 (head_dim up to 128) and 128

@@ -6,7 +6,7 @@ import pytest
 
 import mvr_attn as M
 import mvr_score as S
-from test_score_api import move_args, scored_args, select_args
+from test_score_api import move_args, scored_args, select_args, weights_args
 
 
 def refused(validate, *args, text, code=M.MVR_E_UNSUPPORTED):
@@ -61,3 +61,27 @@ def test_a_split_never_asks_for_more_than_its_budget():
                 assert workspace(q, np.maximum(keys, q), total, dtype=dtype, num_kv_heads=heads, num_q_heads=heads * rng.integers(1, 9),
                                  head_dim=int(rng.choice([32, 64, 128, 256]))) <= budget
     assert workspace([1] * 4, [30000] * 4) > 0  # (and calls are split)
+
+
+def mixed(num_seqs, longest, **kw):
+    """One prompt among single tokens."""
+    return dict(num_seqs=num_seqs, max_q_len=longest, max_seq_len=max(longest, 64), max_pages_per_seq=1 << 12,
+                total_q=num_seqs - 1 + longest, lse_stride_head=1 << 24, q_stride_head=1 << 28, **kw)
+
+
+@pytest.mark.parametrize("num_seqs,longest", [(256, 8192), (512, 4096), (1024, 2048), (4000, 32768), (65536, 4)])
+def test_mixed_batches_count_the_tokens_that_are_there(num_seqs, longest):
+    """Accepted as mvr_paged_attention accepts them, whatever the longest request would take in every place."""
+    S.validate_scored(*scored_args(**mixed(num_seqs, longest)))
+    S.validate_weights(*weights_args(**mixed(num_seqs, longest)))
+
+
+def test_most_row_tiles_of_a_call():
+    """2^24 blocks of 256 threads: by max_q_len where the tokens are not known."""
+    sizes = dict(num_q_heads=16, num_kv_heads=1)  # a tile per token
+    for total in (0, 1 << 24):
+        S.validate_scored(*scored_args(**{**mixed(2040, 8192, **sizes), "total_q": 0}))
+        refused(S.validate_scored, *scored_args(**{**mixed(2049, 8192, **sizes), "total_q": total}), text="more than one call takes")
+    S.validate_scored(*scored_args(**{**mixed(2049, 8192, **sizes), "total_q": 1 << 23}))
+    weights = weights_args(**{**mixed(2049, 8192, **sizes), "total_q": 0})
+    S.validate_weights(*weights)  # whose blocks are those of the keys
