@@ -78,9 +78,11 @@ typedef struct mvr_score_rules {
        its KV head's group), or up to an eighth less: calls of more are refused, counted by
        total_q where it and cu_q_lens are given, else by max_q_len for every request;
      - a NaN or an infinity in the K or V row of a key reaches only the rows that
-       see the key.
+       see the key.  An infinity in a V row may come out of those as an infinity or as a
+       NaN (it is multiplied by a probability in parts, which may be 0): which of them is
+       the plan's, and may change with the hints.
    Host tables (seq_lens_host, cu_q_lens_host) and sum_seq_lens only shape the
-   launch; rows are computed from the device tables whatever they hold. */
+   launch, and with it the order of sums and the rounding of probabilities; rows are computed from the device tables whatever they hold. */
 int mvr_paged_attention_scored(const mvr_paged_attention_args* args, const mvr_score_rules* rules);
 
 /* Bytes of workspace that the call needs (0: none; 96 MiB at most; contents need no
