@@ -49,8 +49,9 @@ extern "C" {
      s = scale * q . k_j,   s = cap * tanh(s / cap),   s - slopes[h] * |p - j|.
    Distances and windows count cache slots: after a cut, whose moves change the
    order, only the cap and masks that end before the moved slots mean what they say.
-   A query that sees no key, as those of a request of length 0, has output 0 and
-   log-sum-exp -infinity. */
+   A query that sees no key has output 0 and log-sum-exp -infinity; so have those in
+   slots below 0, of requests shorter than their query tokens (length 0 among them),
+   which the checks refuse. */
 typedef struct mvr_score_rules {
   float cap;                  /* > 0; 0: scores are not capped */
   int32_t window;             /* keys that a query sees at most, up to itself; 0: any number */
@@ -68,7 +69,8 @@ typedef struct mvr_score_rules {
    hints.  Scores, softmax state and sums are held in 32 bits.  F16 probabilities
    enter the product with V with 20 bits, and calls of many rows round them to F16 for
    it (in steps of 2^-31 of a row's largest, where they are that small), not for the
-   sum that divides them.  Differences to mvr_paged_attention:
+   sum that divides them: their outputs are up to 1.4 times as far from the formula.
+   A cap adds an error of 2^-20 of the capped score at most.  Differences to mvr_paged_attention:
      - a request may have q_len 0: nothing is computed for it, so total_q, where
        given, lies in [0, num_seqs * max_q_len];
      - rows of q, out and lse from cu_q_lens[num_seqs] on are neither read nor

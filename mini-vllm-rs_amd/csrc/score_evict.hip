@@ -20,8 +20,8 @@ constexpr int kWave = 64;
 // Which tokens stay: a block per (layer, request, KV head).
 //
 // Ranks become a search for one number.  A token's key is 2^32 - 1 where it is
-// protected, else its weight's bits in an order that ascends with the weight (0 for a
-// NaN, as for -infinity).  The keep-th largest key T is found digit by digit from the
+// protected, else its weight's bits in an order that ascends with the weight (a NaN's is
+// -infinity's; 0, below all, for tokens in pages outside the pool).  The keep-th largest key T is found digit by digit from the
 // top, with a histogram of the digit of the keys that share the digits found before;
 // tokens above T stay, and of those at T the lowest slots, as many as are missing.  What
 // stays past slot `keep` and what goes below it are as many, and are paired in ascending
@@ -306,8 +306,9 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_tokens_kernel(Select
 // look up the pages of all their slots at once, then share the rows' vectors out among
 // them, a batch of K and V in flight together.  No slot is both a source and a target,
 // so rows move in any order.  Bound by HBM where there are many: 180,000 rows of 256
-// bytes of K and V in random pages 47.4 us, 3.9 TB/s read and written (a large copy: 5.1);
-// 8 vectors to a batch 49.5, 16 moves to a wavefront 48.6.
+// bytes of K and V in random pages 47.2 us, 3.9 TB/s read and written (a large copy: 5.1);
+// 16 moves to a wavefront 48.1 (rows of 128 and 512 bytes 22.4 and 45.8, with 16 22.9 and
+// 46.5), 8 vectors to a batch 49.5.
 // ---------------------------------------------------------------------------
 constexpr int kMoveThreads = 256, kMoveWaves = kMoveThreads / kWave;
 constexpr int kWaveMoves = kWave / 2;

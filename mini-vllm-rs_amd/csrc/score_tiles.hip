@@ -24,7 +24,8 @@
 // them, in 4 wavefronts, two blocks to a CU, or in 8, one, where blocks are fewer than
 // CUs.  32/8 heads of 128 F16, unsplit, 64 rows, 128, 128 in 8 wavefronts: 32 requests of
 // 16 tokens on 4,000 102, 107 and 100 us (16 rows streamed: 179); a prompt of 2,000 57, 59
-// and 57 (170); documents of 1,500 in a prompt of 6,000 178, 163 and 183.
+// and 57 (170); documents of 1,500 in a prompt of 6,000 178, 163 and 183 (163 to 172 in 128 on other
+// days).
 #include "key_tiles.hpp"
 #include "score_common.hpp"
 
@@ -261,8 +262,13 @@ __global__ __launch_bounds__(kWaveSize* W, (score_tile_waves_per_simd(32 * RW, W
   // In block c the lane holds tokens 32 c + 8 (e / 4) + 4 hh + e % 4 of its row.
   // Scores less the running maximum (log2 units), which moves, and O and the sum with it,
   // only where a score exceeds it by enough; then P = 2^x in place, and its sum.
-  // F16: the product with V takes P rounded to F16 (half a step, 2^-11 of p; a second
-  // product for what the rounding leaves would cost a quarter), the sum holds 32 bits.
+  // F16: the product with V takes P rounded to F16 (half a step, 2^-11 of p), the sum
+  // holds 32 bits.  Outputs are 1.4 times as far from the formula as with all of P (2.9e-4
+  // of them against 2.1e-4, the rounding of the output itself).  A second product, with
+  // what the rounding leaves, is the matrix pipe's half again: four of 256 on 2,048 with a
+  // cap 57.5 -> 65.1 us, documents 163 -> 193, a prompt of 8,192 537 -> 711 (interleaved
+  // with the exponentials 704), 32 requests of 16 tokens on 4,000 102 -> 104.  The
+  // streaming kernel, bound by HBM, has it.
   auto softmax = [&](float16v (&sc)[kSub], int first, bool masked) __attribute__((always_inline)) { // first: the tile's first key
     float x[16 * kSub];
 #pragma unroll
