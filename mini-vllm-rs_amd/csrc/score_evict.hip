@@ -21,11 +21,11 @@ constexpr int kWave = 64;
 //
 // Ranks become a search for one number.  A token's key is 2^32 - 1 where it is
 // protected, else its weight's bits in an order that ascends with the weight (a NaN's is
-// -infinity's; 0, below all, for tokens in pages outside the pool).  The keep-th largest key T is found digit by digit from the
-// top, with a histogram of the digit of the keys that share the digits found before;
-// tokens above T stay, and of those at T the lowest slots, as many as are missing.  What
-// stays past slot `keep` and what goes below it are as many, and are paired in ascending
-// order.
+// -infinity's; 0, below all, for tokens in pages outside the pool).  The keep-th largest
+// key T is found digit by digit from the top, with a histogram of the digit of the keys
+// that share the digits found before; tokens above T stay, and of those at T the lowest
+// slots, as many as are missing.  What stays past slot `keep` and what goes below it are
+// as many, and are paired in ascending order.
 //
 // The weights are read once, and their keys held in LDS for the passes over them; a
 // thread takes four slots at a time, with one 16-byte access each to weights, positions

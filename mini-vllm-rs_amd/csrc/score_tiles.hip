@@ -24,8 +24,8 @@
 // them, in 4 wavefronts, two blocks to a CU, or in 8, one, where blocks are fewer than
 // CUs.  32/8 heads of 128 F16, unsplit, 64 rows, 128, 128 in 8 wavefronts: 32 requests of
 // 16 tokens on 4,000 102, 107 and 100 us (16 rows streamed: 179); a prompt of 2,000 57, 59
-// and 57 (170); documents of 1,500 in a prompt of 6,000 178, 163 and 183 (163 to 172 in 128 on other
-// days).
+// and 57 (170); documents of 1,500 in a prompt of 6,000 178, 163 and 183 (163 to 172 in 128
+// on other days).
 #include "key_tiles.hpp"
 #include "score_common.hpp"
 
